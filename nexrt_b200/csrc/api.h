@@ -205,6 +205,35 @@ int nexrt_tc_oproj_allreduce(const void* planes, const void* descale, const void
 int nexrt_attn_front_tail(const void* pre, const void* ctl, void* q_raw, void* gate, void* k_raw, void* v_cache, int hd, int nq, int ngate, int kvh, int M,
                           int cache_len, int ksplit, void* stream);   /* pre: [ksplit][M][R] partial planes of a chunk's GEMM */
 
+// ---- a key-value cache in pages, shared by several sequences (rope.cu, paged_attn.cu, pages.cu) -------------------------
+// Pools: [pages][kv heads][slots][dim], one for K and one for V of every layer; table: int32 [rows][width], -1 where there is no page.
+// Types: 0 bf16, 1 fp16, 2 fp32.  A bad page or row is left out and latches kStatusBadPage in `status` (may be NULL).
+int nexrt_rope_append(const void* q, const void* k, const void* v, const void* positions, const void* rows, void* q_out, void* k_out, void* v_out,
+                      const void* table, const void* inv_freq, const void* q_norm, const void* k_norm, void* status, const int64_t* strides, int tokens, int q_heads,
+                      int kv_heads, int dim, int rotary, int interleaved, int table_rows, int width, int page, int pages, int in_type, int out_type, float scale,
+                      float eps, void* stream);   /* table NULL: k goes to k_out, v is not used; strides: (token, head) of q, k, v, q_out, (page, head, slot) of the pools, row of the table */
+int nexrt_paged_ctas(int seqs, int q_heads, int kv_heads, int width, int page, int window);   /* CTAs of a call: its scratch is 2 * that * 16 * (dim + 2) floats */
+int nexrt_paged_attn(const void* q, const void* k_pages, const void* v_pages, const void* table, const void* lens, const void* slopes, void* out, void* lse,
+                     void* scratch, void* status, const int64_t* strides, int seqs, int q_heads, int kv_heads, int dim, int width, int page, int pages, int window,
+                     int type, float scale, float softcap, int ctas, void* stream);   /* strides: (sequence, head) of q and out, (page, head, slot) of the pools, rows of the table and of lse */
+int64_t nexrt_paged_slot(const int* table, int64_t stride, int rows, int width, int page, int pages, int row, int pos);   /* host: slot of the pool that holds a position, or -1 */
+int nexrt_paged_split(const int* lens, int seqs, int items, int64_t room, int window, int grid, int64_t* out, int most);   /* host: how the keys are split over CTAs */
+int nexrt_page_fork(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* table, int64_t table_stride, int rows, int width,
+                    const void* lens, const void* parents, const void* grow, int grow_all, void* table_out, int64_t out_stride, void* lens_out, void* refs,
+                    void* scratch, void* status, int rows_out, void* stream);   /* scratch: int[pages + 3 rows_out] */
+int nexrt_page_compact(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* table, int64_t table_stride, int rows, int width,
+                       const void* lens, void* table_out, int64_t out_stride, void* refs_out, void* remap, void* live, void* scratch, void* status,
+                       void* stream);   /* scratch: int[5 pages + 1] */
+int nexrt_page_copy(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* src, const void* dst, int n, void* scratch, void* status,
+                    void* stream);   /* scratch: int[3 n] */
+
+// ---- beam search (beam.cu) ------------------------------------------------------------------------------------------------
+int nexrt_beam_slices(int vocab);   /* a call's scratch is batch * beams * slices * (k + 2) words of 8 bytes */
+int nexrt_beam_select(const void* logits, const void* scores, const void* finished, const int64_t* strides, void* scores_out, void* rows_out, void* tokens_out,
+                      void* scratch, void* status, int batch, int beams, int vocab, int k, int eos, int type, void* stream);   /* k <= 64, beams <= 256 */
+int nexrt_reorder_rows(const void* const* in, void* const* out, const int64_t* meta, int tensors, const void* rows, int64_t r_0, int64_t r_1, int cols, int n,
+                       int n_in, void* status, void* stream);   /* out[t][i] = in[t][rows[i]], at most 16 tensors */
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,6 +27,9 @@ enum Status : int {
     kStatusCpTimeout = 4,       // context-parallel partial did not arrive
     kStatusBadToken = 5,        // token id outside the vocabulary
     kStatusPipeTimeout = 6,     // an mbarrier / TMA / tensor-core completion did not arrive
+    kStatusBadPage = 7,         // a page table, a list of pages or a list of rows names something that does not exist
+    kStatusNoPages = 8,         // the pool has no free page, or the table no column, for a row that should grow
+    kStatusPageConflict = 9,    // a list of copies names a page as both source and target, or as target twice
 };
 
 // Control block shared by all three decode modes (int32[32]).  Python mirror: runtime/control.py.

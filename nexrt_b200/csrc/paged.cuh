@@ -1,0 +1,53 @@
+// A key-value cache in pages: pool [pages][kv heads][slots of a page][head dim] for K and for V, and a table that names the
+// pages of every sequence.  The index arithmetic that the kernels share, as host and device functions: the host forms are what
+// the CPU tests run (nexrt_paged_slot, nexrt_paged_split).
+#pragma once
+
+#include "common.cuh"
+
+namespace nexrt {
+
+struct PageTable {
+    const int* table;    // [rows][width]: page of positions [page * j, page * (j + 1)) of a row, -1: none
+    int64_t stride;      // ints between two rows
+    int rows, width;
+    int page;            // slots of a page
+    int pages;           // pages of the pool
+};
+
+// Entry `j` of a row's pages, or -1 where it names no page of the pool.
+__host__ __device__ __forceinline__ int page_at(const PageTable& t, int row, int j) {
+    if (row < 0 || row >= t.rows || j < 0 || j >= t.width) return -1;
+    const int p = t.table[row * t.stride + j];
+    return p >= 0 && p < t.pages ? p : -1;
+}
+
+// Slot of the pool (page * slots + slot) that holds position `pos` of `row`, or -1.
+__host__ __device__ __forceinline__ int64_t page_slot(const PageTable& t, int row, int pos) {
+    if (pos < 0) return -1;
+    const int j = pos / t.page, p = page_at(t, row, j);
+    return p < 0 ? -1 : static_cast<int64_t>(p) * t.page + (pos - j * t.page);
+}
+
+// Pages that `len` positions take.
+__host__ __device__ __forceinline__ int pages_of(int len, int page) { return len <= 0 ? 0 : (len - 1) / page + 1; }
+
+// ---- the split of a batch's keys over the CTAs of the attention kernel ------------------------------------------------
+// Work is counted in chunks of kChunk keys of one (sequence, kv head, head group): `total` of them in the order sequence,
+// head, chunk.  CTA c of n takes chunks [total c / n, total (c + 1) / n), so all CTAs have the same work whatever the lengths.
+constexpr int kChunk = 64;
+
+// Keys [lo, hi) that the query behind the last of `len` keys sees; `room` keys have a place in the table.
+__host__ __device__ __forceinline__ void key_span(int len, int64_t room, int window, int& lo, int& hi) {
+    hi = len < 0 ? 0 : (len > room ? static_cast<int>(room) : len);
+    lo = window > 0 && hi > window ? hi - window : 0;
+}
+__host__ __device__ __forceinline__ int chunks_of(int lo, int hi) { return hi <= lo ? 0 : (hi - 1) / kChunk - lo / kChunk + 1; }
+
+__host__ __device__ __forceinline__ int64_t range_begin(int64_t total, int c, int n) { return total * c / n; }
+// The CTA whose range holds chunk x: the largest c with total c / n <= x.
+__host__ __device__ __forceinline__ int owner_of(int64_t x, int64_t total, int n) { return static_cast<int>((n * (x + 1) - 1) / total); }
+// CTAs that get work: at most `grid`, no more than there are chunks.
+__host__ __device__ __forceinline__ int active_ctas(int64_t total, int grid) { return total < grid ? (total > 0 ? static_cast<int>(total) : 1) : grid; }
+
+}  // namespace nexrt

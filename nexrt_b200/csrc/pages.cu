@@ -1,0 +1,454 @@
+// Pages of a shared key-value cache: rows of a table are continued, forked and freed, the pages they share are counted, a
+// begun page that is about to be written is copied, live pages are moved to the front of the pool.
+//
+// Everything is planned on the device, so that a beam-search step needs no word from the host and can be captured: a grid
+// copies and counts the table (integer atomics: the order does not show), one CTA plans (what is ordered - which row copies,
+// which page is free next - is a prefix sum over rows or pages), a grid moves the bytes.  Free pages are those that no row of
+// the table names; the lowest go first, to the rows in their order.
+//
+// Bound by the bytes of the copied pages; for a table without copies by the launches and the plan's few round trips.
+#include "api.h"
+#include "paged.cuh"
+
+namespace nexrt {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanRows = 4096;         // rows whose plan one CTA holds in shared memory
+constexpr int kPagesPerThread = 8;
+
+// Sum of `v` over the threads before this one; `total` gets the sum over all.  red: 33 ints.
+__device__ __forceinline__ int block_prefix(int v, int* red, int& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += n;
+    }
+    __syncthreads();
+    if (lane == 31) red[warp] = s;
+    __syncthreads();
+    if (warp == 0) {
+        int w = lane < static_cast<int>(blockDim.x >> 5) ? red[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int n = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += n;
+        }
+        red[lane] = w;
+    }
+    __syncthreads();
+    total = red[31];
+    return s - v + (warp ? red[warp - 1] : 0);
+}
+
+__device__ __forceinline__ void latch(int* status, Status code) {
+    if (status) atomicCAS(status, 0, static_cast<int>(code));
+}
+
+// Positions of old row p that a new row takes over: what has a place in the table.
+__device__ __forceinline__ int kept_len(const PageTable& t, const int* lens, int p) {
+    if (p < 0 || p >= t.rows) return 0;
+    const int64_t room = static_cast<int64_t>(t.width) * t.page;
+    const int n = lens[p];
+    return n < 0 ? 0 : (n > room ? static_cast<int>(room) : n);
+}
+
+// new table[r] = old table[parents[r]] (-1 behind its last page), refs[page] = rows that name it.  refs comes in as zero.
+__global__ void __launch_bounds__(256) fork_rows_kernel(PageTable t, const int* lens, const int* parents, int* out, int64_t out_stride, int* refs, int n,
+                                                        int* status) {
+    pdl_launch_dependents();
+    pdl_wait();
+    for (int r = blockIdx.y; r < n; r += gridDim.y) {
+        const int p = parents ? parents[r] : r;
+        if (threadIdx.x == 0 && blockIdx.x == 0 && (p >= t.rows || (p >= 0 && lens[p] > static_cast<int64_t>(t.width) * t.page))) latch(status, kStatusBadPage);
+        const int used = pages_of(kept_len(t, lens, p), t.page);
+        for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < t.width; j += gridDim.x * blockDim.x) {
+            int page = -1;
+            if (j < used) {
+                page = page_at(t, p, j);
+                if (page < 0) latch(status, kStatusBadPage);
+                else atomicAdd(refs + page, 1);
+            }
+            if (out) out[r * out_stride + j] = page;
+        }
+    }
+}
+
+struct ForkPlan {
+    PageTable t;                // the old table
+    const int *lens, *parents, *grow;
+    int* table;                 // the new one, as fork_rows_kernel left it
+    int64_t table_stride;
+    int *lens_out, *refs;
+    int* copies;                // [n][3]: source page, target page, positions to copy (0: none)
+    int* free_list;             // [pages] scratch
+    int* status;
+    int n, grow_all, pages;
+};
+
+// One CTA.  A row with g more positions needs pages for them, and, if it goes on writing in a begun page that other rows hold
+// too, a copy of that page.  Where all holders of the page go on writing, the first of them keeps it.
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkPlan a) {
+    extern __shared__ int plan_smem[];
+    int* const last = plan_smem;             // [n] begun page that the row writes in, -1: none
+    int* const fresh = last + a.n;           // [n] pages that the row takes; bit 30: the first of them is a copy
+    __shared__ int red[33];
+    pdl_launch_dependents();
+    pdl_wait();
+    constexpr int kCopy = 1 << 30;
+    for (int r = threadIdx.x; r < a.n; r += blockDim.x) {
+        const int p = a.parents[r], len = kept_len(a.t, a.lens, p);
+        const bool alive = p >= 0 && p < a.t.rows;
+        int g = alive ? (a.grow ? a.grow[r] : a.grow_all) : 0;
+        if (g < 0) g = 0;
+        const int used = pages_of(len, a.t.page);
+        int want = 0, open = -1;
+        if (g > 0) {
+            if (static_cast<int64_t>(len) + g > static_cast<int64_t>(a.t.width) * a.t.page) {
+                latch(a.status, kStatusNoPages);
+                g = 0;
+            } else if (len % a.t.page) {
+                open = a.table[r * a.table_stride + used - 1];
+                if (open < 0) g = 0;         // the page is missing (latched before): nowhere to write
+            }
+            if (g > 0) want = pages_of(len + g, a.t.page) - used;
+        }
+        last[r] = open;
+        fresh[r] = want;
+        a.lens_out[r] = len + g;
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < a.n; r += blockDim.x) {
+        const int page = last[r];
+        if (page < 0) continue;
+        const int held = a.refs[page];
+        if (held <= 1) continue;
+        int same = 0, first = 1;
+        for (int i = 0; i < a.n; ++i)
+            if (last[i] == page) {
+                ++same;
+                if (i < r) first = 0;
+            }
+        if (!(same == held && first)) fresh[r] += 1 + kCopy;     // only this thread reads or writes this entry
+    }
+    __syncthreads();
+
+    // pages wanted by all rows, and the lowest free ones of the pool
+    int need = 0;
+    for (int r0 = 0; r0 < a.n; r0 += blockDim.x) {
+        const int r = r0 + threadIdx.x;
+        int total;
+        block_prefix(r < a.n ? fresh[r] & (kCopy - 1) : 0, red, total);
+        need += total;
+    }
+    int found = 0;
+    for (int p0 = 0; p0 < a.pages && found < need; p0 += kPlanThreads * kPagesPerThread) {
+        const int base = p0 + threadIdx.x * kPagesPerThread;
+        int mask = 0;
+#pragma unroll
+        for (int i = 0; i < kPagesPerThread; ++i)
+            if (base + i < a.pages && a.refs[base + i] == 0) mask |= 1 << i;
+        int total;
+        int at = found + block_prefix(__popc(mask), red, total);
+#pragma unroll
+        for (int i = 0; i < kPagesPerThread; ++i)
+            if (mask >> i & 1) a.free_list[at++] = base + i;
+        found += total;
+    }
+    __syncthreads();
+
+    int before = 0;
+    for (int r0 = 0; r0 < a.n; r0 += blockDim.x) {
+        const int r = r0 + threadIdx.x;
+        const int f = r < a.n ? fresh[r] : 0, k = f & (kCopy - 1);
+        int total;
+        const int at = before + block_prefix(k, red, total);
+        before += total;
+        if (r >= a.n) continue;
+        const int p = a.parents[r], len = kept_len(a.t, a.lens, p);
+        int src = 0, dst = 0, fill = 0;
+        if (k > 0 && at + k > found) {
+            latch(a.status, kStatusNoPages);                     // the pool is full: the row keeps what it has and does not grow
+            a.lens_out[r] = len;
+        } else if (k > 0) {
+            int* row = a.table + r * a.table_stride;
+            int used = pages_of(len, a.t.page), i = 0;
+            if (f & kCopy) {
+                src = last[r];
+                dst = a.free_list[at];
+                fill = len % a.t.page;
+                row[used - 1] = dst;
+                a.refs[dst] = 1;
+                atomicSub(a.refs + src, 1);
+                i = 1;
+            }
+            for (; i < k; ++i) {
+                const int page = a.free_list[at + i];
+                row[used++] = page;
+                a.refs[page] = 1;
+            }
+        }
+        a.copies[3 * r] = src;
+        a.copies[3 * r + 1] = dst;
+        a.copies[3 * r + 2] = fill;
+    }
+}
+
+struct CompactPlan {
+    const int* refs;            // [pages] rows that name a page
+    int *refs_out, *remap;      // of the moved pages; new place of a page, -1: free
+    int* copies;                // [pages][3]
+    int* n_copies;
+    int* live;
+    int* holes;                 // [pages] scratch
+    int pages;
+};
+
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const CompactPlan a) {
+    __shared__ int red[33];
+    pdl_launch_dependents();
+    pdl_wait();
+    constexpr int kStep = kPlanThreads * kPagesPerThread;
+    int live = 0;
+    for (int p0 = 0; p0 < a.pages; p0 += kStep) {
+        const int base = p0 + threadIdx.x * kPagesPerThread;
+        int c = 0, total;
+#pragma unroll
+        for (int i = 0; i < kPagesPerThread; ++i) c += base + i < a.pages && a.refs[base + i] > 0;
+        block_prefix(c, red, total);
+        live += total;
+    }
+    // holes in front of `live`, in order; what stays keeps its count
+    int holes = 0;
+    for (int p0 = 0; p0 < live; p0 += kStep) {
+        const int base = p0 + threadIdx.x * kPagesPerThread;
+        int mask = 0, total;
+#pragma unroll
+        for (int i = 0; i < kPagesPerThread; ++i) {
+            const int p = base + i;
+            if (p >= live) break;
+            const int n = a.refs[p];
+            if (n > 0) {
+                a.remap[p] = p;
+                a.refs_out[p] = n;
+            } else {
+                a.remap[p] = -1;
+                mask |= 1 << i;
+            }
+        }
+        int at = holes + block_prefix(__popc(mask), red, total);
+#pragma unroll
+        for (int i = 0; i < kPagesPerThread; ++i)
+            if (mask >> i & 1) a.holes[at++] = base + i;
+        holes += total;
+    }
+    __syncthreads();
+    // pages behind `live` move into them, in order
+    int moved = 0;
+    for (int p0 = live / kPagesPerThread * kPagesPerThread; p0 < a.pages; p0 += kStep) {
+        const int base = p0 + threadIdx.x * kPagesPerThread;
+        int mask = 0, total;
+#pragma unroll
+        for (int i = 0; i < kPagesPerThread; ++i) {
+            const int p = base + i;
+            if (p < live || p >= a.pages) continue;
+            a.refs_out[p] = 0;
+            if (a.refs[p] > 0) mask |= 1 << i;
+            else a.remap[p] = -1;
+        }
+        int at = moved + block_prefix(__popc(mask), red, total);
+#pragma unroll
+        for (int i = 0; i < kPagesPerThread; ++i)
+            if (mask >> i & 1) {
+                const int to = a.holes[at], p = base + i;
+                a.remap[p] = to;
+                a.refs_out[to] = a.refs[p];
+                a.copies[3 * at] = p;
+                a.copies[3 * at + 1] = to;
+                a.copies[3 * at + 2] = -1;                       // the whole page
+                ++at;
+            }
+        moved += total;
+    }
+    if (threadIdx.x == 0) {
+        *a.n_copies = moved;
+        *a.live = live;
+    }
+}
+
+// Checks a caller's list of copies: pages that do not exist, a target that is also a source, a target given twice (the last one counts).
+__global__ void __launch_bounds__(256) copy_list_kernel(const int* src, const int* dst, int n, int pages, int* copies, int* status) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= n) return;
+    const int s = src[i], d = dst[i];
+    int fill = -1;
+    if (s < 0 || d < 0 || s == d) {
+        fill = 0;                                                // left out
+    } else if (s >= pages || d >= pages) {
+        latch(status, kStatusBadPage);
+        fill = 0;
+    } else {
+        for (int j = 0; j < n; ++j) {
+            const int sj = src[j], dj = dst[j];
+            if (sj < 0 || dj < 0 || sj == dj || j == i) continue;
+            if (sj == d || (dj == d && j > i)) {
+                latch(status, kStatusPageConflict);
+                fill = 0;
+            }
+        }
+    }
+    copies[3 * i] = s;
+    copies[3 * i + 1] = d;
+    copies[3 * i + 2] = fill;
+}
+
+struct PageMove {
+    char* pool;                 // [planes][pages][heads][slots][dim]
+    const int* copies;          // [n][3] source, target, positions (-1: the page, 0: nothing)
+    const int* n_copies;        // null: n
+    int n, planes, heads;
+    int64_t plane_bytes, page_bytes, head_bytes, slot_bytes;
+    // the table of a compaction, renamed by the same launch
+    PageTable t;
+    const int *lens, *remap;
+    int* table_out;
+    int64_t table_stride;
+};
+
+constexpr int kMoveThreads = 256;
+constexpr int kMovePiece = kMoveThreads * 16 * 4;     // bytes that a CTA moves at a time: four 16-byte loads a thread in flight
+
+__global__ void __launch_bounds__(kMoveThreads) page_move_kernel(const PageMove a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int n = a.n_copies ? *a.n_copies : a.n;
+    if (a.table_out) {
+        for (int r = blockIdx.x; r < a.t.rows; r += gridDim.x) {
+            const int used = pages_of(kept_len(a.t, a.lens, r), a.t.page);
+            for (int j = threadIdx.x; j < a.t.width; j += blockDim.x) {
+                const int p = j < used ? page_at(a.t, r, j) : -1;
+                a.table_out[r * a.table_stride + j] = p < 0 ? -1 : a.remap[p];
+            }
+        }
+    }
+    // a piece never crosses a head, so that copies of a begun page move its written positions only
+    const int per_head = static_cast<int>((a.head_bytes + kMovePiece - 1) / kMovePiece);
+    const int64_t units = static_cast<int64_t>(n) * a.planes * a.heads * per_head;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int piece = static_cast<int>(u % per_head);
+        int64_t rest = u / per_head;
+        const int head = static_cast<int>(rest % a.heads);
+        rest /= a.heads;
+        const int plane = static_cast<int>(rest % a.planes), i = static_cast<int>(rest / a.planes);
+        const int fill = a.copies[3 * i + 2];
+        if (fill == 0) continue;
+        const int64_t bytes = fill < 0 ? a.head_bytes : fill * a.slot_bytes;
+        const int64_t begin = static_cast<int64_t>(piece) * kMovePiece;
+        char* base = a.pool + plane * a.plane_bytes + head * a.head_bytes;
+        const char* src = base + a.copies[3 * i] * a.page_bytes;
+        char* dst = base + a.copies[3 * i + 1] * a.page_bytes;
+        uint4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t o = begin + (k * kMoveThreads + threadIdx.x) * 16;
+            if (o < bytes) v[k] = *reinterpret_cast<const uint4*>(src + o);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t o = begin + (k * kMoveThreads + threadIdx.x) * 16;
+            if (o < bytes) *reinterpret_cast<uint4*>(dst + o) = v[k];
+        }
+    }
+}
+
+static int move_launch(PageMove& a, void* pool, int planes, int pages, int heads, int slots, int slot_bytes, cudaStream_t st) {
+    a.pool = static_cast<char*>(pool);
+    a.planes = planes; a.heads = heads;
+    a.slot_bytes = slot_bytes; a.head_bytes = static_cast<int64_t>(slots) * slot_bytes;
+    a.page_bytes = a.head_bytes * heads; a.plane_bytes = a.page_bytes * pages;
+    const int64_t units = static_cast<int64_t>(a.n) * planes * heads * ((a.head_bytes + kMovePiece - 1) / kMovePiece);
+    const int64_t most = 8ll * sm_count();
+    int64_t grid = units < most ? units : most;
+    if (a.table_out && grid < a.t.rows) grid = a.t.rows < most ? a.t.rows : most;
+    return grid > 0 ? launch(page_move_kernel, dim3(static_cast<unsigned>(grid)), dim3(kMoveThreads), 0, st, a) : 0;
+}
+
+static bool pool_ok(const void* pool, int planes, int pages, int heads, int slots, int slot_bytes) {
+    return planes >= 0 && pages >= 0 && heads >= 1 && slots >= 1 && slot_bytes >= 16 && slot_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(pool) & 15) == 0;
+}
+
+}  // namespace nexrt
+
+using namespace nexrt;
+
+// scratch: int[pages + 3 rows_out].  grow: positions that every new row will append (null: grow_all for all).
+extern "C" int nexrt_page_fork(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* table, int64_t table_stride, int rows, int width,
+                               const void* lens, const void* parents, const void* grow, int grow_all, void* table_out, int64_t out_stride, void* lens_out, void* refs,
+                               void* scratch, void* status, int rows_out, void* stream) {
+    if (!pool_ok(pool, planes, pages, heads, slots, slot_bytes) || rows < 0 || width < 0 || rows_out < 0 || rows_out > kPlanRows) return cudaErrorInvalidValue;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (pages > 0)
+        if (const cudaError_t e = cudaMemsetAsync(refs, 0, sizeof(int) * static_cast<size_t>(pages), st); e != cudaSuccess) return static_cast<int>(e);
+    if (rows_out == 0) return 0;
+    PageTable t = {static_cast<const int*>(table), table_stride, rows, width, slots, pages};
+    if (width > 0) {
+        const int cols = (width + 255) / 256;
+        const int e = launch(fork_rows_kernel, dim3(cols < 64 ? cols : 64, rows_out), dim3(256), 0, st, t, static_cast<const int*>(lens), static_cast<const int*>(parents),
+                             static_cast<int*>(table_out), out_stride, static_cast<int*>(refs), rows_out, static_cast<int*>(status));
+        if (e) return e;
+    }
+    ForkPlan p = {};
+    p.t = t; p.lens = static_cast<const int*>(lens); p.parents = static_cast<const int*>(parents); p.grow = static_cast<const int*>(grow);
+    p.table = static_cast<int*>(table_out); p.table_stride = out_stride; p.lens_out = static_cast<int*>(lens_out); p.refs = static_cast<int*>(refs);
+    p.copies = static_cast<int*>(scratch) + pages; p.free_list = static_cast<int*>(scratch);
+    p.status = static_cast<int*>(status); p.n = rows_out; p.grow_all = grow_all; p.pages = pages;
+    if (const int e = launch(fork_plan_kernel, dim3(1), dim3(kPlanThreads), sizeof(int) * 2 * rows_out, st, p)) return e;
+    PageMove m = {};
+    m.copies = p.copies; m.n = rows_out;
+    return move_launch(m, pool, planes, pages, heads, slots, slot_bytes, st);
+}
+
+// scratch: int[5 pages + 1].
+extern "C" int nexrt_page_compact(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* table, int64_t table_stride, int rows, int width,
+                                  const void* lens, void* table_out, int64_t out_stride, void* refs_out, void* remap, void* live, void* scratch, void* status,
+                                  void* stream) {
+    if (!pool_ok(pool, planes, pages, heads, slots, slot_bytes) || rows < 0 || width < 0) return cudaErrorInvalidValue;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int* refs = static_cast<int*>(scratch);
+    if (pages > 0)
+        if (const cudaError_t e = cudaMemsetAsync(refs, 0, sizeof(int) * static_cast<size_t>(pages), st); e != cudaSuccess) return static_cast<int>(e);
+    PageTable t = {static_cast<const int*>(table), table_stride, rows, width, slots, pages};
+    if (rows > 0 && width > 0) {
+        const int cols = (width + 255) / 256;
+        const int e = launch(fork_rows_kernel, dim3(cols < 64 ? cols : 64, rows < 65535 ? rows : 65535), dim3(256), 0, st, t, static_cast<const int*>(lens),
+                             static_cast<const int*>(nullptr), static_cast<int*>(nullptr), out_stride, refs, rows, static_cast<int*>(status));
+        if (e) return e;
+    }
+    CompactPlan p = {};
+    p.refs = refs; p.refs_out = static_cast<int*>(refs_out); p.remap = static_cast<int*>(remap);
+    p.holes = refs + pages; p.copies = refs + 2 * static_cast<int64_t>(pages); p.n_copies = refs + 5 * static_cast<int64_t>(pages);
+    p.live = static_cast<int*>(live); p.pages = pages;
+    if (const int e = launch(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p)) return e;
+    PageMove m = {};
+    m.copies = p.copies; m.n_copies = p.n_copies; m.n = pages;
+    m.t = t; m.lens = static_cast<const int*>(lens); m.remap = p.remap; m.table_out = static_cast<int*>(table_out); m.table_stride = out_stride;
+    return move_launch(m, pool, planes, pages, heads, slots, slot_bytes, st);
+}
+
+// scratch: int[3 n].
+extern "C" int nexrt_page_copy(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* src, const void* dst, int n, void* scratch,
+                               void* status, void* stream) {
+    if (!pool_ok(pool, planes, pages, heads, slots, slot_bytes) || n < 0) return cudaErrorInvalidValue;
+    if (n == 0) return 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int* copies = static_cast<int*>(scratch);
+    if (const int e = launch(copy_list_kernel, dim3((n + 255) / 256), dim3(256), 0, st, static_cast<const int*>(src), static_cast<const int*>(dst), n, pages, copies,
+                             static_cast<int*>(status)))
+        return e;
+    PageMove m = {};
+    m.copies = copies; m.n = n;
+    return move_launch(m, pool, planes, pages, heads, slots, slot_bytes, st);
+}

@@ -38,6 +38,7 @@ class LLChannelStruct(ctypes.Structure):
 
 
 CH = POINTER(LLChannelStruct)
+I64 = POINTER(c_int64)
 
 _PROTOTYPES = {
     "nexrt_set_pdl": [ci],
@@ -110,6 +111,16 @@ _PROTOTYPES = {
     "nexrt_attn_front_tail": [vp] * 6 + [ci] * 7 + [vp],
     "nexrt_tc_moe_l1": [vp] * 7 + [ci] * 6 + [cf, ci, vp, vp],
     "nexrt_tc_moe_l2_allreduce": [vp] * 8 + [ci] * 6 + [CH, cu, vp, vp],
+    "nexrt_rope_append": [vp] * 13 + [I64] + [ci] * 12 + [cf, cf, vp],
+    "nexrt_paged_ctas": [ci] * 6,
+    "nexrt_paged_attn": [vp] * 10 + [I64] + [ci] * 9 + [cf, cf, ci, vp],
+    "nexrt_paged_split": [vp, ci, ci, c_int64, ci, ci, vp, ci],
+    "nexrt_page_fork": [vp] + [ci] * 5 + [vp, c_int64, ci, ci, vp, vp, vp, ci, vp, c_int64, vp, vp, vp, vp, ci, vp],
+    "nexrt_page_compact": [vp] + [ci] * 5 + [vp, c_int64, ci, ci, vp, vp, c_int64] + [vp] * 6,
+    "nexrt_page_copy": [vp] + [ci] * 5 + [vp, vp, ci, vp, vp, vp],
+    "nexrt_beam_slices": [ci],
+    "nexrt_beam_select": [vp] * 3 + [I64] + [vp] * 5 + [ci] * 6 + [vp],
+    "nexrt_reorder_rows": [vp, vp, I64, ci, vp, c_int64, c_int64, ci, ci, ci, vp, vp],
     "nexrt_ipc_alloc": [c_size_t, POINTER(c_void_p)],
     "nexrt_ipc_get_handle": [vp, vp],
     "nexrt_ipc_open": [vp, POINTER(c_void_p)],
@@ -136,6 +147,8 @@ def load(build: bool = True) -> ctypes.CDLL:
         fn.restype = ci
     lib.nexrt_attn_decode_smem.argtypes = [ci, ci, ci, ci]
     lib.nexrt_attn_decode_smem.restype = c_size_t
+    lib.nexrt_paged_slot.argtypes = [vp, c_int64, ci, ci, ci, ci, ci, ci]
+    lib.nexrt_paged_slot.restype = c_int64
     lib.nexrt_moe_router_rows_split.argtypes = []
     lib.nexrt_moe_router_rows_split.restype = ci
     lib.nexrt_launch_count.argtypes = []
@@ -185,3 +198,33 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+def longs(*values: int):
+    """An ``int64_t[]`` argument."""
+    return (c_int64 * len(values))(*values)
+
+
+def on_device(device: torch.device, call, what: str) -> None:
+    """``call(stream)`` on ``device``'s current stream, with that device current: the operators' tensors may lie on another one."""
+    if device.index == torch.cuda.current_device():
+        check(call(torch.cuda.current_stream(device).cuda_stream), what)
+        return
+    with torch.cuda.device(device):
+        check(call(torch.cuda.current_stream(device).cuda_stream), what)
+
+
+def same_cuda_device(what: str, *tensors: Optional[torch.Tensor]) -> torch.device:
+    """The CUDA device that all the tensors given lie on; a ``ValueError`` where there is none."""
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+    if device.type != "cuda":
+        raise ValueError(f"{what} runs on a CUDA device, the tensors are on {device}")
+    return device
+
+
+def check_status(what: str, status: Optional[torch.Tensor]) -> None:
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
+        raise ValueError(f"{what}: status is one int32")

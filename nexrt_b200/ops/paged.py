@@ -1,0 +1,212 @@
+"""A key-value cache in pages that several sequences share (``csrc/paged_attn.cu``, ``csrc/pages.cu``).
+
+The engine's own cache (``attn.py: FullAttn``) is one contiguous block for one sequence.  Here the keys and values of a batch lie
+in a pool of pages: ``kv [layers, 2, pages, kv heads, slots, dim]`` (K and V of every layer), and ``table`` int32 ``[rows, width]``
+names, row by row, the page of positions ``[slots * j, slots * (j + 1))``; behind a row's last page it holds -1.  ``lens`` int32
+``[rows]`` are the rows' positions.  Rows may share pages (a common prompt, beams of one request); a page is free when no row
+names it within its length.
+
+Everything is planned on the device: no call waits for the host, all of them can be captured into a CUDA graph.  What a kernel
+finds wrong (a page that does not exist, a full pool) is left out and latched in ``status`` (``runtime/control.py: Status``).
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+
+from ..runtime.control import Status
+from .lib import KernelError, check_status, load as lib, longs, on_device, ptr, same_cuda_device
+from .rope import TYPES, rope_append
+
+HEAD_DIMS = (64, 128, 192, 256)
+MAX_ROWS = 4096
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, scale: Optional[float] = None,
+                    softcap: float = 0.0, window: int = 0, slopes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                    status: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """One new token of every sequence over its pages: ``q [rows, heads, dim]`` against keys ``[max(0, len - window), len)`` of each row
+    (``window`` 0: all), whose own key is the last of them.  ``k_pages`` / ``v_pages [pages, kv heads, slots, dim]`` are one layer's
+    (``kv[layer, 0]``, ``kv[layer, 1]``), bf16 or fp16 like q; dims 64, 128, 192 or 256; heads a multiple of the kv heads.
+
+    Scores are ``q.k * scale`` (default ``dim ** -0.5``), then ``softcap * tanh(s / softcap)`` if it is not zero, then
+    ``s - slopes[head] * distance`` if ``slopes`` (fp32 ``[heads]``) is given.  A row without keys gives zeros and an lse of -inf, and so
+    does one whose scores are all -inf.  Returns ``out [rows, heads, dim]``, with ``return_lse`` also fp32 ``[rows, heads]``: the natural
+    logarithm of the sum of exp of the scores.  Keys on a page that the table does not name count as masked and latch ``BAD_PAGE``."""
+    what = "paged_attention"
+    if q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float16) or q.stride(2) != 1:
+        raise ValueError(f"{what}: q is [rows, heads, dim] in bf16 or fp16 with a contiguous last dimension")
+    rows, heads, dim = q.shape
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1 or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+        raise ValueError(f"{what}: k_pages and v_pages are [pages, kv heads, slots, dim] of q's type, with the same strides and a contiguous last dimension")
+    pages, kv_heads, slots = k_pages.shape[:3]
+    if dim not in HEAD_DIMS or k_pages.shape[3] != dim:
+        raise ValueError(f"{what}: head dimensions are {HEAD_DIMS}, those of q and of the pages the same")
+    if kv_heads < 1 or slots < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"{what}: {heads} heads on {kv_heads} kv heads")
+    if any(s % 8 for s in k_pages.stride()[:3]) or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
+        raise ValueError(f"{what}: rows of the pages start on 16-byte boundaries")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != rows or table.stride(1) != 1:
+        raise ValueError(f"{what}: table is int32 [rows, pages of a row] with contiguous rows")
+    if lens.dtype != torch.int32 or lens.shape != (rows,) or not lens.is_contiguous():
+        raise ValueError(f"{what}: lens is int32 [rows]")
+    if not (softcap >= 0.0 and math.isfinite(softcap)) or window < 0:
+        raise ValueError(f"{what}: softcap and window are not negative")
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous()):
+        raise ValueError(f"{what}: slopes is fp32 [heads]")
+    check_status(what, status)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError(f"{what}: out is like q")
+    lse = torch.empty(rows, heads, dtype=torch.float32, device=q.device) if return_lse else None
+    device = same_cuda_device(what, q, k_pages, v_pages, table, lens, slopes, out, status)
+    if rows:
+        L = lib()
+        width = table.shape[1]
+        window = min(window, 2**31 - 1)
+        ctas = L.nexrt_paged_ctas(rows, heads, kv_heads, width, slots, window)
+        scratch = torch.empty(2 * ctas * 16 * (dim + 2), dtype=torch.float32, device=device)
+        strides = longs(q.stride(0), q.stride(1), out.stride(0), out.stride(1), *k_pages.stride()[:3], table.stride(0), heads)
+        on_device(device, lambda st: L.nexrt_paged_attn(
+            ptr(q), ptr(k_pages), ptr(v_pages), ptr(table), ptr(lens), ptr(slopes), ptr(out), ptr(lse), ptr(scratch), ptr(status), strides, rows, heads, kv_heads, dim,
+            width, slots, pages, window, TYPES[q.dtype], dim**-0.5 if scale is None else scale, softcap, ctas, st), what)
+    return (out, lse) if return_lse else out
+
+
+def _pool(what: str, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor):
+    """Arguments of the page kernels: base, planes, pages, heads, slots, bytes of a slot."""
+    if kv.dim() != 6 or kv.shape[1] != 2 or not kv.is_contiguous():
+        raise ValueError(f"{what}: kv is a contiguous [layers, 2, pages, kv heads, slots, dim]")
+    if kv.shape[3] < 1 or kv.shape[4] < 1 or kv.shape[5] * kv.element_size() % 16 or kv.shape[5] < 1 or kv.data_ptr() % 16:
+        raise ValueError(f"{what}: a slot of the pool takes a multiple of 16 bytes and starts on such a boundary")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+        raise ValueError(f"{what}: table is int32 [rows, pages of a row] with contiguous rows")
+    if lens.dtype != torch.int32 or lens.shape != (table.shape[0],) or not lens.is_contiguous():
+        raise ValueError(f"{what}: lens is int32 [rows]")
+    return ptr(kv), 2 * kv.shape[0], kv.shape[2], kv.shape[3], kv.shape[4], kv.shape[5] * kv.element_size()
+
+
+def _fresh(what: str, name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor, *old: torch.Tensor) -> torch.Tensor:
+    if t is None:
+        return torch.empty(shape, dtype=torch.int32, device=like.device)
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or (t.numel() and t.stride(-1) != 1) or (t.dim() == 1 and not t.is_contiguous()):
+        raise ValueError(f"{what}: {name} is int32 {list(shape)} with contiguous rows")
+    for o in old:
+        if o is not None and t.numel() and o.numel() and t.untyped_storage().data_ptr() == o.untyped_storage().data_ptr():
+            raise ValueError(f"{what}: {name} shares memory with an input: the rows are read while it is written")
+    return t
+
+
+def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, grow: Union[int, torch.Tensor] = 0, *, table_out: Optional[torch.Tensor] = None,
+               lens_out: Optional[torch.Tensor] = None, refs: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Row ``r`` of the new table goes on with row ``parents[r]`` of the old one (int32, at most 4096; -1: the row is empty) and gets
+    room for ``grow`` more positions (an int for all rows, or int32 ``[rows]``): ``(table, lens + grow, refs)``, where ``refs`` int32
+    ``[pages]`` says how many rows name a page.  Rows that nobody continues are freed with what they alone held.
+
+    Full pages are shared.  A begun page that a growing row shares with others is copied, its written positions in all layers;
+    where all its holders grow, the lowest row keeps it.  New pages are the lowest free ones, in the order of the rows.  A row for
+    which there is no page, or no column in the table, keeps its length and latches ``NO_PAGES``; a page or parent that does not
+    exist latches ``BAD_PAGE``.  The outputs must not share memory with ``table`` or ``lens``."""
+    what = "fork_pages"
+    pool = _pool(what, kv, table, lens)
+    if parents.dtype != torch.int32 or parents.dim() != 1 or not parents.is_contiguous() or parents.numel() > MAX_ROWS:
+        raise ValueError(f"{what}: parents is int32 [rows], at most {MAX_ROWS}")
+    n, width, pages = parents.numel(), table.shape[1], kv.shape[2]
+    each = grow if isinstance(grow, torch.Tensor) else None
+    if each is not None and (each.dtype != torch.int32 or each.shape != (n,) or not each.is_contiguous()):
+        raise ValueError(f"{what}: grow is an int or int32 [rows]")
+    if each is None and not 0 <= grow < 2**31:
+        raise ValueError(f"{what}: grow is not negative")
+    check_status(what, status)
+    table_out = _fresh(what, "table_out", table_out, (n, width), table, table)
+    lens_out = _fresh(what, "lens_out", lens_out, (n,), table, lens, parents, each)
+    refs = _fresh(what, "refs", refs, (pages,), table, lens, parents, each, table)
+    device = same_cuda_device(what, kv, table, lens, parents, each, table_out, lens_out, refs, status)
+    scratch = torch.empty(pages + 3 * n, dtype=torch.int32, device=device)
+    on_device(device, lambda st: lib().nexrt_page_fork(*pool, ptr(table), table.stride(0), table.shape[0], width, ptr(lens), ptr(parents), ptr(each), 0 if each is not None else grow,
+                                                       ptr(table_out), table_out.stride(0), ptr(lens_out), ptr(refs), ptr(scratch), ptr(status), n, st), what)
+    return table_out, lens_out, refs
+
+
+def compact_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, table_out: Optional[torch.Tensor] = None, refs: Optional[torch.Tensor] = None,
+                  status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Moves the pages that rows name to the front of the pool, all layers: of ``live`` such pages those behind the first ``live``
+    places go, in order, into the holes in front.  Returns ``(table, refs, remap, live)``: the renamed table, rows per page, new
+    place of every page (-1: it was free) and ``live`` int32 ``[1]``.  What lies in the pool from ``live`` on is free."""
+    what = "compact_pages"
+    pool = _pool(what, kv, table, lens)
+    pages = kv.shape[2]
+    check_status(what, status)
+    table_out = _fresh(what, "table_out", table_out, tuple(table.shape), table, table)
+    refs = _fresh(what, "refs", refs, (pages,), table, lens, table)
+    remap = torch.empty(pages, dtype=torch.int32, device=table.device)
+    live = torch.empty(1, dtype=torch.int32, device=table.device)
+    device = same_cuda_device(what, kv, table, lens, table_out, refs, status)
+    scratch = torch.empty(5 * pages + 1, dtype=torch.int32, device=device)
+    on_device(device, lambda st: lib().nexrt_page_compact(*pool, ptr(table), table.stride(0), table.shape[0], table.shape[1], ptr(lens), ptr(table_out), table_out.stride(0), ptr(refs),
+                                                          ptr(remap), ptr(live), ptr(scratch), ptr(status), st), what)
+    return table_out, refs, remap, live
+
+
+def copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *, status: Optional[torch.Tensor] = None) -> None:
+    """Page ``src[i]`` to page ``dst[i]`` in all layers (int32, one list each).  A negative entry is left out; one beyond the pool latches
+    ``BAD_PAGE``.  A target that is also a source is left out, of a target given twice only the last counts; both latch ``PAGE_CONFLICT``."""
+    what = "copy_pages"
+    for t in (src, dst):
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() != src.numel():
+            raise ValueError(f"{what}: src and dst are int32 lists of the same length")
+    pool = _pool(what, kv, src.view(-1, 1), src)
+    check_status(what, status)
+    device = same_cuda_device(what, kv, src, dst, status)
+    scratch = torch.empty(3 * src.numel(), dtype=torch.int32, device=device)
+    on_device(device, lambda st: lib().nexrt_page_copy(*pool, ptr(src), ptr(dst), src.numel(), ptr(scratch), ptr(status), st), what)
+
+
+class PagedCache:
+    """Pool, table, lengths and status word of a batch, at fixed addresses (a captured step stays valid).
+
+    One decode step: ``fork(parents, 1)`` - or ``fork(grow=1)`` to go on with every row -, then for every layer ``append`` (the new
+    tokens' positions are ``lens - 1``) and ``attend``.  ``check()`` waits for the device and raises what the kernels latched."""
+
+    def __init__(self, layers: int, pages: int, kv_heads: int, slots: int, dim: int, rows: int, max_len: int, dtype: torch.dtype = torch.bfloat16,
+                 device: Union[str, torch.device] = "cuda"):
+        if min(layers, pages, kv_heads, slots, rows, max_len) < 1 or dim not in HEAD_DIMS or dtype not in (torch.bfloat16, torch.float16) or rows > MAX_ROWS:
+            raise ValueError(f"PagedCache: sizes are positive, at most {MAX_ROWS} rows, head dimensions {HEAD_DIMS}, bf16 or fp16")
+        i32 = dict(dtype=torch.int32, device=device)
+        self.kv = torch.zeros(layers, 2, pages, kv_heads, slots, dim, dtype=dtype, device=device)
+        self.table = torch.full((rows, -(-max_len // slots)), -1, **i32)
+        self.lens = torch.zeros(rows, **i32)
+        self.refs = torch.zeros(pages, **i32)
+        self.status = torch.zeros(1, **i32)
+        self.same = torch.arange(rows, **i32)
+
+    def fork(self, parents: Optional[torch.Tensor] = None, grow: Union[int, torch.Tensor] = 0) -> None:
+        """``fork_pages`` on the cache's own table: every row of it goes on with one of its rows, or is freed (-1)."""
+        parents = self.same if parents is None else parents
+        if parents.shape != self.lens.shape:
+            raise ValueError("PagedCache.fork: one parent for every row of the cache")
+        table, lens, _ = fork_pages(self.kv, self.table, self.lens, parents, grow, refs=self.refs, status=self.status)
+        self.table.copy_(table)
+        self.lens.copy_(lens)
+
+    def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, rows: torch.Tensor, inv_freq: torch.Tensor, **how) -> torch.Tensor:
+        return rope_append(q, k, v, positions, rows, self.kv[layer, 0], self.kv[layer, 1], self.table, inv_freq, status=self.status, **how)
+
+    def attend(self, layer: int, q: torch.Tensor, **how) -> torch.Tensor:
+        return paged_attention(q, self.kv[layer, 0], self.kv[layer, 1], self.table, self.lens, status=self.status, **how)
+
+    def compact(self) -> torch.Tensor:
+        """Pages in use move to the front; returns their number (int32 ``[1]`` on the device)."""
+        table, _, _, live = compact_pages(self.kv, self.table, self.lens, refs=self.refs, status=self.status)
+        self.table.copy_(table)
+        return live
+
+    def check(self) -> None:
+        code = int(self.status.item())
+        if code:
+            names = {v: k for k, v in vars(Status).items() if isinstance(v, int)}
+            raise KernelError(f"paged cache: {names.get(code, code)}")

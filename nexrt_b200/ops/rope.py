@@ -1,0 +1,130 @@
+"""Rotary positions (``csrc/rope.cu``): rows of q and k heads normalised and rotated, k and v stored into the pages of their
+sequences, in one launch.  The decode kernels of the engine rotate in their own prologue (half layout, unscaled, one sequence);
+these entry points are for batches over a paged cache (``ops/paged.py``) and for models with another layout or scaling.
+
+Pair ``i`` of a head at position ``p`` turns by ``p * inv_freq[i]``; ``scale`` multiplies cos and sin.  The angle is formed in
+64 bits, so far positions lose nothing.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from .lib import check_status, load as lib, longs, on_device, ptr, same_cuda_device
+
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_DIM = 256
+
+
+def rope_frequencies(rotary: int, theta: float, scaling: Optional[str] = None, factor: float = 1.0, trained: int = 0, fast: float = 32.0,
+                     slow: float = 1.0) -> Tuple[torch.Tensor, float]:
+    """``(inv_freq [rotary / 2] fp32 on the CPU, scale)`` for a model trained on ``trained`` positions and used on ``factor`` times as many.
+
+    ``scaling``: ``None``; ``"linear"`` - all positions divided by the factor; ``"base"`` - theta raised so that the slowest pair is
+    divided by the factor; ``"ramp"`` - pairs that turn ``fast`` times or more over the trained positions are left, those that turn less
+    than ``slow`` times are divided by the factor, with a linear ramp between, and cos and sin grow by 0.1 ln(factor) + 1."""
+    if rotary < 2 or rotary % 2 or not theta > 1.0 or not math.isfinite(theta):
+        raise ValueError("rope_frequencies: rotary is even and positive, theta finite and above 1")
+    if scaling not in (None, "linear", "base", "ramp") or not factor >= 1.0 or not math.isfinite(factor):
+        raise ValueError("rope_frequencies: scaling is None, 'linear', 'base' or 'ramp', with a factor of 1 or more")
+    n = rotary // 2
+    if scaling == "base":
+        theta = theta * factor ** (rotary / (rotary - 2)) if rotary > 2 else theta
+    inv = [theta ** (-2.0 * i / rotary) for i in range(n)]
+    scale = 1.0
+    if scaling == "linear":
+        inv = [f / factor for f in inv]
+    elif scaling == "ramp":
+        if trained < 1 or not fast > slow > 0:
+            raise ValueError("rope_frequencies: 'ramp' needs the trained positions and fast > slow > 0")
+        at = lambda turns: rotary * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
+        low, high = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), rotary - 1)
+        keep = [1.0 - min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0) for i in range(n)]
+        inv = [f / factor * (1.0 - m) + f * m for f, m in zip(inv, keep)]
+        scale = 0.1 * math.log(factor) + 1.0
+    return torch.tensor(inv, dtype=torch.float32), scale
+
+
+def _heads(what: str, x: torch.Tensor, tokens: int, dim: int, dtype: torch.dtype) -> None:
+    if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != dim or x.dtype != dtype or x.stride(2) != 1:
+        raise ValueError(f"{what}: tensors of heads are [tokens, heads, dim] of one type with a contiguous last dimension")
+
+
+def _common(what, q, positions, inv_freq, norms):
+    if q.dim() != 3 or q.dtype not in TYPES or q.stride(2) != 1:
+        raise ValueError(f"{what}: q is [tokens, heads, dim] in bf16, fp16 or fp32 with a contiguous last dimension")
+    tokens, _, dim = q.shape
+    if dim < 8 or dim > MAX_DIM or dim % 8:
+        raise ValueError(f"{what}: head dimensions are multiples of 8 up to {MAX_DIM}, not {dim}")
+    if positions.dtype != torch.int32 or positions.shape != (tokens,) or not positions.is_contiguous():
+        raise ValueError(f"{what}: positions is int32 [tokens]")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or 2 * inv_freq.numel() > dim:
+        raise ValueError(f"{what}: inv_freq is fp32 [rotary / 2] with rotary at most the head dimension")
+    for w in norms:
+        if w is not None and (w.dtype != torch.float32 or w.shape != (dim,) or not w.is_contiguous()):
+            raise ValueError(f"{what}: norm multipliers are fp32 [dim]")
+    return tokens, dim
+
+
+def rope(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0, norm: Optional[torch.Tensor] = None,
+         eps: float = 1e-6, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``q [tokens, heads, dim]`` at ``positions`` int32 ``[tokens]``, rotated (after an RMSNorm with the multiplier ``norm``, if given); ``out`` may be ``q``."""
+    tokens, dim = _common("rope", q, positions, inv_freq, (norm,))
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _heads("rope", out, tokens, dim, q.dtype)
+    if out.shape[1] != q.shape[1]:
+        raise ValueError("rope: out has other heads than q")
+    device = same_cuda_device("rope", q, positions, inv_freq, norm, out)
+    if q.numel() == 0:
+        return out
+    strides = longs(q.stride(0), q.stride(1), 0, 0, 0, 0, out.stride(0), out.stride(1), 0, 0, 0, 0)
+    kind = TYPES[q.dtype]
+    on_device(device, lambda st: lib().nexrt_rope_append(ptr(q), None, None, ptr(positions), None, ptr(out), None, None, None, ptr(inv_freq), ptr(norm), None, None, strides,
+                                                         tokens, q.shape[1], 0, dim, 2 * inv_freq.numel(), int(interleaved), 0, 0, 1, 0, kind, kind, scale, eps, st), "rope")
+    return out
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, rows: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                table: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0, q_norm: Optional[torch.Tensor] = None,
+                k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """New tokens of a paged cache: q and k ``[tokens, heads, dim]`` are normalised (``q_norm``, ``k_norm``: fp32 ``[dim]``) and rotated
+    to ``positions`` int32 ``[tokens]``; k and v go to the slot of that position in row ``rows[i]`` of ``table`` (``ops/paged.py``), the
+    rotated q is returned in the pages' type.  q, k and v may be views of one projection's output, in the pages' type or in fp32.
+
+    A negative ``rows[i]`` is padding: its q is rotated, nothing is stored.  A position whose page the table does not name is left out
+    and latches ``BAD_PAGE`` in ``status``.  Two tokens of a call with the same slot leave it undefined."""
+    what = "rope_append"
+    tokens, dim = _common(what, q, positions, inv_freq, (q_norm, k_norm))
+    _heads(what, k, tokens, dim, q.dtype)
+    _heads(what, v, tokens, dim, q.dtype)
+    if k.shape != v.shape:
+        raise ValueError(f"{what}: k and v have the same heads")
+    if rows.dtype != torch.int32 or rows.shape != (tokens,) or not rows.is_contiguous():
+        raise ValueError(f"{what}: rows is int32 [tokens]")
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride() or k_pages.dtype != v_pages.dtype or k_pages.stride(3) != 1:
+        raise ValueError(f"{what}: k_pages and v_pages are [pages, kv heads, slots, dim] with the same strides and a contiguous last dimension")
+    if k_pages.shape[1] != k.shape[1] or k_pages.shape[3] != dim or k_pages.shape[2] < 1:
+        raise ValueError(f"{what}: the pages have other heads than k")
+    if k_pages.dtype not in (torch.bfloat16, torch.float16) or q.dtype not in (k_pages.dtype, torch.float32):
+        raise ValueError(f"{what}: pages are bf16 or fp16, q, k and v the same or fp32")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+        raise ValueError(f"{what}: table is int32 [rows, pages of a row] with contiguous rows")
+    check_status(what, status)
+    if out is None:
+        out = torch.empty(q.shape, dtype=k_pages.dtype, device=q.device)
+    _heads(what, out, tokens, dim, k_pages.dtype)
+    if out.shape[1] != q.shape[1]:
+        raise ValueError(f"{what}: out has other heads than q")
+    device = same_cuda_device(what, q, k, v, positions, rows, k_pages, v_pages, table, inv_freq, q_norm, k_norm, out, status)
+    if tokens == 0:
+        return out
+    strides = longs(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1), *k_pages.stride()[:3], table.stride(0))
+    on_device(device, lambda st: lib().nexrt_rope_append(
+        ptr(q), ptr(k), ptr(v), ptr(positions), ptr(rows), ptr(out), ptr(k_pages), ptr(v_pages), ptr(table), ptr(inv_freq), ptr(q_norm), ptr(k_norm), ptr(status), strides,
+        tokens, q.shape[1], k.shape[1], dim, 2 * inv_freq.numel(), int(interleaved), table.shape[0], table.shape[1], k_pages.shape[2], k_pages.shape[0], TYPES[q.dtype],
+        TYPES[k_pages.dtype], scale, eps, st), what)
+    return out

@@ -41,6 +41,9 @@ class Status:
     CP_TIMEOUT = 4
     BAD_TOKEN = 5
     PIPE_TIMEOUT = 6
+    BAD_PAGE = 7
+    NO_PAGES = 8
+    PAGE_CONFLICT = 9
 
 
 _HEADER_NAMES = {
@@ -51,7 +54,8 @@ _HEADER_NAMES = {
     "kCtlForcedMean10": Ctl.FORCED_MEAN10, "kCtlWords": CTL_WORDS,
     "kStatusOk": Status.OK, "kStatusReduceTimeout": Status.REDUCE_TIMEOUT, "kStatusNonFinite": Status.NON_FINITE,
     "kStatusBadConfig": Status.BAD_CONFIG, "kStatusCpTimeout": Status.CP_TIMEOUT, "kStatusBadToken": Status.BAD_TOKEN,
-    "kStatusPipeTimeout": Status.PIPE_TIMEOUT, "kMaxRows": MAX_ROWS,
+    "kStatusPipeTimeout": Status.PIPE_TIMEOUT, "kStatusBadPage": Status.BAD_PAGE,
+    "kStatusNoPages": Status.NO_PAGES, "kStatusPageConflict": Status.PAGE_CONFLICT, "kMaxRows": MAX_ROWS,
 }
 
 

@@ -1,0 +1,255 @@
+"""Pages of a shared cache: forking, freeing, growing, copying and compacting against a statement in plain Python, full pools and tables, bad entries,
+and a random walk of a cache whose contents are followed token by token."""
+
+import random
+
+import pytest
+import torch
+
+from nexrt_b200.ops.lib import KernelError
+from nexrt_b200.ops.paged import PagedCache, compact_pages, copy_pages, fork_pages
+from nexrt_b200.runtime.capture import graph_capture
+from nexrt_b200.runtime.control import Status
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def held(table, lens, page):
+    count = {}
+    for row, n in zip(table, lens):
+        for p in row[: -(-n // page)]:
+            count[p] = count.get(p, 0) + 1
+    return count
+
+
+def fork_in_python(kv, table, lens, parents, grow, page):
+    """(kv, table, lens, refs, short): ``short`` - a row did not get its pages."""
+    pages, width = kv.shape[2], len(table[0]) if table else 0
+    new = [table[p][: -(-lens[p] // page)] if p >= 0 else [] for p in parents]
+    n = [lens[p] if p >= 0 else 0 for p in parents]
+    count = held(new, n, page)
+    short, want, open_ = False, [0] * len(n), [None] * len(n)
+    g = [x if p >= 0 else 0 for x, p in zip(grow, parents)]
+    for r in range(len(n)):
+        if g[r] > 0 and n[r] + g[r] > width * page:
+            g[r], short = 0, True
+        if g[r] > 0:
+            want[r] = -(-(n[r] + g[r]) // page) - len(new[r])
+            open_[r] = new[r][-1] if n[r] % page else None
+    copies = [o is not None and count[o] > 1 and not (open_.count(o) == count[o] and open_.index(o) == r) for r, o in enumerate(open_)]
+    free = [p for p in range(pages) if p not in count]
+    refs, out, at = dict(count), kv.clone(), 0
+    for r in range(len(n)):
+        k = want[r] + copies[r]
+        mine, at = free[at : at + k], at + k
+        if len(mine) < k:
+            g[r], short = 0, True
+            continue
+        if copies[r]:
+            p = mine.pop(0)
+            out[:, :, p, :, : n[r] % page] = kv[:, :, open_[r], :, : n[r] % page]
+            new[r][-1], refs[p] = p, 1
+            refs[open_[r]] -= 1
+        for p in mine:
+            new[r].append(p)
+            refs[p] = 1
+    return out, [t + [-1] * (width - len(t)) for t in new], [a + b for a, b in zip(n, g)], [refs.get(p, 0) for p in range(pages)], short
+
+
+def random_rows(r, rows, width, pages, page):
+    """A table with shared prefixes, as forks leave it, and rows of any length."""
+    table, lens = [], []
+    free = list(range(pages))
+    r.shuffle(free)
+    for i in range(rows):
+        if table and r.random() < 0.5:
+            j = r.randrange(i)
+            n = r.randint(0, lens[j])
+            t = table[j][: -(-n // page)]
+        else:
+            n = min(r.choice([0, 1, page - 1, page, page + 1, r.randint(0, width * page)]), width * page, len(free) * page)
+            t = [free.pop() for _ in range(-(-n // page))]
+        table.append(t)
+        lens.append(n)
+    return [t + [-1] * (width - len(t)) for t in table], lens
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_fork_is_its_statement(seed):
+    r = random.Random(seed)
+    page, rows, width, heads, dim = r.choice([1, 2, 16, 5]), r.randint(1, 40), r.randint(1, 12), r.choice([1, 3]), r.choice([64, 128])
+    pages = r.choice([rows * width * 2 + 5, max(4, rows * width // 3)])
+    table, lens = random_rows(r, rows, width, pages, page)
+    n = r.choice([rows, 1, rows * 3])
+    parents = [r.choice([-1, r.randrange(rows), r.randrange(rows)]) for _ in range(n)]
+    grow = r.choice([[1] * n, [0] * n, [r.randint(0, 2 * page + 1) for _ in range(n)]])
+    dtype = r.choice([torch.bfloat16, torch.float32, torch.int8])
+    kv = torch.randint(-100, 100, (r.randint(1, 3), 2, pages, heads, page, dim), device=DEV).to(dtype)
+    want = fork_in_python(kv, table, lens, parents, grow, page)
+    status = ints([0])
+    t, l, refs = fork_pages(kv, ints(table), ints(lens), ints(parents), grow[0] if len(set(grow)) == 1 else ints(grow), status=status)
+    assert t.tolist() == want[1] and l.tolist() == want[2] and refs.tolist() == want[3]
+    assert torch.equal(kv, want[0]) and int(status) == (Status.NO_PAGES if want[4] else 0)
+
+
+def test_fork_of_many_rows_and_a_wide_table():
+    r = random.Random(1)
+    page, rows, width = 2, 2500, 600
+    pages = 30000
+    table, lens = random_rows(r, 40, width, pages, page)
+    parents = [r.randrange(40) for _ in range(rows)]
+    kv = torch.randint(-100, 100, (1, 2, pages, 1, page, 16), device=DEV).to(torch.int8)
+    want = fork_in_python(kv, table, lens, parents, [1] * rows, page)
+    t, l, refs = fork_pages(kv, ints(table), ints(lens), ints(parents), 1)
+    assert t.tolist() == want[1] and l.tolist() == want[2] and refs.tolist() == want[3] and torch.equal(kv, want[0])
+
+
+def test_fork_reports_and_survives_bad_input():
+    kv = torch.zeros(1, 2, 6, 1, 4, 64, dtype=torch.bfloat16, device=DEV)
+
+    def run(table, lens, parents, grow=0):
+        status = ints([0])
+        t, l, refs = fork_pages(kv, ints(table), ints(lens), ints(parents), grow, status=status)
+        return t.tolist(), l.tolist(), refs.tolist(), int(status)
+
+    assert run([[0, 1]], [8], [5, 0]) == ([[-1, -1], [0, 1]], [0, 8], [1, 1, 0, 0, 0, 0], Status.BAD_PAGE)          # a parent that does not exist
+    assert run([[0, 6]], [8], [0]) == ([[0, -1]], [8], [1, 0, 0, 0, 0, 0], Status.BAD_PAGE)                          # a page that does not exist
+    assert run([[0, -9]], [7], [0], 1) == ([[0, -1]], [7], [1, 0, 0, 0, 0, 0], Status.BAD_PAGE)                      # ... and is written next: the row stays
+    assert run([[0, 1]], [9], [0]) == ([[0, 1]], [8], [1, 1, 0, 0, 0, 0], Status.BAD_PAGE)                           # longer than the table
+    assert run([[0, 1]], [8], [0], 1) == ([[0, 1]], [8], [1, 1, 0, 0, 0, 0], Status.NO_PAGES)                        # no column left
+    assert run([[0, 1]], [2**31 - 1], [0], 2**31 - 1)[1] == [8]
+    assert run([[0]], [-3], [0], 0) == ([[-1]], [0], [0] * 6, 0)
+    assert run([[0]], [4], []) == ([], [], [0] * 6, 0)
+    full = run([[0, 1, 2, 3, 4, 5]], [24], [0, -1])
+    assert full == ([[0, 1, 2, 3, 4, 5], [-1] * 6], [24, 0], [1] * 6, 0)
+    assert run([[0, 1, 2, 3, 4, 5], [-1] * 6], [24, 0], [0, 1], ints([0, 1]))[1:] == ([24, 0], [1] * 6, Status.NO_PAGES)   # the pool is full
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_compact_is_its_statement(seed):
+    r = random.Random(100 + seed)
+    page, rows, width = r.choice([1, 4, 16]), r.randint(1, 30), r.randint(1, 40)
+    pages = r.choice([rows * width + 3, rows * width * 5 + 9000 * (seed % 2)])
+    table, lens = random_rows(r, rows, width, pages, page)
+    kv = torch.randint(-100, 100, (r.randint(1, 2), 2, pages, r.choice([1, 2]), page, 64), device=DEV).to(torch.int8)
+    count = held(table, lens, page)
+    live = len(count)
+    holes = iter([p for p in range(live) if p not in count])
+    to = {p: p if p < live else next(holes) for p in sorted(count)}
+    want = kv.clone()
+    for p, q in to.items():
+        want[:, :, q] = kv[:, :, p]
+    dirty = [[p if j < -(-n // page) else r.choice([-1, 0, 10**6]) for j, p in enumerate(row)] for row, n in zip(table, lens)]   # behind the last page: anything
+    status = ints([0])
+    t, refs, remap, n = compact_pages(kv, ints(dirty), ints(lens), status=status)
+    assert t.tolist() == [[to[p] if p >= 0 else -1 for p in row] for row in table] and int(n) == live and int(status) == 0
+    assert remap.tolist() == [to.get(p, -1) for p in range(pages)]
+    back = {q: p for p, q in to.items()}
+    assert refs.tolist() == [count[back[p]] if p in back else 0 for p in range(pages)]
+    assert torch.equal(kv, want)
+
+
+def test_copy_pages():
+    kv = torch.randint(-100, 100, (3, 2, 50, 2, 7, 64), device=DEV).to(torch.bfloat16)
+
+    def run(src, dst):
+        a, status = kv.clone(), ints([0])
+        copy_pages(a, ints(src), ints(dst), status=status)
+        return a, int(status)
+
+    a, code = run([3, 4, 3, -1, 9, 11], [40, 41, 42, 0, -1, 11])
+    want = kv.clone()
+    want[:, :, [40, 41, 42]] = kv[:, :, [3, 4, 3]]
+    assert code == 0 and torch.equal(a, want)
+    a, code = run([3, 50, 4], [40, 41, 1000])
+    want = kv.clone()
+    want[:, :, 40] = kv[:, :, 3]
+    assert code == Status.BAD_PAGE and torch.equal(a, want)
+    a, code = run([3, 4, 40, 5], [40, 41, 42, 41])                # 40 is a source too; 41 is given twice
+    want = kv.clone()
+    want[:, :, 42], want[:, :, 41] = kv[:, :, 40], kv[:, :, 5]
+    assert code == Status.PAGE_CONFLICT and torch.equal(a, want)
+    assert torch.equal(run([], [])[0], kv)
+
+
+def test_offsets_beyond_32_bits():
+    """Planes of 2.6 GB, so that pages at the end start beyond 2^32 bytes."""
+    kv = torch.empty(1, 2, 80, 1, 32768, 512, dtype=torch.bfloat16, device=DEV)
+    kv[:, :, 79].normal_()
+    copy_pages(kv, ints([79]), ints([78]))
+    assert torch.equal(kv[:, :, 78], kv[:, :, 79])
+    t, refs, remap, live = compact_pages(kv, ints([[79]]), ints([32768]))
+    assert t.tolist() == [[0]] and torch.equal(kv[:, :, 0], kv[:, :, 79])
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_a_cache_followed_token_by_token(seed):
+    """Rows fork, grow, are freed and compacted at random; each token's K and V are its number, and every row has to read back its own tokens."""
+    r = random.Random(seed)
+    page, rows, width = r.choice([1, 3, 8]), 9, 12
+    cache = PagedCache(2, 60 if page == 1 else 40, 1, page, 64, rows, width * page)
+    tokens, counter = [[] for _ in range(rows)], 0
+    inv = torch.zeros(0, device=DEV)
+    for step in range(60):
+        parents = [r.choice([i, i, i, r.randrange(rows), -1]) for i in range(rows)]
+        grow = [r.choice([0, 1, 1, 3]) for _ in range(rows)]
+        cache.fork(ints(parents), ints(grow))
+        lens, old = cache.lens.tolist(), tokens
+        tokens = []
+        for i, p in enumerate(parents):
+            before = list(old[p]) if p >= 0 else []
+            assert lens[i] in (len(before), len(before) + (grow[i] if p >= 0 else 0))
+            new = lens[i] - len(before)
+            tokens.append(before + list(range(counter, counter + new)))
+            counter += new
+        at = [(i, j) for i in range(rows) for j in range(len(tokens[i])) if tokens[i][j] >= counter - sum(grow) and j >= len(old[parents[i]] if parents[i] >= 0 else [])]
+        if at:
+            for layer in range(2):
+                x = torch.tensor([float(tokens[i][j] % 199 + layer) for i, j in at], device=DEV)[:, None, None].expand(-1, 1, 64).to(torch.bfloat16).contiguous()
+                cache.append(layer, x, x, -x, ints([j for _, j in at]), ints([i for i, _ in at]), inv)
+        if r.random() < 0.2:
+            live = int(cache.compact())
+            assert live == int((cache.refs > 0).sum()) and not cache.refs[live:].any()
+        table, refs = cache.table.tolist(), cache.refs.tolist()
+        assert refs == [held(table, lens, page).get(p, 0) for p in range(len(refs))]
+        for i in range(rows):
+            for layer in range(2):
+                for j, t in enumerate(tokens[i]):
+                    slot = cache.kv[layer, :, table[i][j // page], 0, j % page, 0].tolist() if step % 10 == 9 else None
+                    assert slot is None or slot == [t % 199 + layer, -(t % 199 + layer)], (step, i, j)
+    if int(cache.status) not in (0, Status.NO_PAGES):
+        cache.check()
+
+
+def test_check_raises_what_was_latched():
+    cache = PagedCache(1, 2, 1, 4, 64, 2, 40)
+    cache.fork(grow=4)
+    cache.check()
+    cache.fork(grow=1)
+    assert cache.lens.tolist() == [4, 4]
+    with pytest.raises(KernelError, match="NO_PAGES"):
+        cache.check()
+
+
+def test_a_captured_step_goes_on_from_replay_to_replay():
+    cache, twin = (PagedCache(1, 30, 1, 4, 64, 3, 64) for _ in range(2))
+    parents = ints([0, 1, 2])
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        cache.fork(parents, 1)
+    graph = torch.cuda.CUDAGraph()
+    with graph_capture(graph, st):
+        cache.fork(parents, 1)
+    twin.fork(parents, 1)
+    for p in ([0, 0, 1], [2, 1, 0], [0, -1, 0], [0, 1, 2], [0, 0, 0]):
+        parents.copy_(ints(p))
+        graph.replay()
+        twin.fork(parents, 1)
+        assert torch.equal(cache.table, twin.table) and torch.equal(cache.lens, twin.lens) and torch.equal(cache.refs, twin.refs)
+    cache.check()
