@@ -45,20 +45,25 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, finished:
         raise ValueError(f"{what}: finished is bool [requests, beams], with an end token of the vocabulary")
     check_status(what, status)
     device = same_cuda_device(what, logits, scores, finished, status)
-    best = torch.empty(batch, k, dtype=torch.float32, device=device)
-    rows = torch.empty(batch, k, dtype=torch.int32, device=device)
-    tokens = torch.empty(batch, k, dtype=torch.int32, device=device)
+    best = scores.new_empty((batch, k))
+    rows, tokens = scores.new_empty((batch, k), dtype=torch.int32), scores.new_empty((batch, k), dtype=torch.int32)
     if batch:
         L = lib()
-        scratch = torch.empty(batch * beams * L.nexrt_beam_slices(vocab) * (k + 2), dtype=torch.int64, device=device)
-        strides = longs(logits.stride(0), logits.stride(1), *scores.stride(), *(finished.stride() if finished is not None else (0, 0)))
-        on_device(device, lambda st: L.nexrt_beam_select(ptr(logits), ptr(scores), ptr(finished), strides, ptr(best), ptr(rows), ptr(tokens), ptr(scratch), ptr(status), batch,
-                                                         beams, vocab, k, eos, TYPES[logits.dtype], st), what)
+        scratch = scores.new_empty(batch * beams * L.nexrt_beam_slices(vocab) * (k + 2), dtype=torch.int64)
+        strides = longs(*logits.stride()[:2], *scores.stride(), *(finished.stride() if finished is not None else (0, 0)))
+        on_device(device, lambda st: L.nexrt_beam_select(
+            logits.data_ptr(), scores.data_ptr(), ptr(finished), strides, best.data_ptr(), rows.data_ptr(), tokens.data_ptr(), scratch.data_ptr(), ptr(status), batch, beams,
+            vocab, k, eos, TYPES[logits.dtype], st), what)
     return best, rows, tokens
 
 
-def _row_dense(t: torch.Tensor) -> bool:
-    return t.dim() > 0 and (t.shape[0] == 0 or t[0].is_contiguous())
+def _rows_of(what: str, t: torch.Tensor, n: int) -> Tuple[int, int, int]:
+    """(address, bytes between rows, bytes of a row) of a tensor of ``n`` dense rows."""
+    shape = t.shape
+    if len(shape) == 0 or shape[0] != n or not (t.is_contiguous() or n == 0 or t[0].is_contiguous()):
+        raise ValueError(f"{what}: every tensor has {n} rows, each of them dense")
+    size = t.element_size()
+    return t.data_ptr(), t.stride()[0] * size, t.numel() // n * size if n else 0
 
 
 def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Optional[Sequence[torch.Tensor]] = None, status: Optional[torch.Tensor] = None) -> List[torch.Tensor]:
@@ -71,23 +76,32 @@ def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Op
     n = rows.numel()
     if not tensors:
         return []
-    n_in = tensors[0].shape[0] if tensors[0].dim() else -1
-    if any(t.dim() == 0 or t.shape[0] != n_in or not _row_dense(t) for t in tensors):
-        raise ValueError(f"{what}: tensors have the same number of rows, each of them dense")
+    n_in = tensors[0].shape[0] if tensors[0].dim() else 0
     if out is None:
-        out = [torch.empty((n, *t.shape[1:]), dtype=t.dtype, device=t.device) for t in tensors]
-    if len(out) != len(tensors) or any(o.dtype != t.dtype or o.shape != (n, *t.shape[1:]) or not _row_dense(o) for o, t in zip(out, tensors)):
-        raise ValueError(f"{what}: out has {n} dense rows for every tensor")
+        out = [t.new_empty((n, *t.shape[1:])) for t in tensors]
+    if len(out) != len(tensors):
+        raise ValueError(f"{what}: one out for every tensor")
     check_status(what, status)
+    moves, spans = [], []
+    for t, o in zip(tensors, out):
+        src, src_row, size = _rows_of(what, t, n_in)
+        dst, dst_row, out_size = _rows_of(what, o, n)
+        if o.dtype != t.dtype or o.shape[1:] != t.shape[1:]:
+            raise ValueError(f"{what}: out has the tensors' types and rows")
+        if out_size:
+            moves.append((src, dst, src_row, dst_row, out_size))
+            spans += ((dst, dst + (n - 1) * dst_row + out_size, 1), (src, src + max(n_in - 1, 0) * src_row + size, 0))
     device = same_cuda_device(what, *tensors, *out, rows, status)
-    held = {t.untyped_storage().data_ptr() for t in tensors if t.numel()}
-    if any(o.numel() and o.untyped_storage().data_ptr() in held for o in out):
-        raise ValueError(f"{what}: out shares memory with the tensors")
-    cols, r0, r1 = (1, rows.stride(0), 0) if rows.dim() == 1 else (max(1, rows.shape[1]), rows.stride(0), rows.stride(1))
-    live = [(t, o) for t, o in zip(tensors, out) if o.numel()]
-    for i in range(0, len(live), _TENSORS):
-        part = live[i : i + _TENSORS]
-        ins, outs = ((ctypes.c_void_p * len(part))(*(p[j].data_ptr() for p in part)) for j in (0, 1))
-        meta = longs(*(x for t, o in part for x in (t.stride(0) * t.element_size(), o.stride(0) * o.element_size(), t[0].numel() * t.element_size())))
-        on_device(device, lambda st: lib().nexrt_reorder_rows(ins, outs, meta, len(part), ptr(rows), r0, r1, cols, n, n_in, ptr(status), st), what)
+    ends = [0, 0]
+    for first, end, side in sorted(spans):
+        if first < ends[1 - side]:
+            raise ValueError(f"{what}: out shares memory with the tensors")
+        ends[side] = max(ends[side], end)
+    cols = max(1, rows.shape[1]) if rows.dim() == 2 else 1
+    r0, r1 = rows.stride() if rows.dim() == 2 else (rows.stride()[0], 0)
+    for i in range(0, len(moves), _TENSORS):
+        part = moves[i : i + _TENSORS]
+        pointers = ctypes.c_void_p * len(part)
+        ins, outs, meta = pointers(*[m[0] for m in part]), pointers(*[m[1] for m in part]), longs(*[x for m in part for x in m[2:]])
+        on_device(device, lambda st: lib().nexrt_reorder_rows(ins, outs, meta, len(part), rows.data_ptr(), r0, r1, cols, n, n_in, ptr(status), st), what)
     return list(out)

@@ -205,23 +205,25 @@ def longs(*values: int):
     return (c_int64 * len(values))(*values)
 
 
-def on_device(device: torch.device, call, what: str) -> None:
-    """``call(stream)`` on ``device``'s current stream, with that device current: the operators' tensors may lie on another one."""
-    if device.index == torch.cuda.current_device():
-        check(call(torch.cuda.current_stream(device).cuda_stream), what)
-        return
-    with torch.cuda.device(device):
-        check(call(torch.cuda.current_stream(device).cuda_stream), what)
+def on_device(device: int, call, what: str) -> None:
+    """``call(stream)`` on the current stream of CUDA device ``device``, with that device current: the operators' tensors may lie on another one."""
+    if device == torch.cuda.current_device():
+        err = call(torch._C._cuda_getCurrentRawStream(device))     # 0.1 us; torch.cuda.current_stream makes a Stream object, 2.2 us
+    else:
+        with torch.cuda.device(device):
+            err = call(torch._C._cuda_getCurrentRawStream(device))
+    if err:
+        check(err, what)
 
 
-def same_cuda_device(what: str, *tensors: Optional[torch.Tensor]) -> torch.device:
-    """The CUDA device that all the tensors given lie on; a ``ValueError`` where there is none."""
-    device = tensors[0].device
+def same_cuda_device(what: str, *tensors: Optional[torch.Tensor]) -> int:
+    """Index of the CUDA device that all the tensors given lie on; a ``ValueError`` where there is none."""
+    device = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: tensors on {device} and {t.device}")
-    if device.type != "cuda":
-        raise ValueError(f"{what} runs on a CUDA device, the tensors are on {device}")
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
+    if device < 0:
+        raise ValueError(f"{what} runs on a CUDA device, the tensors are on {tensors[0].device}")
     return device
 
 

@@ -37,19 +37,22 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     does one whose scores are all -inf.  Returns ``out [rows, heads, dim]``, with ``return_lse`` also fp32 ``[rows, heads]``: the natural
     logarithm of the sum of exp of the scores.  Keys on a page that the table does not name count as masked and latch ``BAD_PAGE``."""
     what = "paged_attention"
-    if q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float16) or q.stride(2) != 1:
+    kind, shape, q_s = q.dtype, q.shape, q.stride()
+    if len(shape) != 3 or kind not in (torch.bfloat16, torch.float16) or q_s[2] != 1:
         raise ValueError(f"{what}: q is [rows, heads, dim] in bf16 or fp16 with a contiguous last dimension")
-    rows, heads, dim = q.shape
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1 or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+    rows, heads, dim = shape
+    pool, pool_s = k_pages.shape, k_pages.stride()
+    if len(pool) != 4 or pool != v_pages.shape or pool_s != v_pages.stride() or pool_s[3] != 1 or k_pages.dtype != kind or v_pages.dtype != kind:
         raise ValueError(f"{what}: k_pages and v_pages are [pages, kv heads, slots, dim] of q's type, with the same strides and a contiguous last dimension")
-    pages, kv_heads, slots = k_pages.shape[:3]
-    if dim not in HEAD_DIMS or k_pages.shape[3] != dim:
+    pages, kv_heads, slots, pool_dim = pool
+    if dim not in HEAD_DIMS or pool_dim != dim:
         raise ValueError(f"{what}: head dimensions are {HEAD_DIMS}, those of q and of the pages the same")
     if kv_heads < 1 or slots < 1 or heads < 1 or heads % kv_heads:
         raise ValueError(f"{what}: {heads} heads on {kv_heads} kv heads")
-    if any(s % 8 for s in k_pages.stride()[:3]) or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
+    k_ptr, v_ptr = k_pages.data_ptr(), v_pages.data_ptr()
+    if (pool_s[0] | pool_s[1] | pool_s[2]) % 8 or (k_ptr | v_ptr) % 16:
         raise ValueError(f"{what}: rows of the pages start on 16-byte boundaries")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != rows or table.stride(1) != 1:
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != rows or table.stride()[1] != 1:
         raise ValueError(f"{what}: table is int32 [rows, pages of a row] with contiguous rows")
     if lens.dtype != torch.int32 or lens.shape != (rows,) or not lens.is_contiguous():
         raise ValueError(f"{what}: lens is int32 [rows]")
@@ -59,40 +62,42 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError(f"{what}: slopes is fp32 [heads]")
     check_status(what, status)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != kind or out.stride()[2] != 1:
         raise ValueError(f"{what}: out is like q")
-    lse = torch.empty(rows, heads, dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
     device = same_cuda_device(what, q, k_pages, v_pages, table, lens, slopes, out, status)
     if rows:
         L = lib()
-        width = table.shape[1]
+        width, o_s = table.shape[1], out.stride()
         window = min(window, 2**31 - 1)
         ctas = L.nexrt_paged_ctas(rows, heads, kv_heads, width, slots, window)
-        scratch = torch.empty(2 * ctas * 16 * (dim + 2), dtype=torch.float32, device=device)
-        strides = longs(q.stride(0), q.stride(1), out.stride(0), out.stride(1), *k_pages.stride()[:3], table.stride(0), heads)
+        scratch = q.new_empty(2 * ctas * 16 * (dim + 2), dtype=torch.float32)
+        strides = longs(q_s[0], q_s[1], o_s[0], o_s[1], pool_s[0], pool_s[1], pool_s[2], table.stride()[0], heads)
         on_device(device, lambda st: L.nexrt_paged_attn(
-            ptr(q), ptr(k_pages), ptr(v_pages), ptr(table), ptr(lens), ptr(slopes), ptr(out), ptr(lse), ptr(scratch), ptr(status), strides, rows, heads, kv_heads, dim,
-            width, slots, pages, window, TYPES[q.dtype], dim**-0.5 if scale is None else scale, softcap, ctas, st), what)
+            q.data_ptr(), k_ptr, v_ptr, table.data_ptr(), lens.data_ptr(), ptr(slopes), out.data_ptr(), ptr(lse), scratch.data_ptr(), ptr(status), strides, rows, heads,
+            kv_heads, dim, width, slots, pages, window, TYPES[kind], dim**-0.5 if scale is None else scale, softcap, ctas, st), what)
     return (out, lse) if return_lse else out
 
 
 def _pool(what: str, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor):
     """Arguments of the page kernels: base, planes, pages, heads, slots, bytes of a slot."""
-    if kv.dim() != 6 or kv.shape[1] != 2 or not kv.is_contiguous():
+    shape = kv.shape
+    if len(shape) != 6 or shape[1] != 2 or not kv.is_contiguous():
         raise ValueError(f"{what}: kv is a contiguous [layers, 2, pages, kv heads, slots, dim]")
-    if kv.shape[3] < 1 or kv.shape[4] < 1 or kv.shape[5] * kv.element_size() % 16 or kv.shape[5] < 1 or kv.data_ptr() % 16:
+    base, slot = kv.data_ptr(), shape[5] * kv.element_size()
+    if shape[3] < 1 or shape[4] < 1 or slot < 16 or slot % 16 or base % 16:
         raise ValueError(f"{what}: a slot of the pool takes a multiple of 16 bytes and starts on such a boundary")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+    if table.dtype != torch.int32 or table.dim() != 2 or table.stride()[1] != 1:
         raise ValueError(f"{what}: table is int32 [rows, pages of a row] with contiguous rows")
-    if lens.dtype != torch.int32 or lens.shape != (table.shape[0],) or not lens.is_contiguous():
+    if lens.dtype != torch.int32 or lens.shape != table.shape[:1] or not lens.is_contiguous():
         raise ValueError(f"{what}: lens is int32 [rows]")
-    return ptr(kv), 2 * kv.shape[0], kv.shape[2], kv.shape[3], kv.shape[4], kv.shape[5] * kv.element_size()
+    return base, 2 * shape[0], shape[2], shape[3], shape[4], slot
 
 
 def _fresh(what: str, name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor, *old: torch.Tensor) -> torch.Tensor:
     if t is None:
-        return torch.empty(shape, dtype=torch.int32, device=like.device)
+        return like.new_empty(shape)
     if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or (t.numel() and t.stride(-1) != 1) or (t.dim() == 1 and not t.is_contiguous()):
         raise ValueError(f"{what}: {name} is int32 {list(shape)} with contiguous rows")
     for o in old:
@@ -126,9 +131,10 @@ def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent
     lens_out = _fresh(what, "lens_out", lens_out, (n,), table, lens, parents, each)
     refs = _fresh(what, "refs", refs, (pages,), table, lens, parents, each, table)
     device = same_cuda_device(what, kv, table, lens, parents, each, table_out, lens_out, refs, status)
-    scratch = torch.empty(pages + 3 * n, dtype=torch.int32, device=device)
-    on_device(device, lambda st: lib().nexrt_page_fork(*pool, ptr(table), table.stride(0), table.shape[0], width, ptr(lens), ptr(parents), ptr(each), 0 if each is not None else grow,
-                                                       ptr(table_out), table_out.stride(0), ptr(lens_out), ptr(refs), ptr(scratch), ptr(status), n, st), what)
+    scratch = table.new_empty(pages + 3 * n)
+    on_device(device, lambda st: lib().nexrt_page_fork(
+        *pool, table.data_ptr(), table.stride()[0], table.shape[0], width, lens.data_ptr(), parents.data_ptr(), ptr(each), 0 if each is not None else grow, table_out.data_ptr(),
+        table_out.stride()[0], lens_out.data_ptr(), refs.data_ptr(), scratch.data_ptr(), ptr(status), n, st), what)
     return table_out, lens_out, refs
 
 
@@ -143,12 +149,12 @@ def compact_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, 
     check_status(what, status)
     table_out = _fresh(what, "table_out", table_out, tuple(table.shape), table, table)
     refs = _fresh(what, "refs", refs, (pages,), table, lens, table)
-    remap = torch.empty(pages, dtype=torch.int32, device=table.device)
-    live = torch.empty(1, dtype=torch.int32, device=table.device)
+    remap, live = table.new_empty(pages), table.new_empty(1)
     device = same_cuda_device(what, kv, table, lens, table_out, refs, status)
-    scratch = torch.empty(5 * pages + 1, dtype=torch.int32, device=device)
-    on_device(device, lambda st: lib().nexrt_page_compact(*pool, ptr(table), table.stride(0), table.shape[0], table.shape[1], ptr(lens), ptr(table_out), table_out.stride(0), ptr(refs),
-                                                          ptr(remap), ptr(live), ptr(scratch), ptr(status), st), what)
+    scratch = table.new_empty(5 * pages + 1)
+    on_device(device, lambda st: lib().nexrt_page_compact(
+        *pool, table.data_ptr(), table.stride()[0], table.shape[0], table.shape[1], lens.data_ptr(), table_out.data_ptr(), table_out.stride()[0], refs.data_ptr(),
+        remap.data_ptr(), live.data_ptr(), scratch.data_ptr(), ptr(status), st), what)
     return table_out, refs, remap, live
 
 
@@ -162,8 +168,8 @@ def copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *, status
     pool = _pool(what, kv, src.view(-1, 1), src)
     check_status(what, status)
     device = same_cuda_device(what, kv, src, dst, status)
-    scratch = torch.empty(3 * src.numel(), dtype=torch.int32, device=device)
-    on_device(device, lambda st: lib().nexrt_page_copy(*pool, ptr(src), ptr(dst), src.numel(), ptr(scratch), ptr(status), st), what)
+    scratch = src.new_empty(3 * src.numel())
+    on_device(device, lambda st: lib().nexrt_page_copy(*pool, src.data_ptr(), dst.data_ptr(), src.numel(), scratch.data_ptr(), ptr(status), st), what)
 
 
 class PagedCache:

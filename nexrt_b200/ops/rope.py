@@ -48,13 +48,17 @@ def rope_frequencies(rotary: int, theta: float, scaling: Optional[str] = None, f
     return torch.tensor(inv, dtype=torch.float32), scale
 
 
-def _heads(what: str, x: torch.Tensor, tokens: int, dim: int, dtype: torch.dtype) -> None:
-    if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != dim or x.dtype != dtype or x.stride(2) != 1:
-        raise ValueError(f"{what}: tensors of heads are [tokens, heads, dim] of one type with a contiguous last dimension")
+def _heads(what: str, x: torch.Tensor, tokens: int, dim: int, dtype: torch.dtype) -> Tuple[int, int, int]:
+    """(heads, stride of a token, stride of a head) of a tensor of heads."""
+    if x.dim() == 3 and x.dtype == dtype:
+        shape, strides = x.shape, x.stride()
+        if shape[0] == tokens and shape[2] == dim and strides[2] == 1:
+            return shape[1], strides[0], strides[1]
+    raise ValueError(f"{what}: tensors of heads are [tokens, heads, dim] of one type with a contiguous last dimension")
 
 
 def _common(what, q, positions, inv_freq, norms):
-    if q.dim() != 3 or q.dtype not in TYPES or q.stride(2) != 1:
+    if q.dim() != 3 or q.dtype not in TYPES or q.stride()[2] != 1:
         raise ValueError(f"{what}: q is [tokens, heads, dim] in bf16, fp16 or fp32 with a contiguous last dimension")
     tokens, _, dim = q.shape
     if dim < 8 or dim > MAX_DIM or dim % 8:
@@ -66,25 +70,26 @@ def _common(what, q, positions, inv_freq, norms):
     for w in norms:
         if w is not None and (w.dtype != torch.float32 or w.shape != (dim,) or not w.is_contiguous()):
             raise ValueError(f"{what}: norm multipliers are fp32 [dim]")
-    return tokens, dim
+    return tokens, dim, 2 * inv_freq.numel()
 
 
 def rope(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0, norm: Optional[torch.Tensor] = None,
          eps: float = 1e-6, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``q [tokens, heads, dim]`` at ``positions`` int32 ``[tokens]``, rotated (after an RMSNorm with the multiplier ``norm``, if given); ``out`` may be ``q``."""
-    tokens, dim = _common("rope", q, positions, inv_freq, (norm,))
+    tokens, dim, rotary = _common("rope", q, positions, inv_freq, (norm,))
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _heads("rope", out, tokens, dim, q.dtype)
-    if out.shape[1] != q.shape[1]:
+        out = q.new_empty(q.shape)
+    hq, q_t, q_h = _heads("rope", q, tokens, dim, q.dtype)
+    ho, o_t, o_h = _heads("rope", out, tokens, dim, q.dtype)
+    if ho != hq:
         raise ValueError("rope: out has other heads than q")
     device = same_cuda_device("rope", q, positions, inv_freq, norm, out)
     if q.numel() == 0:
         return out
-    strides = longs(q.stride(0), q.stride(1), 0, 0, 0, 0, out.stride(0), out.stride(1), 0, 0, 0, 0)
+    strides = longs(q_t, q_h, 0, 0, 0, 0, o_t, o_h, 0, 0, 0, 0)
     kind = TYPES[q.dtype]
-    on_device(device, lambda st: lib().nexrt_rope_append(ptr(q), None, None, ptr(positions), None, ptr(out), None, None, None, ptr(inv_freq), ptr(norm), None, None, strides,
-                                                         tokens, q.shape[1], 0, dim, 2 * inv_freq.numel(), int(interleaved), 0, 0, 1, 0, kind, kind, scale, eps, st), "rope")
+    on_device(device, lambda st: lib().nexrt_rope_append(q.data_ptr(), None, None, positions.data_ptr(), None, out.data_ptr(), None, None, None, inv_freq.data_ptr(), ptr(norm),
+                                                         None, None, strides, tokens, hq, 0, dim, rotary, interleaved, 0, 0, 1, 0, kind, kind, scale, eps, st), "rope")
     return out
 
 
@@ -98,33 +103,37 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     A negative ``rows[i]`` is padding: its q is rotated, nothing is stored.  A position whose page the table does not name is left out
     and latches ``BAD_PAGE`` in ``status``.  Two tokens of a call with the same slot leave it undefined."""
     what = "rope_append"
-    tokens, dim = _common(what, q, positions, inv_freq, (q_norm, k_norm))
-    _heads(what, k, tokens, dim, q.dtype)
-    _heads(what, v, tokens, dim, q.dtype)
-    if k.shape != v.shape:
+    tokens, dim, rotary = _common(what, q, positions, inv_freq, (q_norm, k_norm))
+    kind, pool_kind = q.dtype, k_pages.dtype
+    hq, q_t, q_h = _heads(what, q, tokens, dim, kind)
+    hk, k_t, k_h = _heads(what, k, tokens, dim, kind)
+    hv, v_t, v_h = _heads(what, v, tokens, dim, kind)
+    if hk != hv:
         raise ValueError(f"{what}: k and v have the same heads")
     if rows.dtype != torch.int32 or rows.shape != (tokens,) or not rows.is_contiguous():
         raise ValueError(f"{what}: rows is int32 [tokens]")
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride() or k_pages.dtype != v_pages.dtype or k_pages.stride(3) != 1:
+    pool, pool_s = k_pages.shape, k_pages.stride()
+    if len(pool) != 4 or pool != v_pages.shape or pool_s != v_pages.stride() or v_pages.dtype != pool_kind or pool_s[3] != 1:
         raise ValueError(f"{what}: k_pages and v_pages are [pages, kv heads, slots, dim] with the same strides and a contiguous last dimension")
-    if k_pages.shape[1] != k.shape[1] or k_pages.shape[3] != dim or k_pages.shape[2] < 1:
+    if pool[1] != hk or pool[3] != dim or pool[2] < 1:
         raise ValueError(f"{what}: the pages have other heads than k")
-    if k_pages.dtype not in (torch.bfloat16, torch.float16) or q.dtype not in (k_pages.dtype, torch.float32):
+    if pool_kind not in (torch.bfloat16, torch.float16) or kind not in (pool_kind, torch.float32):
         raise ValueError(f"{what}: pages are bf16 or fp16, q, k and v the same or fp32")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+    if table.dtype != torch.int32 or table.dim() != 2 or table.stride()[1] != 1:
         raise ValueError(f"{what}: table is int32 [rows, pages of a row] with contiguous rows")
     check_status(what, status)
     if out is None:
-        out = torch.empty(q.shape, dtype=k_pages.dtype, device=q.device)
-    _heads(what, out, tokens, dim, k_pages.dtype)
-    if out.shape[1] != q.shape[1]:
+        out = q.new_empty(q.shape, dtype=pool_kind)
+    ho, o_t, o_h = _heads(what, out, tokens, dim, pool_kind)
+    if ho != hq:
         raise ValueError(f"{what}: out has other heads than q")
     device = same_cuda_device(what, q, k, v, positions, rows, k_pages, v_pages, table, inv_freq, q_norm, k_norm, out, status)
     if tokens == 0:
         return out
-    strides = longs(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1), *k_pages.stride()[:3], table.stride(0))
+    table_rows, width = table.shape
+    strides = longs(q_t, q_h, k_t, k_h, v_t, v_h, o_t, o_h, pool_s[0], pool_s[1], pool_s[2], table.stride()[0])
     on_device(device, lambda st: lib().nexrt_rope_append(
-        ptr(q), ptr(k), ptr(v), ptr(positions), ptr(rows), ptr(out), ptr(k_pages), ptr(v_pages), ptr(table), ptr(inv_freq), ptr(q_norm), ptr(k_norm), ptr(status), strides,
-        tokens, q.shape[1], k.shape[1], dim, 2 * inv_freq.numel(), int(interleaved), table.shape[0], table.shape[1], k_pages.shape[2], k_pages.shape[0], TYPES[q.dtype],
-        TYPES[k_pages.dtype], scale, eps, st), what)
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), rows.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
+        inv_freq.data_ptr(), ptr(q_norm), ptr(k_norm), ptr(status), strides, tokens, hq, hk, dim, rotary, interleaved, table_rows, width, pool[2], pool[0], TYPES[kind],
+        TYPES[pool_kind], scale, eps, st), what)
     return out
