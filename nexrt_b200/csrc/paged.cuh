@@ -50,4 +50,14 @@ __host__ __device__ __forceinline__ int owner_of(int64_t x, int64_t total, int n
 // CTAs that get work: at most `grid`, no more than there are chunks.
 __host__ __device__ __forceinline__ int active_ctas(int64_t total, int grid) { return total < grid ? (total > 0 ? static_cast<int>(total) : 1) : grid; }
 
+// ---- asynchronous copies of 16 bytes into shared memory -------------------------------------------------------------------
+#ifdef __CUDACC__
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
+    const int n = valid ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+#endif
+
 }  // namespace nexrt

@@ -46,12 +46,6 @@ template <int D> constexpr size_t ring_bytes() { return static_cast<size_t>(kPaW
 template <int D> constexpr size_t merge_bytes() { return sizeof(float) * kPaWarps * kPaRows * (D + 4); }
 template <int D> constexpr size_t paged_smem() { return (ring_bytes<D>() > merge_bytes<D>() ? ring_bytes<D>() : merge_bytes<D>()) + D / 16 * 512; }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
-    const int n = valid ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }

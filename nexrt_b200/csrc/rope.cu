@@ -6,10 +6,11 @@
 // taken in turns in 64 bits and reduced before it is rounded to 32: at position 262144 a 32-bit product is 0.016 rad off, and
 // sinpi / cospi of a reduced turn need no range reduction of their own.
 //
-// Bound by the bytes (each value read and written once).  A CTA takes one token: its sines serve all its heads, and lie in the
-// registers of the lanes that need them, multiplied with the norm's multipliers.  A head lies over 8, 16 or 32 lanes, eight
-// values a lane: its sum of squares is three to five shuffles, and a value meets the other one of its pair in its own lane
-// (interleaved), by a shuffle of the raw words, or, where half the rotated dims are no multiple of eight, in shared memory.
+// Bound by the bytes (each value read and written once), with the instructions close behind.  The heads of all tokens are cut into
+// equal runs, one per resident warp, so the last wave is as full as the first; a warp keeps four steps of loads in flight over
+// the tokens' borders and makes a token's sines itself, so no warp waits for another.  The factors of a token - sines times the
+// norm's multipliers - stay in registers for all its heads.  A head lies over 4, 8 or 16 lanes, 16 values a lane: its sum of
+// squares is two to four shuffles for several heads at once; sums and products go two values an instruction.
 #include "api.h"
 #include "paged.cuh"
 
@@ -105,168 +106,261 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 
 constexpr int kRopeThreads = 128;
+constexpr int kRopeResident = 6;        // CTAs on an SM
 constexpr int kRopeWarps = kRopeThreads / 32;
 
-// How a value meets the other one of its pair.
-enum RopeLayout { kPairsInLane, kPairsByShuffle, kPairsByLine };
+// How a value meets the other one of its pair: (2 i, 2 i + 1) are in one lane; the rotated dims lie in the first halves of the lanes'
+// values, a shuffle apart; they are the two halves of a lane's values; anything else goes through shared memory, and so do tensors that
+// cannot be read 16 bytes at a time.
+enum RopeLayout { kPairsInLane, kPairsByShuffle, kPairsAcross, kPairsByLine };
 
-// LPH lanes hold a head (8 values each): 8 for dims up to 64, 16 up to 128, 32 up to 256.
+// LPH lanes hold a head, 16 values each: 4 for dims up to 64, 8 up to 128, 16 up to 256.  Values 8 sub .. and LPH * 8 + 8 sub .. are lane
+// sub's, so that a warp reads whole lines.
 template <typename TI, typename TO, int LPH, int LAYOUT>
-__global__ void __launch_bounds__(kRopeThreads, sizeof(TI) == 4 ? 6 : 7) rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const __grid_constant__ RopeArgs a) {
     constexpr int kHeads = 32 / LPH;                     // heads that a warp turns at once
-    constexpr int kAhead = sizeof(TI) == 4 ? 2 : 4;      // of which so many are in flight
-    __shared__ float2 turn[128];                         // (cos, sin) of the token's pairs
-    __shared__ int64_t slot_s;                           // where the token's slot lies in the pools, -1: nowhere
-    __shared__ float line[LAYOUT == kPairsByLine ? kRopeWarps : 1][256];
+    constexpr int kAhead = 4;                            // steps of which so many are in flight
+    constexpr int kFar = LPH * 8;                        // from a lane's first eight values to its second
+    constexpr bool kVec = LAYOUT != kPairsByLine;
+    constexpr int kWide = sizeof(TI) == 4 ? 2 : 1;       // 16-byte pieces of eight values
+    __shared__ float2 turns_s[kRopeWarps][128];          // (cos, sin) of a warp's token's pairs
+    __shared__ float line[LAYOUT == kPairsByLine ? kRopeWarps : 1][LAYOUT == kPairsByLine ? 512 : 1];
+    __shared__ uint4 ring_s[kVec ? kRopeWarps : 1][kVec ? kAhead : 1][2 * kWide][32];   // a lane reads back what it copied itself
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LPH;
     const int e0 = sub * 8, half = a.rotary / 2;
-    const bool in_dim = e0 < a.dim;
-    const int heads = a.q_heads + 2 * a.kv_heads, qk = a.q_heads + a.kv_heads;
-    const int64_t t = blockIdx.x;
-    const TI* const q = static_cast<const TI*>(a.q) + t * a.q_t + e0;
-    const TI* const k = static_cast<const TI*>(a.k) + t * a.k_t + e0;
-    const TI* const v = static_cast<const TI*>(a.v) + t * a.v_t + e0;
-    TO* const q_out = static_cast<TO*>(a.q_out) + t * a.qo_t + e0;
+    const bool vec = kVec || a.vec;                      // 16-byte stores
+    const int heads = a.q_heads + 2 * a.kv_heads, qk = a.q_heads + a.kv_heads, steps = (heads + kHeads - 1) / kHeads;
+    float2* const turn = turns_s[warp];
 
-    // ---- a warp's heads lie side by side, so that few warps meet more than one kind; the first loads do not wait for the angles
-    const int per_warp = ((heads + kHeads - 1) / kHeads + kRopeWarps - 1) / kRopeWarps * kHeads;
-    const int end = min(heads, (warp + 1) * per_warp), first = warp * per_warp + lane / LPH;
-    Eight<TI> raw[kAhead];
-    auto fetch = [&](int h, Eight<TI>& r) {
-        if (!in_dim || h >= end) {
-            r.clear();
-            return;
-        }
-        r.load(h < a.q_heads ? q + static_cast<int64_t>(h) * a.q_h
-                             : (h < qk ? k + static_cast<int64_t>(h - a.q_heads) * a.k_h : v + static_cast<int64_t>(h - qk) * a.v_h), a.vec);
+    // ---- this warp's steps, of all tokens' (kHeads heads of one token each)
+    const int64_t total = static_cast<int64_t>(a.tokens) * steps;
+    const int n = gridDim.x * kRopeWarps, w_id = blockIdx.x * kRopeWarps + warp;
+    const int64_t begin = total * w_id / n;
+    int left = static_cast<int>(total * (w_id + 1) / n - begin), ahead = left;
+    if (left == 0) return;
+    int t = static_cast<int>(begin / steps), i = static_cast<int>(begin - static_cast<int64_t>(t) * steps);
+
+    uint4 (*const ring)[2 * kWide][32] = ring_s[kVec ? warp : 0];
+    int ft = t, fi = i;                                  // the step that is fetched next
+    auto source = [&](int t_, int h) -> const TI* {
+        if (h < a.q_heads) return static_cast<const TI*>(a.q) + t_ * a.q_t + static_cast<int64_t>(h) * a.q_h + e0;
+        if (h < qk) return static_cast<const TI*>(a.k) + t_ * a.k_t + static_cast<int64_t>(h - a.q_heads) * a.k_h + e0;
+        return static_cast<const TI*>(a.v) + t_ * a.v_t + static_cast<int64_t>(h - qk) * a.v_h + e0;
     };
+    auto fetch = [&](int at) {
+        const int h = fi * kHeads + lane / LPH;
+        if (ahead > 0 && h < heads) {
+            const TI* src = source(ft, h);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) fetch(first + i * kHeads, raw[i]);
-
-    const int pos = a.positions[t];
-    if (a.paged && threadIdx.x == kRopeThreads - 1) {
-        int64_t at = -1;
-        const int row = a.rows[t];
-        if (row >= 0) {                                  // a negative row is padding: nothing is stored for it
-            const int j = pos / a.table.page, page = pos < 0 ? -1 : page_at(a.table, row, j);
-            if (page >= 0) at = page * a.page_s + (pos - j * a.table.page) * a.slot_s;
-            else if (a.status) atomicCAS(a.status, 0, static_cast<int>(kStatusBadPage));
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int j = 0; j < kWide; ++j)
+                    cp16(static_cast<uint32_t>(__cvta_generic_to_shared(&ring[at][c * kWide + j][lane])), src + (e0 + c * kFar < a.dim ? c * kFar + j * 4 : 0), e0 + c * kFar < a.dim);
         }
-        slot_s = at;
+        cp_commit();
+        --ahead;
+        if (++fi == steps) {
+            fi = 0;
+            ++ft;
+        }
+    };
+    if (kVec) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) fetch(u);
     }
-    for (int i = threadIdx.x; i < half; i += kRopeThreads) {
-        double turns = static_cast<double>(pos) * static_cast<double>(a.inv_freq[i]) * 0.15915494309189533577;
-        turns -= rint(turns);
-        float s, c;
-        sincospif(2.f * static_cast<float>(turns), &s, &c);
-        turn[i] = make_float2(c * a.scale, s * a.scale);
-    }
-    __syncthreads();
-    const int64_t slot = a.paged ? slot_s : -1;
-    TO* const k_out = static_cast<TO*>(a.k_out) + slot + e0;
-    TO* const v_out = static_cast<TO*>(a.v_out) + slot + e0;
+
+    // ---- a token: its angles, and the entry of the table that its k and v need; the next one's position and row are on their way
+    int pos = 0, row = -1, entry = -1, next_pos = a.positions[t], next_row = a.paged ? a.rows[t] : -1;
+    auto begin_token = [&]() {
+        pos = next_pos;
+        row = next_row;
+        if (t + 1 < a.tokens) {
+            next_pos = a.positions[t + 1];
+            if (a.paged) next_row = a.rows[t + 1];
+        }
+        const int j = pos / a.table.page;
+        const bool named = row >= 0 && row < a.table.rows && pos >= 0 && j < a.table.width;
+        entry = named ? a.table.table[row * a.table.stride + j] : -1;
+        __syncwarp();
+        for (int p = lane; p < half; p += 32) {
+            double turns = static_cast<double>(pos) * static_cast<double>(a.inv_freq[p]) * 0.15915494309189533577;
+            turns -= rint(turns);
+            float s, c;
+            sincospif(2.f * static_cast<float>(turns), &s, &c);
+            turn[p] = make_float2(c * a.scale, s * a.scale);
+        }
+        __syncwarp();
+    };
 
     // ---- value i of the lane becomes r (x cw + other sw): cos and sin, and the norm's multipliers of both
-    float2 cw[4], sw[4];
+    float2 cw[2][4], sw[2][4];
     int kind = -1;                                       // whose they are: 0 q, 1 k
+    const bool pairs_in_lane = LAYOUT == kPairsInLane || (LAYOUT == kPairsByLine && a.interleaved);
     auto factors = [&](const float* w) {
-        float c[8], s[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int e = e0 + i;
-            c[i] = w != nullptr ? w[e] : 1.f;
-            s[i] = 0.f;
-            if (e < a.rotary) {
-                const bool second = LAYOUT == kPairsInLane ? (i & 1) : e >= half;
-                const int pair = LAYOUT == kPairsInLane ? e >> 1 : (second ? e - half : e);
-                const int other = LAYOUT == kPairsInLane ? e ^ 1 : (second ? e - half : e + half);
-                const float2 cs = turn[pair];
-                c[i] *= cs.x;
-                s[i] = (second ? cs.y : -cs.y) * (w != nullptr ? w[other] : 1.f);
+        for (int c = 0; c < 2; ++c) {
+            float cs_[8], sn[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = e0 + c * kFar + i;
+                cs_[i] = w != nullptr && e < a.dim ? w[e] : 1.f;
+                sn[i] = 0.f;
+                if (e < a.rotary) {
+                    const bool second = pairs_in_lane ? (i & 1) : e >= half;
+                    const int pair = pairs_in_lane ? e >> 1 : (second ? e - half : e);
+                    const int other = pairs_in_lane ? e ^ 1 : (second ? e - half : e + half);
+                    const float2 cs = turn[pair];
+                    cs_[i] *= cs.x;
+                    sn[i] = (second ? cs.y : -cs.y) * (w != nullptr ? w[other] : 1.f);
+                }
             }
-        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            cw[i] = make_float2(c[2 * i], c[2 * i + 1]);
-            sw[i] = make_float2(s[2 * i], s[2 * i + 1]);
+            for (int i = 0; i < 4; ++i) {
+                cw[c][i] = make_float2(cs_[2 * i], cs_[2 * i + 1]);
+                sw[c][i] = make_float2(sn[2 * i], sn[2 * i + 1]);
+            }
         }
     };
     const bool turned = e0 < a.rotary;
     const int from = !turned ? lane : (e0 < half ? lane + half / 8 : lane - half / 8);
     const float inv_dim = 1.f / static_cast<float>(a.dim);
 
-    for (int h0 = first; h0 - lane / LPH < end; h0 += kAhead * kHeads) {
+    begin_token();
+    for (int at = 0; left > 0; --left, at = at + 1 == kAhead ? 0 : at + 1) {
+        if (i == steps) {
+            i = 0;
+            ++t;
+            kind = -1;
+            begin_token();
+        }
+        const int h = i++ * kHeads + lane / LPH;
+        Eight<TI> raw[2];
+        if (kVec) {
+            cp_wait<kAhead - 1>();
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int h = h0 + u * kHeads;
-            if (h - lane / LPH >= end) break;            // the same for all lanes of the warp
-            // (a value that does not turn meets a zero: no 0 * infinity)
-            float2 x[4], other[4];
-            raw[u].values(x);
-            if (LAYOUT == kPairsByShuffle) {
-                Eight<TI> o;
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int i = 0; i < Eight<TI>::kWords; ++i) {
-                    o.w[i] = __shfl_sync(0xffffffffu, raw[u].w[i], from);
-                    o.w[i] = turned ? o.w[i] : 0u;
+                for (int j = 0; j < kWide; ++j) {
+                    const uint4 v = ring[at][c * kWide + j][lane];
+                    raw[c].w[4 * j] = v.x; raw[c].w[4 * j + 1] = v.y; raw[c].w[4 * j + 2] = v.z; raw[c].w[4 * j + 3] = v.w;
                 }
-                o.values(other);
-            } else if (LAYOUT == kPairsInLane) {
+        } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) other[i] = e0 + 2 * i < a.rotary ? make_float2(x[i].y, x[i].x) : make_float2(0.f, 0.f);
-            } else {
-                float* const mine = line[warp] + (lane - sub) * 8;
-                __syncwarp();
+            for (int c = 0; c < 2; ++c) {
+                if (h < heads && e0 + c * kFar < a.dim) raw[c].load(source(t, h) + c * kFar, a.vec);
+                else raw[c].clear();
+            }
+        }
+        float2 x[2][4];
+        raw[0].values(x[0]);
+        raw[1].values(x[1]);
+        float2 other[4];                             // of the first eight, by shuffle
+        if (LAYOUT == kPairsByShuffle) {
+            Eight<TI> o;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) *reinterpret_cast<float2*>(mine + e0 + 2 * i) = x[i];
-                __syncwarp();
+            for (int i = 0; i < Eight<TI>::kWords; ++i) {
+                o.w[i] = __shfl_sync(0xffffffffu, raw[0].w[i], from);
+                o.w[i] = turned ? o.w[i] : 0u;       // a value that does not turn meets a zero: no 0 * infinity
+            }
+            o.values(other);
+        }
+        float* const mine = line[LAYOUT == kPairsByLine ? warp : 0] + (lane - sub) * 16;
+        if (LAYOUT == kPairsByLine) {
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<float2*>(mine + e0 + c * kFar + 2 * i) = x[c][i];
+            __syncwarp();
+        }
+        float r = 1.f;
+        if (a.q_norm != nullptr || a.k_norm != nullptr) {
+            float2 sq = mul2(x[0][0], x[0][0]);
+#pragma unroll
+            for (int i = 1; i < 4; ++i) sq = fma2(x[0][i], x[0][i], sq);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sq = fma2(x[1][i], x[1][i], sq);
+            float ss = sq.x + sq.y;
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if ((h < a.q_heads ? a.q_norm : a.k_norm) != nullptr) r = rsqrtf(fmaf(ss, inv_dim, a.eps));
+        }
+        if (kVec) {
+            __syncwarp();
+            fetch(at);                               // into the place that was just read
+        }
+        if (h >= heads) continue;
+        if (h < qk) {
+            if (kind != (h < a.q_heads ? 0 : 1)) {
+                kind = h < a.q_heads ? 0 : 1;
+                factors(kind ? a.k_norm : a.q_norm);
+            }
+            const float2 rr = make_float2(r, r);
+            if (LAYOUT == kPairsByShuffle) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int e = e0 + 2 * i;
-                    other[i].x = e < a.rotary ? mine[e < half ? e + half : e - half] : 0.f;
-                    other[i].y = e + 1 < a.rotary ? mine[e + 1 < half ? e + 1 + half : e + 1 - half] : 0.f;
+                    x[0][i] = mul2(rr, fma2(other[i], sw[0][i], mul2(x[0][i], cw[0][i])));
+                    x[1][i] = mul2(rr, mul2(x[1][i], cw[1][i]));
                 }
-            }
-            float r = 1.f;
-            if (a.q_norm != nullptr || a.k_norm != nullptr) {
-                float2 sq = mul2(x[0], x[0]);
+            } else if (LAYOUT == kPairsAcross) {
 #pragma unroll
-                for (int i = 1; i < 4; ++i) sq = fma2(x[i], x[i], sq);
-                float ss = sq.x + sq.y;
-#pragma unroll
-                for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                if ((h < a.q_heads ? a.q_norm : a.k_norm) != nullptr) r = rsqrtf(fmaf(ss, inv_dim, a.eps));
-            }
-            fetch(h + kAhead * kHeads, raw[u]);
-            if (!in_dim || h >= end) continue;
-            if (h < qk) {
-                if (kind != (h < a.q_heads ? 0 : 1)) {
-                    kind = h < a.q_heads ? 0 : 1;
-                    factors(kind ? a.k_norm : a.q_norm);
+                for (int i = 0; i < 4; ++i) {
+                    const float2 y = x[0][i], z = x[1][i];
+                    x[0][i] = mul2(rr, fma2(z, sw[0][i], mul2(y, cw[0][i])));
+                    x[1][i] = mul2(rr, fma2(y, sw[1][i], mul2(z, cw[1][i])));
                 }
-                const float2 rr = make_float2(r, r);
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = mul2(rr, fma2(other[i], sw[i], mul2(x[i], cw[i])));
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = e0 + c * kFar + 2 * i;
+                        float2 o = make_float2(0.f, 0.f);
+                        if (pairs_in_lane) {
+                            if (e < a.rotary) o = make_float2(x[c][i].y, x[c][i].x);
+                        } else {
+                            if (e < a.rotary) o.x = mine[e < half ? e + half : e - half];
+                            if (e + 1 < a.rotary) o.y = mine[e + 1 < half ? e + 1 + half : e + 1 - half];
+                        }
+                        x[c][i] = mul2(rr, fma2(o, sw[c][i], mul2(x[c][i], cw[c][i])));
+                    }
             }
-            if (h < a.q_heads) store8(q_out + static_cast<int64_t>(h) * a.qo_h, x, a.vec);
-            else if (slot >= 0) store8((h < qk ? k_out : v_out) + static_cast<int64_t>(h < qk ? h - a.q_heads : h - qk) * a.head_s, x, a.vec);
         }
+        TO* dst;
+        if (h < a.q_heads) {
+            dst = static_cast<TO*>(a.q_out) + t * a.qo_t + static_cast<int64_t>(h) * a.qo_h + e0;
+        } else {
+            if (row < 0) continue;                   // padding: nothing is stored for it
+            if (entry < 0 || entry >= a.table.pages) {
+                if (a.status) atomicCAS(a.status, 0, static_cast<int>(kStatusBadPage));
+                continue;
+            }
+            dst = static_cast<TO*>(h < qk ? a.k_out : a.v_out) + entry * a.page_s + static_cast<int64_t>(pos % a.table.page) * a.slot_s +
+                  static_cast<int64_t>(h < qk ? h - a.q_heads : h - qk) * a.head_s + e0;
+        }
+        if (e0 < a.dim) store8(dst, x[0], vec);
+        if (e0 + kFar < a.dim) store8(dst + kFar, x[1], vec);
     }
 }
 
 template <typename TI, typename TO, int LPH> static int rope_layout(const RopeArgs& a, cudaStream_t st) {
-    const dim3 grid(a.tokens), block(kRopeThreads);
+    constexpr int kHeads = 32 / LPH;
+    const int64_t steps = static_cast<int64_t>(a.tokens) * ((a.q_heads + 2 * a.kv_heads + kHeads - 1) / kHeads), most = static_cast<int64_t>(kRopeResident) * sm_count();
+    const int64_t ctas = (steps + kRopeWarps - 1) / kRopeWarps;
+    const dim3 grid(static_cast<unsigned>(ctas < most ? ctas : most)), block(kRopeThreads);
+    if (!a.vec) return launch(rope_kernel<TI, TO, LPH, kPairsByLine>, grid, block, 0, st, a);
     if (a.interleaved) return launch(rope_kernel<TI, TO, LPH, kPairsInLane>, grid, block, 0, st, a);
-    if (a.rotary % 16 == 0) return launch(rope_kernel<TI, TO, LPH, kPairsByShuffle>, grid, block, 0, st, a);   // both values of a pair at the same place of their lanes
+    if (a.rotary % 16 == 0 && a.rotary <= LPH * 8) return launch(rope_kernel<TI, TO, LPH, kPairsByShuffle>, grid, block, 0, st, a);
+    if (a.rotary == LPH * 16) return launch(rope_kernel<TI, TO, LPH, kPairsAcross>, grid, block, 0, st, a);
     return launch(rope_kernel<TI, TO, LPH, kPairsByLine>, grid, block, 0, st, a);
 }
 
 template <typename TI, typename TO> static int rope_launch(const RopeArgs& a, cudaStream_t st) {
-    if (a.dim <= 64) return rope_layout<TI, TO, 8>(a, st);
-    if (a.dim <= 128) return rope_layout<TI, TO, 16>(a, st);
-    return rope_layout<TI, TO, 32>(a, st);
+    if (a.dim <= 64) return rope_layout<TI, TO, 4>(a, st);
+    if (a.dim <= 128) return rope_layout<TI, TO, 8>(a, st);
+    return rope_layout<TI, TO, 16>(a, st);
 }
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -291,7 +385,7 @@ extern "C" int nexrt_rope_append(const void* q, const void* k, const void* v, co
     a.q_h = static_cast<int>(strides[1]); a.k_h = static_cast<int>(strides[3]); a.v_h = static_cast<int>(strides[5]);
     a.qo_h = static_cast<int>(strides[7]); a.head_s = static_cast<int>(strides[9]);
     a.positions = static_cast<const int*>(positions); a.rows = static_cast<const int*>(rows);
-    a.table = {static_cast<const int*>(table), strides[11], table_rows, width, page, pages};
+    a.table = {static_cast<const int*>(table), strides[11], table_rows, width, page < 1 ? 1 : page, pages};
     a.inv_freq = static_cast<const float*>(inv_freq); a.q_norm = static_cast<const float*>(q_norm); a.k_norm = static_cast<const float*>(k_norm);
     a.status = static_cast<int*>(status);
     a.tokens = tokens; a.q_heads = q_heads; a.kv_heads = kv_heads; a.dim = dim; a.rotary = rotary; a.interleaved = interleaved;
