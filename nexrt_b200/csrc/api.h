@@ -212,7 +212,7 @@ int nexrt_rope_append(const void* q, const void* k, const void* v, const void* p
                       const void* table, const void* inv_freq, const void* q_norm, const void* k_norm, void* status, const int64_t* strides, int tokens, int q_heads,
                       int kv_heads, int dim, int rotary, int interleaved, int table_rows, int width, int page, int pages, int in_type, int out_type, float scale,
                       float eps, void* stream);   /* table NULL: q alone, kv_heads 0; strides: (token, head) of q, k, v, q_out, (page, head, slot) of the pools, row of the table */
-int nexrt_paged_ctas(int seqs, int q_heads, int kv_heads, int width, int page, int window);   /* CTAs of a call: its scratch is 2 * that * 16 * (dim + 2) floats */
+int nexrt_paged_ctas(int seqs, int q_heads, int kv_heads, int width, int page, int window);   /* CTAs of a call: its scratch is that many times 32 (dim + 2) + 4 floats */
 int nexrt_paged_attn(const void* q, const void* k_pages, const void* v_pages, const void* table, const void* lens, const void* slopes, void* out, void* lse,
                      void* scratch, void* status, const int64_t* strides, int seqs, int q_heads, int kv_heads, int dim, int width, int page, int pages, int window,
                      int type, float scale, float softcap, int ctas, void* stream);   /* strides: (sequence, head) of q and out, (page, head, slot) of the pools, rows of the table and of lse */

@@ -6,9 +6,10 @@
 // Bound by the bytes of K and V: with at most 16 query heads on a key head there are at most 32 multiply-adds a byte.  So the
 // design is for the stream.  The keys of the whole batch are cut into equal ranges, one per resident CTA (two on an SM), whatever
 // the sequences' lengths; a CTA walks its range item by item (sequence, key head, up to 16 query heads).  A warp has a ring of
-// 16-key half tiles (K, V, K, V ...) of its own in shared memory, filled by 16-byte cp.async row by row through the page table, so
-// it waits for nobody, and pages of any size, also ones that end inside a tile, cost the same.  Rows are padded by 16 bytes:
-// ldmatrix and the copies meet no bank twice.  Products are mma.sync m16n8k16 - a tensor-memory product wants 128 rows, and here
+// 16-key half tiles (K, V, K, V ...) of its own in shared memory, filled row by row through the page table, so it waits for nobody, and
+// pages of any size, also ones that end inside a tile, cost the same.  From 128 dims up a row is one bulk copy (cp.async.bulk, one
+// instruction for the 16 rows of a half tile: streaming 419 MB takes 64 us in rows of 512 bytes, 66 in rows of 256, but 100 in rows of
+// 128); rows of 64 dims go by 16-byte cp.async (70 us).  Rows are padded by 16 bytes: ldmatrix and the copies meet no bank twice.  Products are mma.sync m16n8k16 - a tensor-memory product wants 128 rows, and here
 // are 16 at most: scores with the query rows on the M side, values transposed (dims on M, rows on N), so that the score
 // fragments are the value product's operands without a shuffle.  P enters as a 16-bit pair hi + lo: one 16-bit P would add an
 // error as large as the result's own rounding.  Maximum, sum and accumulators are 32 bits.
@@ -24,17 +25,21 @@ constexpr int kPaWarps = 4;
 constexpr int kPaThreads = kPaWarps * 32;
 constexpr int kPaRows = 16;                 // query rows of an item
 constexpr int kTile = 16;                   // keys of a warp's tile
+constexpr uint32_t kNoRow = 0xffffffffu;
 static_assert(kChunk == kPaWarps * kTile, "a chunk is one tile a warp");
 
 struct PagedAttnArgs {
     const void *q, *k, *v;
     void* out;
     float* lse;                              // may be null
-    int64_t q_b, q_h, o_b, o_h, page_s, head_s, slot_s, lse_b;
+    int64_t q_b, q_h, o_b, o_h, head_s, lse_b;
+    uint32_t page_s, slot_s;                 // of a pool, in units of 16 bytes: a row's place is 32 bits wide
     PageTable table;
     const int* lens;
     const float* slopes;                     // may be null
     float *ws_o, *ws_ml;                     // parts: [2 grid][16][dim], [2 grid][16][2]
+    int4* cuts;                              // [min(grid, items)] of a cut item: sequence, first head, first CTA, parts; parts 0: none
+    int by_item;                             // cuts of items, not of CTAs
     int* status;
     int seqs, kv_heads, group, head_groups, window, grid;
     float scale, softcap;
@@ -44,7 +49,7 @@ template <int D> constexpr int ring_depth() { return D == 256 ? 3 : (D == 192 ? 
 template <int D> constexpr int half_bytes() { return kTile * (D * 2 + 16); }
 template <int D> constexpr size_t ring_bytes() { return static_cast<size_t>(kPaWarps) * ring_depth<D>() * half_bytes<D>(); }
 template <int D> constexpr size_t merge_bytes() { return sizeof(float) * kPaWarps * kPaRows * (D + 4); }
-template <int D> constexpr size_t paged_smem() { return (ring_bytes<D>() > merge_bytes<D>() ? ring_bytes<D>() : merge_bytes<D>()) + D / 16 * 512; }
+template <int D> constexpr size_t paged_smem() { return  (ring_bytes<D>() > merge_bytes<D>() ? ring_bytes<D>() : merge_bytes<D>()) + D / 16 * 512; }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -83,12 +88,13 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 }
 
 // ---- where a CTA's range lies ------------------------------------------------------------------------------------------
-// Chunks of one item of sequence b.
+// Chunks of one item of sequence b, and what all its items count.
 __device__ __forceinline__ int seq_chunks(const PagedAttnArgs& a, int b) {
     int lo, hi;
     key_span(a.lens[b], static_cast<int64_t>(a.table.width) * a.table.page, a.window, lo, hi);
     return chunks_of(lo, hi);
 }
+__device__ __forceinline__ int64_t seq_cost(const PagedAttnArgs& a, int items, int b) { return static_cast<int64_t>(cost_of(seq_chunks(a, b))) * items; }
 
 // Sum over the CTA's threads of `v`, and the sum over the threads before this one.  Every thread calls it.  red: 32 words.
 __device__ __forceinline__ int64_t scan_add(int64_t v, int64_t* red, int64_t& total) {
@@ -112,31 +118,57 @@ __device__ __forceinline__ int64_t scan_add(int64_t v, int64_t* red, int64_t& to
 }
 
 struct Place {
-    int seq;            // sequence, or seqs when there is none
-    int64_t first;      // chunks in front of the sequence
+    int seq;            // sequence
+    int64_t first;      // units in front of it
 };
 
-__device__ __forceinline__ int64_t total_chunks(const PagedAttnArgs& a, int items, int64_t* red) {
-    int64_t mine = 0, total;
-    for (int b = threadIdx.x; b < a.seqs; b += blockDim.x) mine += static_cast<int64_t>(seq_chunks(a, b)) * items;
-    scan_add(mine, red, total);
+// Units of the whole batch; with up to as many sequences as threads `cost` and `at` are those of this thread's sequence and of the ones in front.
+__device__ __forceinline__ int64_t total_cost(const PagedAttnArgs& a, int items, int64_t* red, int64_t& cost, int64_t& at) {
+    cost = at = 0;
+    if (a.seqs == 1) {
+        if (threadIdx.x == 0) cost = seq_cost(a, items, 0);
+        return seq_cost(a, items, 0);
+    }
+    int64_t total;
+    for (int b = threadIdx.x; b < a.seqs; b += blockDim.x) cost += seq_cost(a, items, b);
+    at = scan_add(cost, red, total);
     return total;
 }
 
-// The sequence that holds chunk x (x < total).  place: shared.
-__device__ __forceinline__ Place find_seq(const PagedAttnArgs& a, int items, int64_t x, int64_t* red, Place* place) {
-    int64_t before = 0;
-    for (int b0 = 0; b0 < a.seqs; b0 += blockDim.x) {
-        const int b = b0 + threadIdx.x;
-        const int64_t n = b < a.seqs ? static_cast<int64_t>(seq_chunks(a, b)) * items : 0;
-        int64_t total;
-        const int64_t at = before + scan_add(n, red, total);
-        if (x >= at && x < at + n) *place = {b, at};
-        before += total;
-        if (x < before) break;
+// The sequence that holds unit x (x < total).  place: shared.
+__device__ __forceinline__ Place find_seq(const PagedAttnArgs& a, int items, int64_t x, int64_t cost, int64_t at, int64_t* red, Place* place) {
+    if (a.seqs == 1) return {0, 0};
+    if (a.seqs <= static_cast<int>(blockDim.x)) {
+        if (x >= at && x < at + cost) *place = {static_cast<int>(threadIdx.x), at};
+    } else {
+        int64_t before = 0;
+        for (int b0 = 0; b0 < a.seqs; b0 += blockDim.x) {
+            const int b = b0 + threadIdx.x;
+            const int64_t n = b < a.seqs ? seq_cost(a, items, b) : 0;
+            int64_t total;
+            const int64_t first = before + scan_add(n, red, total);
+            if (x >= first && x < first + n) *place = {b, first};
+            before += total;
+            if (x < before) break;
+        }
     }
     __syncthreads();
     return *place;
+}
+
+// A ring place's copies have arrived.  Bounded: a wait that runs out latches kStatusPipeTimeout, and those behind it are short; the
+// result is not to be used then, but every copy has been waited for when the kernel ends.
+__device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t phase, bool& late, int* status) {
+    bool ok = false;
+    for (int i = late ? 1 << 10 : 1 << 20; i > 0 && !ok; --i) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(phase) : "memory");
+        ok = done != 0;
+    }
+    if (!ok) {
+        late = true;
+        if (status) atomicCAS(status, 0, static_cast<int>(kStatusPipeTimeout));
+    }
 }
 
 template <typename T, int D, int NTR, bool MODS>
@@ -148,109 +180,159 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const __grid_
     __shared__ int64_t red[32];
     __shared__ Place place;
     __shared__ float part_m[kPaWarps][kPaRows], part_l[kPaWarps][kPaRows];
+    __shared__ uint64_t bars[kPaWarps][R];
+    constexpr bool kBulk = D >= 192;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const uint32_t bar0 = static_cast<uint32_t>(__cvta_generic_to_shared(&bars[warp][0]));
+    if (kBulk) {
+        if (lane < R) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar0 + lane * 8) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        __syncwarp();
+    }
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int items = a.kv_heads * a.head_groups;
     const int64_t room = static_cast<int64_t>(a.table.width) * a.table.page;
 
-    // sequences without keys: zeros, and an lse of -infinity
-    for (int b = blockIdx.x; b < a.seqs; b += gridDim.x) {
-        if (a.lens[b] > room && threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, static_cast<int>(kStatusBadPage));
-        if (seq_chunks(a, b)) continue;
-        const int heads = a.kv_heads * a.group;
-        for (int i = threadIdx.x; i < heads * D; i += kPaThreads) static_cast<T*>(a.out)[b * a.o_b + i / D * a.o_h + i % D] = static_cast<T>(0.f);
-        if (a.lse)
-            for (int i = threadIdx.x; i < heads; i += kPaThreads) a.lse[b * a.lse_b + i] = -INFINITY;
+    int64_t my_cost, my_at;
+    const int64_t total = total_cost(a, items, red, my_cost, my_at);
+    const int n = active_ctas(total, gridDim.x);
+    int64_t x = 0, x_end = 0, first = 0;
+    int b = 0;
+    if (total > 0 && static_cast<int>(blockIdx.x) < n) {
+        x = range_begin(total, blockIdx.x, n);
+        x_end = range_begin(total, blockIdx.x + 1, n);
+        const Place start = find_seq(a, items, x, my_cost, my_at, red, &place);
+        b = start.seq;
+        first = start.first;
     }
 
-    const int64_t total = total_chunks(a, items, red);
-    const int n = active_ctas(total, gridDim.x);
-    if (total == 0 || static_cast<int>(blockIdx.x) >= n) return;
-    int64_t x = range_begin(total, blockIdx.x, n);
-    const int64_t x_end = range_begin(total, blockIdx.x + 1, n);
-    const Place start = find_seq(a, items, x, red, &place);
-    int b = start.seq;
-    int64_t first = start.first;
-    const int64_t range0 = x;
-
     const uint32_t my_ring = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + warp * R * HALF;
-    // ldmatrix rows of this lane.  K: keys on the rows; V: keys on the rows, read transposed
+    // ldmatrix row of this lane: keys on the rows, V's read transposed
     const uint32_t k_lane = ((lane & 7) + ((lane >> 4) << 3)) * PITCH + ((lane >> 3) & 1) * 16;
-    const uint32_t v_lane = ((lane & 7) + ((lane >> 4) << 3)) * PITCH + ((lane >> 3) & 1) * 16;
+    int to = 0, use = 0;                                               // places of the ring: of the next half that is fed, and used
+    uint32_t phases = 0;                                               // bit: phase of a place's barrier
+    bool late = false;
+    int4 cut = make_int4(0, 0, 0, 0);                                  // the item that this CTA begins and another one ends
 
     while (x < x_end) {
         int lo, hi;
         key_span(a.lens[b], room, a.window, lo, hi);
-        const int per = chunks_of(lo, hi);
-        if (x >= first + static_cast<int64_t>(per) * items) {        // also sequences without keys
-            first += static_cast<int64_t>(per) * items;
+        const int per = chunks_of(lo, hi), cost = cost_of(per);
+        if (x >= first + static_cast<int64_t>(cost) * items) {       // also sequences without keys
+            first += static_cast<int64_t>(cost) * items;
             ++b;
             continue;
         }
-        const int item = static_cast<int>((x - first) / per);
-        const int64_t item0 = first + static_cast<int64_t>(item) * per;
-        const int c0 = static_cast<int>(x - item0);
-        const int c1 = item0 + per < x_end ? per : static_cast<int>(x_end - item0);
+        const int item = static_cast<int>(quotient(x - first, cost));
+        const int64_t item0 = first + static_cast<int64_t>(item) * cost;
+        int c0, c1;
+        item_part(item0, per, x, x_end, c0, c1);
+        x = item0 + cost;
+        if (c1 <= c0) continue;                                       // the range ends in front of the item's first chunk
         const int kvh = item / a.head_groups, h0 = kvh * a.group + item % a.head_groups * kPaRows;
         const int rows = min(kPaRows, (kvh + 1) * a.group - h0);
         const int key0 = (lo / kChunk + c0) * kChunk + warp * kTile;  // first key of this warp's tile of chunk c0
         const int tiles = c1 - c0;
-        const T* const kbase = static_cast<const T*>(a.k) + kvh * a.head_s;
-        const T* const vbase = static_cast<const T*>(a.v) + kvh * a.head_s;
+        const char* const kbase = static_cast<const char*>(a.k) + kvh * a.head_s * 2;
+        const char* const vbase = static_cast<const char*>(a.v) + kvh * a.head_s * 2;
 
-        // ---- page lookups one tile ahead of the copies: lane l (mod 16) finds the row of key l of the tile, -1 outside
-        auto find = [&](int tile) -> int64_t {
+        // ---- page lookups one tile ahead of the copies: lane l (mod 16) finds the row of key l of the tile, in units of 16 bytes
+        auto find = [&](int tile) -> uint32_t {
             const int p = key0 + tile * kChunk + (lane & 15);
-            if (tile >= tiles || p < lo || p >= hi) return -1;
+            if (tile >= tiles || p < lo || p >= hi) return kNoRow;
             const int j = p / a.table.page, page = page_at(a.table, b, j);
             if (page < 0) {
                 if (a.status) atomicCAS(a.status, 0, static_cast<int>(kStatusBadPage));
-                return -1;
+                return kNoRow;
             }
-            return static_cast<int64_t>(page) * a.page_s + static_cast<int64_t>(p - j * a.table.page) * a.slot_s;
+            return static_cast<uint32_t>(page) * a.page_s + static_cast<uint32_t>(p - j * a.table.page) * a.slot_s;
         };
-        auto issue = [&](int half, int64_t at) {
+        // the first tiles' lookups side by side.  at: rows of the tile that is being copied, next: of the one behind it; newest: which
+        // of its keys are there
+        constexpr int Q = R / 2;
+        uint32_t at = kNoRow, newest = 0, ahead[Q + 1];
+#pragma unroll
+        for (int i = 0; i <= Q; ++i) ahead[i] = find(i);
+        auto copy = [&](int half) {
             if (half < 2 * tiles) {
-                const T* base = (half & 1) ? vbase : kbase;
-                const uint32_t dst = my_ring + half % R * HALF;
+                const char* const base = (half & 1) ? vbase : kbase;
+                const uint32_t ring_to = my_ring + to * HALF;
+                if (kBulk) {
+                    const uint32_t bar = bar0 + to * 8;
+                    if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(__popc(newest) * D * 2) : "memory");
+                    if ((half & 1) && newest != 0xffffu) {             // values of absent keys meet a P of zero: they have to be numbers
+                        for (int i = lane; i < kTile * CPR; i += 32)
+                            if (!(newest >> (i / CPR) & 1)) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring_to + i / CPR * PITCH + i % CPR * 16), "r"(0) : "memory");
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    __syncwarp();
+                    if (lane < kTile && at != kNoRow)
+                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                                     ::"r"(ring_to + lane * PITCH), "l"(base + static_cast<uint64_t>(at) * 16), "r"(D * 2), "r"(bar) : "memory");
+                } else {
 #pragma unroll
-                for (int i = 0; i < kTile * CPR / 32; ++i) {
-                    const int idx = i * 32 + lane, r = idx / CPR, c = idx - r * CPR;
-                    const int64_t off = __shfl_sync(0xffffffffu, at, r);
-                    cp16(dst + r * PITCH + c * 16, base + (off < 0 ? 0 : off + c * 8), off >= 0);
+                    for (int i = 0; i < kTile * CPR / 32; ++i) {
+                        const int r = i * (32 / CPR) + lane / CPR, c = lane % CPR;
+                        const uint32_t row = __shfl_sync(0xffffffffu, at, r);
+                        cp16(ring_to + r * PITCH + c * 16, base + c * 16 + (row == kNoRow ? 0ull : static_cast<uint64_t>(row) * 16), row != kNoRow);
+                    }
                 }
+                to = to + 1 == R ? 0 : to + 1;
             }
-            cp_commit();
+            if (!kBulk) cp_commit();
         };
-        // halves 0 .. R-2 are in flight before the first is used; `at`: rows of the tile that is being copied
-        int64_t at = find(0), next = find(1);
-        auto feed = [&](int half) {
-            if (half > 0 && !(half & 1)) {
-                at = next;
-                next = find(half / 2 + 1);
-            }
-            issue(half, at);
-        };
+        // halves 0 .. R-2 are on their way before the first is used.  masks: which keys are there, 16 bits a tile, of the tile in use and
+        // of the R / 2 - 1 behind it
+        uint64_t masks = 0;
 #pragma unroll
-        for (int i = 0; i < R - 1; ++i) feed(i);
+        for (int i = 0; i < R - 1; ++i) {
+            if (i % 2 == 0) {
+                at = ahead[i / 2];
+                newest = __ballot_sync(0xffffffffu, at != kNoRow) & 0xffffu;
+                masks |= static_cast<uint64_t>(newest) << (i * 8);
+            }
+            copy(i);
+        }
+        uint32_t next = ahead[Q];
+        int fed = R - 1;
+        auto feed = [&]() {
+            if (!(fed & 1)) {
+                at = next;
+                next = find(fed / 2 + 1);
+                newest = __ballot_sync(0xffffffffu, at != kNoRow) & 0xffffu;
+            }
+            copy(fed++);
+        };
+        auto arrived = [&]() {
+            if (kBulk) bar_wait(bar0 + use * 8, phases >> use & 1, late, a.status);
+            else cp_wait<R - 2>();
+            __syncwarp();
+        };
+        auto used = [&]() {
+            phases ^= 1u << use;
+            use = use + 1 == R ? 0 : use + 1;
+        };
 
         // ---- query fragments
         {
             const T* q = static_cast<const T*>(a.q) + b * a.q_b;
-            for (int i = threadIdx.x; i < KS * 32; i += kPaThreads) {
-                const int ks = i >> 5, l = i & 31, gr = l >> 2, d = ks * 16 + (l & 3) * 2;
+            const bool pairs = ((reinterpret_cast<uintptr_t>(q) >> 1 | a.q_h) & 1) == 0;
+#pragma unroll
+            for (int i0 = 0; i0 < KS * 32; i0 += kPaThreads) {
+                const int i = i0 + threadIdx.x, ks = i >> 5, l = i & 31, gr = l >> 2, d = ks * 16 + (l & 3) * 2;
                 uint32_t f[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const int r = gr + (u & 1) * 8, dd = d + (u >> 1) * 8;
                     f[u] = 0;
-                    if (r < rows) {
-                        const unsigned short* s = reinterpret_cast<const unsigned short*>(q + (h0 + r) * a.q_h + dd);
-                        f[u] = s[0] | static_cast<uint32_t>(s[1]) << 16;
+                    if (r < rows && ks < KS) {
+                        const T* s = q + (h0 + r) * a.q_h + dd;
+                        if (pairs) f[u] = *reinterpret_cast<const uint32_t*>(s);
+                        else f[u] = reinterpret_cast<const unsigned short*>(s)[0] | static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(s)[1]) << 16;
                     }
                 }
-                qf[i] = make_uint4(f[0], f[1], f[2], f[3]);
+                if (ks < KS) qf[i] = make_uint4(f[0], f[1], f[2], f[3]);
             }
         }
         __syncthreads();
@@ -268,27 +350,37 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const __grid_
             slope[r] = MODS && a.slopes && g + 8 * r < rows ? a.slopes[h0 + g + 8 * r] * 1.4426950408889634f : 0.f;
         }
         const float scale2 = a.scale * 1.4426950408889634f;
+        // with few registers' worth of queries they stay there
+        constexpr bool kHold = KS * NTR <= 16;
+        uint32_t qr[kHold ? KS : 1][4];
+        if (kHold) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint4 q4 = qf[ks * 32 + lane];
+                qr[ks][0] = q4.x; qr[ks][1] = NTR == 1 ? 0u : q4.y; qr[ks][2] = q4.z; qr[ks][3] = NTR == 1 ? 0u : q4.w;
+            }
+        }
 
-        int64_t here = find(0);                                        // rows of the tile in use: which of its keys are there
         for (int i = 0; i < tiles; ++i) {
-            const unsigned int have = __ballot_sync(0xffffffffu, here >= 0);
-            here = find(i + 1);
+            const uint32_t have = static_cast<uint32_t>(masks) & 0xffffu;
             // ---- scores
-            cp_wait<R - 2>();
-            __syncwarp();
-            feed(2 * i + R - 1);
+            arrived();
+            feed();
             float s[2][4];
 #pragma unroll
             for (int u = 0; u < 2; ++u) s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
-            const uint32_t kt = my_ring + (2 * i) % R * HALF + k_lane;
+            const uint32_t kt = my_ring + use * HALF + k_lane;
+            used();
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 uint32_t kf[4];
                 ldsm4(kf, kt + ks * 32);
-                const uint4 q4 = qf[ks * 32 + lane];
-                const uint32_t qa[4] = {q4.x, q4.y, q4.z, q4.w};
-                mma16816(s[0], qa, kf[0], kf[1], T());
-                mma16816(s[1], qa, kf[2], kf[3], T());
+                if (!kHold) {
+                    const uint4 q4 = qf[ks * 32 + lane];
+                    qr[0][0] = q4.x; qr[0][1] = q4.y; qr[0][2] = q4.z; qr[0][3] = q4.w;
+                }
+                mma16816(s[0], qr[kHold ? ks : 0], kf[0], kf[1], T());
+                mma16816(s[1], qr[kHold ? ks : 0], kf[2], kf[3], T());
             }
             // ---- mask and running softmax: row g + 8 r has its 16 scores in the four lanes of a g
             uint32_t ph[NTR][2], pl[NTR][2];
@@ -337,10 +429,10 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const __grid_
                 }
             }
             // ---- values
-            cp_wait<R - 2>();
-            __syncwarp();
-            feed(2 * i + R);
-            const uint32_t vt = my_ring + (2 * i + 1) % R * HALF + v_lane;
+            arrived();
+            feed();
+            const uint32_t vt = my_ring + use * HALF + k_lane;
+            used();
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
                 uint32_t vf[4];
@@ -351,8 +443,9 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const __grid_
                     mma16816(o[j][r], vf, pl[r][0], pl[r][1], T());
                 }
             }
+            masks = masks >> 16 | static_cast<uint64_t>(newest) << (16 * (R / 2 - 1));
         }
-        cp_wait<0>();
+        if (!kBulk) cp_wait<0>();
 
         // ---- join the warps: rings are free from here on
 #pragma unroll
@@ -388,8 +481,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const __grid_
         }
         __syncthreads();
         const bool whole = c0 == 0 && c1 == per;
-        // a part that began in front of this range is the CTA's first, else its last
-        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (item0 < range0 ? 0 : 1);
+        // a part whose item began in front of this range is the CTA's first, else its last
+        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (c0 == 0);
         for (int i = threadIdx.x; i < rows * (D / 4); i += kPaThreads) {
             const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -415,78 +508,105 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const __grid_
                 }
             }
         }
+        if (c0 == 0) {
+            const int parts = whole ? 0 : owner_of(item0 + cost - 1, total, n) - static_cast<int>(blockIdx.x) + 1;
+            cut = make_int4(b, h0, blockIdx.x, parts);
+            if (a.by_item && threadIdx.x == 0) a.cuts[b * items + item] = cut;
+        }
+        // the next item's copies go where these values lay
+        if (kBulk) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
-        x = item0 + c1;
+    }
+
+    if (!a.by_item && threadIdx.x == 0) a.cuts[blockIdx.x] = cut;
+
+    // ---- sequences without keys: zeros, and an lse of -infinity
+    for (int s = blockIdx.x; s < a.seqs; s += gridDim.x) {
+        if (a.lens[s] > room && threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, static_cast<int>(kStatusBadPage));
+        if (seq_chunks(a, s)) continue;
+        const int heads = a.kv_heads * a.group;
+        for (int i = threadIdx.x; i < heads * D; i += kPaThreads) static_cast<T*>(a.out)[s * a.o_b + i / D * a.o_h + i % D] = static_cast<T>(0.f);
+        if (a.lse)
+            for (int i = threadIdx.x; i < heads; i += kPaThreads) a.lse[s * a.lse_b + i] = -INFINITY;
+        if (a.by_item)
+            for (int i = threadIdx.x; i < items; i += kPaThreads) a.cuts[s * items + i] = make_int4(0, 0, 0, 0);
     }
 }
 
-// One CTA per (sequence, query head): joins the parts of an item that was cut.  Threads: D / 4 lanes of four dims, in 1024 / D * 4 groups of parts.
+// One CTA per (cut, row): joins the parts of an item that was cut.  The parts' maxima and sums first, then their accumulators with
+// D / 4 lanes of four dims side by side and the parts shared out over the groups of lanes.
+constexpr int kJoinThreads = 512;
+constexpr int kMaxCtas = 1024;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttnArgs a) {
-    constexpr int LANES = D / 4, GROUPS = 256 / LANES;
-    __shared__ int64_t red[32];
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int LANES = D / 4, GROUPS = kJoinThreads / LANES;
+    __shared__ float weight[kMaxCtas], top_s[kJoinThreads / 32], sum_s[kJoinThreads / 32];
     __shared__ float4 acc_s[GROUPS][LANES];
-    __shared__ float ml_s[GROUPS][2];
     pdl_launch_dependents();
     pdl_wait();
-    const int heads = a.kv_heads * a.group, b = blockIdx.x / heads, h = blockIdx.x - b * heads;
-    const int items = a.kv_heads * a.head_groups;
-    const int per = seq_chunks(a, b);
-    if (per == 0) return;
-    // chunks in front of sequence b, and of all
-    int64_t mine = 0, before = 0, total;
-    for (int i = threadIdx.x; i < a.seqs; i += blockDim.x) {
-        const int64_t c = static_cast<int64_t>(seq_chunks(a, i)) * items;
-        mine += c;
-        if (i < b) before += c;
+    const int4 cut = a.cuts[blockIdx.x];
+    const int b = cut.x, row = blockIdx.y, h = cut.y + row, cta0 = cut.z, parts = cut.w;
+    if (parts == 0 || h >= (cut.y / a.group + 1) * a.group) return;
+    // part p: row of the scratch.  Where an item begins it is its CTA's second part, elsewhere the first
+    auto slot_of = [&](int p) { return (2 * static_cast<int64_t>(cta0 + p) + (p == 0)) * kPaRows + row; };
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+    // the first parts' accumulators are on their way while the weights are made
+    constexpr int kEarly = 4;
+    float4 early[kEarly];
+#pragma unroll
+    for (int i = 0; i < kEarly; ++i) {
+        early[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (grp < GROUPS && grp + i * GROUPS < parts) early[i] = *reinterpret_cast<const float4*>(a.ws_o + slot_of(grp + i * GROUPS) * D + d * 4);
     }
-    scan_add(mine, red, total);
-    int64_t first;
-    scan_add(before, red, first);
-    const int n = active_ctas(total, a.grid);
-    const int kvh = h / a.group, in_group = h - kvh * a.group, item = kvh * a.head_groups + in_group / kPaRows, row = in_group % kPaRows;
-    const int64_t item0 = first + static_cast<int64_t>(item) * per;
-    const int cta0 = owner_of(item0, total, n), cta1 = owner_of(item0 + per - 1, total, n);
-    if (cta0 == cta1) return;                                           // one CTA wrote it
-    const int d = threadIdx.x % LANES, grp = threadIdx.x / LANES;
     float m = -INFINITY, l = 0.f;
+    for (int p = threadIdx.x; p < parts; p += kJoinThreads) {
+        weight[p] = a.ws_ml[slot_of(p) * 2];
+        m = max_nan(m, weight[p]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) top_s[warp] = m;
+    __syncthreads();
+    m = top_s[0];
+#pragma unroll
+    for (int i = 1; i < kJoinThreads / 32; ++i) m = max_nan(m, top_s[i]);
+    const float shift = m == -INFINITY ? 0.f : m;
+    for (int p = threadIdx.x; p < parts; p += kJoinThreads) {
+        const float w = exp2f(weight[p] - shift);
+        weight[p] = w;
+        l = fmaf(a.ws_ml[slot_of(p) * 2 + 1], w, l);
+    }
+    l = warp_sum(l);
+    if (lane == 0) sum_s[warp] = l;
+    __syncthreads();
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     if (grp < GROUPS) {
-        for (int c = cta0 + grp; c <= cta1; c += GROUPS) {
-            const int64_t slot = (2 * static_cast<int64_t>(c) + (c == cta0)) * kPaRows + row;
-            const float pm = a.ws_ml[slot * 2], pl = a.ws_ml[slot * 2 + 1];
-            const float4 p = *reinterpret_cast<const float4*>(a.ws_o + slot * D + d * 4);
-            const float mn = max_nan(m, pm);
-            if (mn == -INFINITY) continue;
-            const float f0 = exp2f(m - mn), f1 = exp2f(pm - mn);
-            l = l * f0 + pl * f1;
-            y.x = y.x * f0 + p.x * f1; y.y = y.y * f0 + p.y * f1; y.z = y.z * f0 + p.z * f1; y.w = y.w * f0 + p.w * f1;
-            m = mn;
-        }
+        auto add = [&](const float4& v, int p) {
+            const float w = weight[p];
+            y.x = fmaf(v.x, w, y.x); y.y = fmaf(v.y, w, y.y); y.z = fmaf(v.z, w, y.z); y.w = fmaf(v.w, w, y.w);
+        };
+#pragma unroll
+        for (int i = 0; i < kEarly; ++i)
+            if (grp + i * GROUPS < parts) add(early[i], grp + i * GROUPS);
+#pragma unroll 4
+        for (int p = grp + kEarly * GROUPS; p < parts; p += GROUPS) add(*reinterpret_cast<const float4*>(a.ws_o + slot_of(p) * D + d * 4), p);
         acc_s[grp][d] = y;
-        if (d == 0) {
-            ml_s[grp][0] = m;
-            ml_s[grp][1] = l;
-        }
     }
     __syncthreads();
     if (grp != 0) return;
-    float top = -INFINITY;
-    for (int i = 0; i < GROUPS; ++i) top = max_nan(top, ml_s[i][0]);
     l = 0.f;
-    y = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (top != -INFINITY) {
-        for (int i = 0; i < GROUPS; ++i) {
-            const float f = exp2f(ml_s[i][0] - top);
-            const float4 p = acc_s[i][d];
-            l += ml_s[i][1] * f;
-            y.x += p.x * f; y.y += p.y * f; y.z += p.z * f; y.w += p.w * f;
-        }
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 32; ++i) l += sum_s[i];
+#pragma unroll
+    for (int i = 1; i < GROUPS; ++i) {
+        const float4 v = acc_s[i][d];
+        y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* out = static_cast<T*>(a.out) + b * a.o_b + h * a.o_h + d * 4;
     out[0] = static_cast<T>(y.x * inv); out[1] = static_cast<T>(y.y * inv); out[2] = static_cast<T>(y.z * inv); out[3] = static_cast<T>(y.w * inv);
-    if (a.lse && d == 0) a.lse[b * a.lse_b + h] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+    if (a.lse && d == 0) a.lse[b * a.lse_b + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 template <typename T, int D> static int paged_launch(const PagedAttnArgs& a, bool join, cudaStream_t st) {
@@ -497,7 +617,8 @@ template <typename T, int D> static int paged_launch(const PagedAttnArgs& a, boo
     if (a.group <= 8) e = mods ? launch(paged_attn_kernel<T, D, 1, true>, grid, block, smem, st, a) : launch(paged_attn_kernel<T, D, 1, false>, grid, block, smem, st, a);
     else e = mods ? launch(paged_attn_kernel<T, D, 2, true>, grid, block, smem, st, a) : launch(paged_attn_kernel<T, D, 2, false>, grid, block, smem, st, a);
     if (e || !join) return e;
-    return launch(paged_join_kernel<T, D>, dim3(a.seqs * a.kv_heads * a.group), dim3(256), 0, st, a);
+    const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads * a.head_groups;
+    return launch(paged_join_kernel<T, D>, dim3(a.by_item ? static_cast<unsigned>(items) : a.grid, a.group < kPaRows ? a.group : kPaRows), dim3(kJoinThreads), 0, st, a);
 }
 
 template <typename T> static int paged_dispatch(const PagedAttnArgs& a, int dim, bool join, cudaStream_t st) {
@@ -514,33 +635,38 @@ template <typename T> static int paged_dispatch(const PagedAttnArgs& a, int dim,
 
 using namespace nexrt;
 
-// CTAs of a call (its parts take 2 * that many * 16 * (dim + 2) floats of scratch).
+// CTAs of a call: its scratch is that many times 32 (dim + 2) + 4 floats.
 extern "C" int nexrt_paged_ctas(int seqs, int q_heads, int kv_heads, int width, int page, int window) {
     if (seqs < 1 || kv_heads < 1 || q_heads < kv_heads) return 1;
     const int64_t room = static_cast<int64_t>(width) * page;
     const int64_t keys = window > 0 && window < room ? window + kChunk : room;
-    const int64_t most = (keys / kChunk + 1) * seqs * kv_heads * ((q_heads / kv_heads + kPaRows - 1) / kPaRows);
+    const int64_t most = (keys / kChunk + 1 + kItemCost) * seqs * kv_heads * ((q_heads / kv_heads + kPaRows - 1) / kPaRows);
     const int64_t resident = 2ll * sm_count();
-    return static_cast<int>(most < resident ? most : resident);
+    return static_cast<int>(most < resident ? most : (resident < kMaxCtas ? resident : kMaxCtas));
 }
 
 // type: 0 bf16, 1 fp16.  strides: q (sequence, head), out, pools (page, head, slot), table row, lse row - in elements.
 extern "C" int nexrt_paged_attn(const void* q, const void* k_pages, const void* v_pages, const void* table, const void* lens, const void* slopes, void* out, void* lse,
                                 void* scratch, void* status, const int64_t* strides, int seqs, int q_heads, int kv_heads, int dim, int width, int page, int pages,
                                 int window, int type, float scale, float softcap, int ctas, void* stream) {
-    if (seqs < 0 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads || width < 0 || page < 1 || pages < 0 || window < 0 || ctas < 1 || !(softcap >= 0.f))
+    if (seqs < 0 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads || width < 0 || page < 1 || pages < 0 || window < 0 || ctas < 1 || ctas > kMaxCtas || !(softcap >= 0.f))
         return cudaErrorInvalidValue;
     if (seqs == 0) return 0;
     PagedAttnArgs a = {};
     a.q = q; a.k = k_pages; a.v = v_pages; a.out = out; a.lse = static_cast<float*>(lse);
     a.q_b = strides[0]; a.q_h = strides[1]; a.o_b = strides[2]; a.o_h = strides[3];
-    a.page_s = strides[4]; a.head_s = strides[5]; a.slot_s = strides[6]; a.lse_b = strides[8];
-    if (((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) || a.page_s % 8 || a.head_s % 8 || a.slot_s % 8) return cudaErrorInvalidValue;
+    a.head_s = strides[5]; a.lse_b = strides[8];
+    if (((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) || strides[4] % 8 || strides[5] % 8 || strides[6] % 8) return cudaErrorInvalidValue;
+    // a row is named by its place in units of 16 bytes: pools of up to 64 GB
+    if (strides[4] < 0 || strides[6] < 0 || (pages > 0 ? pages - 1 : 0) * (strides[4] / 8) + (page - 1) * (strides[6] / 8) >= kNoRow) return cudaErrorInvalidValue;
+    a.page_s = static_cast<uint32_t>(strides[4] / 8); a.slot_s = static_cast<uint32_t>(strides[6] / 8);
     a.table = {static_cast<const int*>(table), strides[7], seqs, width, page, pages};
     a.lens = static_cast<const int*>(lens); a.slopes = static_cast<const float*>(slopes);
-    a.ws_o = static_cast<float*>(scratch); a.ws_ml = a.ws_o + static_cast<int64_t>(2) * ctas * kPaRows * dim;
+    a.cuts = static_cast<int4*>(scratch);
+    a.ws_o = reinterpret_cast<float*>(a.cuts + ctas); a.ws_ml = a.ws_o + static_cast<int64_t>(2) * ctas * kPaRows * dim;
     a.status = static_cast<int*>(status);
     a.seqs = seqs; a.kv_heads = kv_heads; a.group = q_heads / kv_heads; a.head_groups = (a.group + kPaRows - 1) / kPaRows;
+    a.by_item = static_cast<int64_t>(seqs) * kv_heads * a.head_groups <= ctas;
     a.window = window; a.grid = ctas; a.scale = scale; a.softcap = softcap;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // with room for one chunk an item is never cut
@@ -558,9 +684,9 @@ extern "C" int nexrt_paged_split(const int* lens, int seqs, int items, int64_t r
     auto chunks = [&](int b) {
         int lo, hi;
         key_span(lens[b], room, window, lo, hi);
-        return static_cast<int64_t>(chunks_of(lo, hi));
+        return chunks_of(lo, hi);
     };
-    for (int b = 0; b < seqs; ++b) total += chunks(b) * items;
+    for (int b = 0; b < seqs; ++b) total += static_cast<int64_t>(cost_of(chunks(b))) * items;
     const int n = active_ctas(total, grid);
     int parts = 0;
     for (int c = 0; total > 0 && c < n; ++c) {
@@ -568,19 +694,24 @@ extern "C" int nexrt_paged_split(const int* lens, int seqs, int items, int64_t r
         const int64_t end = range_begin(total, c + 1, n);
         int b = 0;
         while (x < end) {
-            const int64_t per = chunks(b);
-            if (x >= first + per * items) {
-                first += per * items;
+            const int per = chunks(b), cost = cost_of(per);
+            if (x >= first + static_cast<int64_t>(cost) * items) {
+                first += static_cast<int64_t>(cost) * items;
                 ++b;
                 continue;
             }
-            const int64_t item = (x - first) / per, item0 = first + item * per, stop = item0 + per < end ? item0 + per : end;
+            const int64_t item = (x - first) / cost, item0 = first + item * cost;
+            int c0, c1;
+            item_part(item0, per, x, end, c0, c1);
+            x = item0 + cost;
+            if (c1 <= c0) continue;
+            // what the joining kernel expects: the first part with the owner of the first chunk, the last with that of the last
+            const bool ends = (c0 != 0 || owner_of(item0 + kItemCost, total, n) == c) && (c1 != per || owner_of(item0 + cost - 1, total, n) == c);
             if (parts < most) {
                 int64_t* o = out + static_cast<int64_t>(parts) * 5;
-                o[0] = c; o[1] = b; o[2] = item; o[3] = x - item0; o[4] = stop - x;
+                o[0] = c; o[1] = b; o[2] = item; o[3] = c0; o[4] = ends ? c1 - c0 : -1;
             }
             ++parts;
-            x = stop;
         }
     }
     return parts;

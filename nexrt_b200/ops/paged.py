@@ -72,7 +72,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         width, o_s = table.shape[1], out.stride()
         window = min(window, 2**31 - 1)
         ctas = L.nexrt_paged_ctas(rows, heads, kv_heads, width, slots, window)
-        scratch = q.new_empty(2 * ctas * 16 * (dim + 2), dtype=torch.float32)
+        scratch = q.new_empty(ctas * (32 * (dim + 2) + 4), dtype=torch.float32)
         strides = longs(q_s[0], q_s[1], o_s[0], o_s[1], pool_s[0], pool_s[1], pool_s[2], table.stride()[0], heads)
         on_device(device, lambda st: L.nexrt_paged_attn(
             q.data_ptr(), k_ptr, v_ptr, table.data_ptr(), lens.data_ptr(), ptr(slopes), out.data_ptr(), ptr(lse), scratch.data_ptr(), ptr(status), strides, rows, heads,

@@ -174,8 +174,9 @@ def test_slot_of_a_position():
 
 @pytest.mark.parametrize("seed", range(60))
 def test_split_covers_every_key_once(seed):
-    """The walk of every CTA, run on the host: each chunk of each item exactly once, equal ranges, and at most two cut items a CTA (its first
-    and its last), which is what the parts' scratch has room for."""
+    """The walk of every CTA, run on the host: each chunk of each item exactly once and with the owners that the joining kernel reckons with
+    (else the count comes back as -1), equal work (an item counts three chunks more than it has), and at most two cut items a CTA
+    (the one it goes on with and the one it begins), which is what the parts' scratch has room for."""
     r = random.Random(seed)
     lib = L.load()
     lens = [r.choice([0, 0, 1, 63, 64, 65, -3, int(math.exp(r.uniform(0, 11)))]) for _ in range(r.randint(1, 40))]
@@ -195,12 +196,14 @@ def test_split_covers_every_key_once(seed):
     for cta, b, i, first, count in out[:n].tolist():
         assert count > 0 and got.get((b, i), 0) == first          # in the order of the keys, without a gap
         got[b, i] = first + count
-        load[cta] = load.get(cta, 0) + count
+        load[cta] = load.get(cta, 0) + count + (3 if first == 0 else 0)
         if count < want[b, i]:
-            cut[cta] = cut.get(cta, 0) + 1
+            cut.setdefault(cta, []).append(first > 0)
     assert got == want
     if load:
-        assert max(load.values()) - min(load.values()) <= 1 and max(cut.values(), default=0) <= 2 and len(load) <= grid
+        total = sum(w + 3 for w in want.values())
+        share = total / min(grid, total)
+        assert max(load.values()) <= share + 4 and all(len(set(c)) == len(c) for c in cut.values()) and len(load) <= grid
 
 
 def test_frequencies():
