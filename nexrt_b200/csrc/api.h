@@ -228,7 +228,7 @@ int nexrt_page_copy(void* pool, int planes, int pages, int heads, int slots, int
                     void* stream);   /* scratch: int[3 n] */
 
 // ---- beam search (beam.cu) ------------------------------------------------------------------------------------------------
-int nexrt_beam_slices(int vocab);   /* a call's scratch is batch * beams * slices * (k + 2) words of 8 bytes */
+int nexrt_beam_slices(int rows, int vocab, int type);   /* a call's scratch is batch * beams * slices * (k + 2) words of 8 bytes */
 int nexrt_beam_select(const void* logits, const void* scores, const void* finished, const int64_t* strides, void* scores_out, void* rows_out, void* tokens_out,
                       void* scratch, void* status, int batch, int beams, int vocab, int k, int eos, int type, void* stream);   /* k <= 64, beams <= 256 */
 int nexrt_reorder_rows(const void* const* in, void* const* out, const int64_t* meta, int tensors, const void* rows, int64_t r_0, int64_t r_1, int cols, int n,

@@ -6,9 +6,12 @@
 // larger logit, then to the lower token.  A finished beam has one candidate, its end token at its own score.
 //
 // Within a beam the order of the totals is that of the logits, so one pass over a slice of a row gives everything that is
-// needed of it: its maximum, its sum of exp and its k largest logits (values stay in registers, 16 a thread).  The k largest:
-// the k-th largest of 64 group maxima bounds them from below, the few values at or above it are ranked by counting.  A second
-// kernel, one CTA a request, joins the slices.  Bound by the logits' bytes; for one request by the two launches.
+// needed of it: its maximum, its sum of exp and its k largest logits.  A CTA walks its slice in steps of 16 KB, 64 bytes a thread in
+// registers as they came, the next step's loads in flight.  The k largest: the k-th largest of 64 or 128 maxima of the first step bounds them from below, the few values
+// at or above it are collected and at the end ranked by counting (equal values in masses are found by bisection instead).  A second
+// kernel, one CTA a request, joins the slices.  Bound by the logits' bytes, and for one request by the two launches.
+#include <type_traits>
+
 #include "api.h"
 #include "common.cuh"
 
@@ -17,10 +20,10 @@ namespace nexrt {
 using u64 = unsigned long long;
 
 constexpr int kBeamMaxK = 64;
-constexpr int kSliceThreads = 512;
-constexpr int kPerThread = 16;
-constexpr int kSliceValues = kSliceThreads * kPerThread;
-constexpr int kBeamGroups = 64;             // of 8 lanes
+constexpr int kSliceThreads = 256;
+constexpr int kPieces = 4;                  // 16-byte pieces of a thread and step
+constexpr int kStepBytes = kSliceThreads * kPieces * 16;
+constexpr int kBeamGroups = 128;            // at most
 constexpr int kBeamKeep = 1024;             // values that are ranked by counting; more (ties) take the search below
 constexpr int kJoinThreads = 1024;
 constexpr int kBeamMaxWidth = 256;          // beams of a request
@@ -67,13 +70,62 @@ __device__ __forceinline__ int cta_sum(int v, int* red) {
     return __reduce_add_sync(0xffffffffu, lane < n ? red[lane] : 0);
 }
 
+// 16 bytes of a row as they came; `top` takes maxNum over two or four such pieces' words without unpacking 16-bit types.
+template <typename T> struct Piece {
+    static constexpr int kValues = 16 / sizeof(T);
+    uint32_t w[4];
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        else return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w[i / 2] >> 16 : w[i / 2])));
+    }
+    __device__ __forceinline__ void operator=(const uint4& v) { w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+    __device__ __forceinline__ float top() const {
+        if constexpr (sizeof(T) == 4) {
+            return fmaxf(fmaxf(value(0), value(1)), fmaxf(value(2), value(3)));
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
+            const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+            return fmaxf(f.x, f.y);
+        } else {
+            const __half2* h = reinterpret_cast<const __half2*>(w);
+            const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+            return fmaxf(f.x, f.y);
+        }
+    }
+};
+
+// The piece at value `at` of a row where it reaches over an end of it, -infinity outside.  Out of line: a row has two of them at most.
+template <typename T> __device__ __noinline__ uint4 edge_piece(const T* base, int at, int vocab) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            w[i] = at + i >= 0 && at + i < vocab ? reinterpret_cast<const uint32_t*>(base)[at + i] : 0xff800000u;
+        } else {
+            const uint32_t low = std::is_same<T, __nv_bfloat16>::value ? 0xff80u : 0xfc00u;
+            const unsigned short* p = reinterpret_cast<const unsigned short*>(base);
+            const int j = at + 2 * i;
+            w[i] = (j >= 0 && j < vocab ? p[j] : low) | (j + 1 >= 0 && j + 1 < vocab ? p[j + 1] : low) << 16;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 2^x for x <= 0, to 2^-22 of the value; below 2^-126 zero
+__device__ __forceinline__ float exp2_down(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kSliceThreads) beam_slice_kernel(const BeamArgs a) {
-    constexpr int VEC = 16 / sizeof(T), NV = kPerThread / VEC;
-    __shared__ float group_top[kBeamGroups];
-    __shared__ double warp_sum_s[kSliceThreads / 32];
+__global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const BeamArgs a) {
+    constexpr int VEC = Piece<T>::kValues, NV = kPieces, kWarps = kSliceThreads / 32;
+    __shared__ float group_top[kBeamGroups], warp_top[kWarps];
+    __shared__ double warp_part[kWarps];
     __shared__ u64 keep[kBeamKeep];
-    __shared__ float bound_s, top_s;
+    __shared__ unsigned int bound_s;
     __shared__ int count_s, red[32];
     pdl_launch_dependents();
     pdl_wait();
@@ -84,86 +136,148 @@ __global__ void __launch_bounds__(kSliceThreads) beam_slice_kernel(const BeamArg
     const int off = static_cast<int>(reinterpret_cast<uintptr_t>(base) / sizeof(T) % VEC);
     const int pieces = (a.vocab + off + VEC - 1) / VEC;
     const int lo = static_cast<int>(static_cast<int64_t>(pieces) * slice / a.slices), hi = static_cast<int>(static_cast<int64_t>(pieces) * (slice + 1) / a.slices);
-    float x[kPerThread];
-    unsigned int have = 0;              // bit per value: inside the row
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = lo + j * kSliceThreads + threadIdx.x, at = c * VEC - off;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) x[j * VEC + i] = -INFINITY;
-        if (c >= hi) continue;
-        if (at >= 0 && at + VEC <= a.vocab) {
-            const uint4 v = ld_stream16(base + at);
-            const T* t = reinterpret_cast<const T*>(&v);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) x[j * VEC + i] = static_cast<float>(t[i]);
-            have |= ((1u << VEC) - 1u) << (j * VEC);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (at + i >= 0 && at + i < a.vocab) {
-                    x[j * VEC + i] = static_cast<float>(base[at + i]);
-                    have |= 1u << (j * VEC + i);
-                }
-        }
-    }
-    auto token_of = [&](int i) { return (lo + i / VEC * kSliceThreads + static_cast<int>(threadIdx.x)) * VEC - off + i % VEC; };
-    auto key_of = [&](int i) -> u64 {
-        if (!(have >> i & 1) || x[i] != x[i]) return 0;
-        return (static_cast<u64>(ord32(x[i])) << 32) | static_cast<unsigned int>(~token_of(i));
-    };
-
-    // ---- maxima of 64 groups, the k-th largest of them, the slice's maximum
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < kPerThread; ++i) top = fmaxf(top, x[i]);
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((lane & 7) == 0) group_top[threadIdx.x >> 3] = top;
+    const int64_t at_slice = static_cast<int64_t>(row) * a.slices + slice;
+    u64* out = a.keys + at_slice * a.k;
     if (threadIdx.x == 0) count_s = 0;
-    __syncthreads();
-    if (threadIdx.x < kBeamGroups) {
-        const float mine = group_top[threadIdx.x];
-        int rank = 0;
-#pragma unroll 8
-        for (int i = 0; i < kBeamGroups; ++i) {
-            const float g = group_top[i];
-            rank += g > mine || (g == mine && i < static_cast<int>(threadIdx.x));
-        }
-        if (rank == 0) top_s = mine;
-        if (rank == a.k - 1) bound_s = mine;
-    }
-    __syncthreads();
-    const float bound = bound_s, m = top_s, shift = m == -INFINITY ? 0.f : m;
 
-    // ---- sum of exp, in 64 bits from 16 values on; the values that can be among the k largest
-    float part = 0.f;
+    // the thread's maximum and its sum of exp below it, in 64 bits from 32 values on
+    float top = -INFINITY, bound = 0.f;
+    double sum = 0.0;
+    bool over = false;                  // more candidates than there is room for
+    Piece<T> ahead[NV];                 // the next step's pieces are on their way while a step is worked on
+    const int full0 = off ? 1 : 0, full1 = (a.vocab + off) / VEC;      // pieces that lie in the row entirely
+    auto fetch = [&](int p0) {
+        if (p0 >= full0 && p0 + kSliceThreads * NV <= min(hi, full1)) {
+            const T* from = base + (static_cast<int64_t>(p0 + threadIdx.x) * VEC - off);
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-        if (have >> i & 1) {
-            part += exp2f((x[i] - shift) * 1.4426950408889634f);
-            if (x[i] >= bound) {
-                const int at = atomicAdd(&count_s, 1);
-                if (at < kBeamKeep) keep[at] = key_of(i);
+            for (int j = 0; j < NV; ++j) ahead[j] = ld_stream16(from + j * kSliceThreads * VEC);
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = p0 + j * kSliceThreads + threadIdx.x, at = c * VEC - off;
+            if (c < hi && at >= 0 && at + VEC <= a.vocab) ahead[j] = ld_stream16(base + at);
+            else ahead[j] = edge_piece(base, at, c < hi ? a.vocab : 0);
+        }
+    };
+    fetch(lo);
+    int step = 0;
+    for (int p0 = lo; p0 < hi; p0 += kSliceThreads * NV, ++step) {
+        Piece<T> x[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) x[j] = ahead[j];
+        if (p0 + kSliceThreads * NV < hi) fetch(p0 + kSliceThreads * NV);
+        float piece_top[NV], new_top = top;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            piece_top[j] = x[j].top();
+            new_top = fmaxf(new_top, piece_top[j]);
+        }
+        const float shift = new_top == -INFINITY ? 0.f : new_top;
+        const float2 minus = make_float2(-shift, -shift), log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+        float2 part = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) {
+                const float2 e = mul2(add2(make_float2(x[j].value(i), x[j].value(i + 1)), minus), log2e);
+                part = add2(part, make_float2(exp2_down(e.x), exp2_down(e.y)));
             }
+        sum = fma(sum, static_cast<double>(exp2_down((top - shift) * 1.4426950408889634f)), static_cast<double>(part.x + part.y));
+        top = new_top;
+        if (p0 == lo) {
+            // the k-th largest maximum of 64 groups of lanes (of 128 for many beams) bounds the k-th largest value of the slice from below
+            const int lanes = a.k > 16 ? 2 : 4, groups = kSliceThreads / lanes, mine_i = threadIdx.x / lanes;
+            float group = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            if (lanes == 4) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, 2));
+            if (threadIdx.x % lanes == 0) group_top[mine_i] = group;
+            if (threadIdx.x == 0) bound_s = 0xffffffffu;
+            __syncthreads();
+            int above = 0;
+#pragma unroll 16
+            for (int i = threadIdx.x % lanes; i < groups; i += lanes) above += group_top[i] > group;
+            above += __shfl_xor_sync(0xffffffffu, above, 1);
+            if (lanes == 4) above += __shfl_xor_sync(0xffffffffu, above, 2);
+            if (threadIdx.x % lanes == 0 && above < a.k) atomicMin(&bound_s, ord32(group));
+            __syncthreads();
+            bound = unord32(bound_s);
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (piece_top[j] >= bound) {
+                uint32_t there = 0;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) there |= static_cast<uint32_t>(x[j].value(i) >= bound) << i;
+                const int first = (p0 + j * kSliceThreads + static_cast<int>(threadIdx.x)) * VEC - off, end = min(a.vocab, hi * VEC - off);
+                for (; there; there &= there - 1) {
+                    const int i = __ffs(there) - 1, token = first + i;
+                    if (token < 0 || token >= end) continue;
+                    float v = x[j].value(0);
+#pragma unroll
+                    for (int n = 1; n < VEC; ++n) v = n == i ? x[j].value(n) : v;
+                    const int to = atomicAdd(&count_s, 1);
+                    if (to < kBeamKeep) keep[to] = (static_cast<u64>(ord32(v)) << 32) | static_cast<unsigned int>(~token);
+                }
+            }
+        if ((step & 3) == 3 && p0 + kSliceThreads * NV < hi) {
+            // half full: only the k largest so far go on, and what follows has to reach the last of them
+            __syncthreads();
+            const int count = count_s;
+            if (count > kBeamKeep) {
+                over = true;
+            } else if (count > kBeamKeep / 2) {
+                u64 mine[kBeamKeep / kSliceThreads];
+                int rank[kBeamKeep / kSliceThreads];
+#pragma unroll
+                for (int i = 0; i < kBeamKeep / kSliceThreads; ++i) {
+                    const int n = i * kSliceThreads + threadIdx.x;
+                    mine[i] = n < count ? keep[n] : 0;
+                    rank[i] = n < count ? 0 : a.k;
+                }
+                for (int j = 0; j < count; ++j) {
+                    const u64 other = keep[j];
+#pragma unroll
+                    for (int i = 0; i < kBeamKeep / kSliceThreads; ++i) rank[i] += other > mine[i];
+                }
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < kBeamKeep / kSliceThreads; ++i) {
+                    if (rank[i] < a.k) keep[rank[i]] = mine[i];
+                    if (rank[i] == a.k - 1) bound_s = static_cast<unsigned int>(mine[i] >> 32);
+                }
+                if (threadIdx.x == 0) count_s = a.k;
+                __syncthreads();
+                bound = unord32(bound_s);
+            }
+            __syncthreads();
         }
     }
-    double sum = part;
+
+    // ---- the CTA's maximum and sum
+    float all = top;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+    if (top != all && top > -INFINITY) sum *= exp2_down((top - all) * 1.4426950408889634f);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) warp_sum_s[warp] = sum;
-    __syncthreads();
-    const int64_t at = static_cast<int64_t>(row) * a.slices + slice;
-    if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int i = 0; i < kSliceThreads / 32; ++i) t += warp_sum_s[i];
-        a.sums[at] = t;
-        a.tops[at] = m;
+    if (lane == 0) {
+        warp_top[warp] = all;
+        warp_part[warp] = sum;
     }
-    u64* out = a.keys + at * a.k;
+    __syncthreads();
+    if (threadIdx.x == kSliceThreads - 1) {
+        float m = warp_top[0];
+#pragma unroll
+        for (int i = 1; i < kWarps; ++i) m = fmaxf(m, warp_top[i]);
+        double t = 0.0;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) t += warp_top[i] == m || warp_top[i] == -INFINITY ? warp_part[i] : warp_part[i] * exp2_down((warp_top[i] - m) * 1.4426950408889634f);
+        a.sums[at_slice] = t;
+        a.tops[at_slice] = m;
+    }
     const int count = count_s;
-    if (count <= kBeamKeep) {
+    if (!over && count <= kBeamKeep) {
         for (int i = threadIdx.x; i < count; i += kSliceThreads) {
             const u64 mine = keep[i];
             int rank = 0;
@@ -173,21 +287,25 @@ __global__ void __launch_bounds__(kSliceThreads) beam_slice_kernel(const BeamArg
         for (int i = count + threadIdx.x; i < a.k; i += kSliceThreads) out[i] = 0;
         return;
     }
-    // many equal values: the k-th largest key bit by bit (keys differ, so exactly k are at or above it)
+    // many equal values: the k-th largest key bit by bit (keys differ, so exactly k are at or above it), the slice read again each time
+    const int first = max(lo * VEC - off, 0), last = min(hi * VEC - off, a.vocab);
+    auto key_at = [&](int token) -> u64 {
+        const float v = static_cast<float>(base[token]);
+        return v != v ? 0 : (static_cast<u64>(ord32(v)) << 32) | static_cast<unsigned int>(~token);
+    };
     u64 edge = 0;
+#pragma unroll 1
     for (int bit = 63; bit >= 0; --bit) {
         const u64 next = edge | (1ull << bit);
         int n = 0;
-#pragma unroll
-        for (int i = 0; i < kPerThread; ++i) n += key_of(i) >= next;
+        for (int i = first + threadIdx.x; i < last; i += kSliceThreads) n += key_at(i) >= next;
         if (cta_sum(n, red) >= a.k) edge = next;
     }
     __syncthreads();
     if (threadIdx.x == 0) count_s = 0;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-        const u64 key = key_of(i);
+    for (int i = first + threadIdx.x; i < last; i += kSliceThreads) {
+        const u64 key = key_at(i);
         if (key != 0 && key >= edge) out[atomicAdd(&count_s, 1)] = key;
     }
     __syncthreads();
@@ -279,15 +397,19 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamArgs 
     }
     if ((lane & 7) == 0) group_top[threadIdx.x >> 3] = top;
     __syncthreads();
-    if (threadIdx.x < kJoinThreads / 8) {
-        const u64 mine = group_top[threadIdx.x];
+    {
+        const int mine_i = threadIdx.x >> 3;                       // eight threads a group
+        const u64 mine = group_top[mine_i];
         int rank = 0;
-#pragma unroll 8
-        for (int i = 0; i < kJoinThreads / 8; ++i) {
-            const u64 g = group_top[i];
-            rank += g > mine || (g == mine && i < static_cast<int>(threadIdx.x));
+#pragma unroll
+        for (int i = 0; i < kJoinThreads / 64; ++i) {
+            const int other = 8 * i + (lane & 7);
+            const u64 g = group_top[other];
+            rank += g > mine || (g == mine && other < mine_i);
         }
-        if (rank == k - 1) bound_s = mine;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        if ((lane & 7) == 0 && rank == k - 1) bound_s = mine;
     }
     __syncthreads();
     const u64 bound = bound_s;
@@ -409,14 +531,20 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
     }
 }
 
-static int beam_slices(int vocab) { return (vocab + 8 + kSliceValues - 1) / kSliceValues; }
+// Slices of a row: no more than there are steps, and together about two waves of CTAs (four on an SM at a time).  A CTA's first step
+// finds its bound, which costs as much as the step; those behind it are cheap.
+static int beam_slices(int rows, int vocab, int type) {
+    const int64_t bytes = (static_cast<int64_t>(vocab) + 8) * (type == 2 ? 4 : 2);
+    const int most = static_cast<int>((bytes + kStepBytes - 1) / kStepBytes), share = 8 * sm_count() / (rows > 0 ? rows : 1);
+    return share < 1 ? 1 : (share < most ? share : most);
+}
 
 }  // namespace nexrt
 
 using namespace nexrt;
 
 // Slices of a row: a call's scratch is batch * beams * slices * (k + 2) words of 8 bytes.
-extern "C" int nexrt_beam_slices(int vocab) { return beam_slices(vocab); }
+extern "C" int nexrt_beam_slices(int rows, int vocab, int type) { return beam_slices(rows, vocab, type); }
 
 // type: 0 bf16, 1 fp16, 2 fp32; strides: logits (request, beam), scores, finished, in elements.
 extern "C" int nexrt_beam_select(const void* logits, const void* scores, const void* finished, const int64_t* strides, void* scores_out, void* rows_out, void* tokens_out,
@@ -428,7 +556,7 @@ extern "C" int nexrt_beam_select(const void* logits, const void* scores, const v
     BeamArgs a = {};
     a.logits = logits; a.scores = static_cast<const float*>(scores); a.finished = static_cast<const unsigned char*>(finished);
     a.l_b = strides[0]; a.l_w = strides[1]; a.s_b = strides[2]; a.s_w = strides[3]; a.f_b = strides[4]; a.f_w = strides[5];
-    a.batch = batch; a.beams = beams; a.vocab = vocab; a.k = k; a.eos = eos; a.slices = beam_slices(vocab);
+    a.batch = batch; a.beams = beams; a.vocab = vocab; a.k = k; a.eos = eos; a.slices = beam_slices(batch * beams, vocab, type);
     const int64_t parts = static_cast<int64_t>(batch) * beams * a.slices;
     a.keys = static_cast<u64*>(scratch);
     a.sums = reinterpret_cast<double*>(a.keys + parts * k);

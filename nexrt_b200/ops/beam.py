@@ -49,7 +49,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, finished:
     rows, tokens = scores.new_empty((batch, k), dtype=torch.int32), scores.new_empty((batch, k), dtype=torch.int32)
     if batch:
         L = lib()
-        scratch = scores.new_empty(batch * beams * L.nexrt_beam_slices(vocab) * (k + 2), dtype=torch.int64)
+        scratch = scores.new_empty(batch * beams * L.nexrt_beam_slices(batch * beams, vocab, TYPES[logits.dtype]) * (k + 2), dtype=torch.int64)
         strides = longs(*logits.stride()[:2], *scores.stride(), *(finished.stride() if finished is not None else (0, 0)))
         on_device(device, lambda st: L.nexrt_beam_select(
             logits.data_ptr(), scores.data_ptr(), ptr(finished), strides, best.data_ptr(), rows.data_ptr(), tokens.data_ptr(), scratch.data_ptr(), ptr(status), batch, beams,

@@ -118,7 +118,7 @@ _PROTOTYPES = {
     "nexrt_page_fork": [vp] + [ci] * 5 + [vp, c_int64, ci, ci, vp, vp, vp, ci, vp, c_int64, vp, vp, vp, vp, ci, vp],
     "nexrt_page_compact": [vp] + [ci] * 5 + [vp, c_int64, ci, ci, vp, vp, c_int64] + [vp] * 6,
     "nexrt_page_copy": [vp] + [ci] * 5 + [vp, vp, ci, vp, vp, vp],
-    "nexrt_beam_slices": [ci],
+    "nexrt_beam_slices": [ci, ci, ci],
     "nexrt_beam_select": [vp] * 3 + [I64] + [vp] * 5 + [ci] * 6 + [vp],
     "nexrt_reorder_rows": [vp, vp, I64, ci, vp, c_int64, c_int64, ci, ci, ci, vp, vp],
     "nexrt_ipc_alloc": [c_size_t, POINTER(c_void_p)],
