@@ -7,6 +7,7 @@
 #pragma once
 
 #include <stddef.h>
+#include <stdint.h>
 
 #ifdef __cplusplus
 extern "C" {
@@ -206,33 +207,69 @@ int nexrt_attn_front_tail(const void* pre, const void* ctl, void* q_raw, void* g
                           int cache_len, int ksplit, void* stream);   /* pre: [ksplit][M][R] partial planes of a chunk's GEMM */
 
 // ---- a key-value cache in pages, shared by several sequences (rope.cu, paged_attn.cu, pages.cu) -------------------------
-// Pools: [pages][kv heads][slots][dim], one for K and one for V of every layer; table: int32 [rows][width], -1 where there is no page.
-// Types: 0 bf16, 1 fp16, 2 fp32.  A bad page or row is left out and latches kStatusBadPage in `status` (may be NULL).
-int nexrt_rope_append(const void* q, const void* k, const void* v, const void* positions, const void* rows, void* q_out, void* k_out, void* v_out,
-                      const void* table, const void* inv_freq, const void* q_norm, const void* k_norm, void* status, const int64_t* strides, int tokens, int q_heads,
-                      int kv_heads, int dim, int rotary, int interleaved, int table_rows, int width, int page, int pages, int in_type, int out_type, float scale,
-                      float eps, void* stream);   /* table NULL: q alone, kv_heads 0; strides: (token, head) of q, k, v, q_out, (page, head, slot) of the pools, row of the table */
-int nexrt_paged_ctas(int seqs, int q_heads, int kv_heads, int width, int page, int window);   /* CTAs of a call: its scratch is that many times 32 (dim + 2) + 4 floats */
-int nexrt_paged_attn(const void* q, const void* k_pages, const void* v_pages, const void* table, const void* lens, const void* slopes, void* out, void* lse,
-                     void* scratch, void* status, const int64_t* strides, int seqs, int q_heads, int kv_heads, int dim, int width, int page, int pages, int window,
-                     int type, float scale, float softcap, int ctas, void* stream);   /* strides: (sequence, head) of q and out, (page, head, slot) of the pools, rows of the table and of lse */
+// These entry points take their arguments as one block (ops/rope.py, ops/paged.py and ops/beam.py pack it; `size` is that of the block
+// and checked).  Pools: [pages][kv heads][slots][dim], one for K and one for V of every layer; table: int32 [rows][width], -1 where
+// there is no page.  Types: 0 bf16, 1 fp16, 2 fp32.  Strides count elements.  A bad page or row is left out and latches kStatusBadPage
+// in `status` (may be NULL).
+typedef struct NexrtRopeArgs {
+    uint64_t size;
+    const void *q, *k, *v, *positions, *rows;
+    void *q_out, *k_pages, *v_pages;
+    const void *table, *inv_freq, *q_norm, *k_norm;   /* table NULL: q alone, kv_heads 0 */
+    void* status;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head, page, head, slot, table_row;
+    int tokens, q_heads, kv_heads, dim, rotary, interleaved, table_rows, width, slots, pages, in_type, out_type;
+    float scale, eps;
+} NexrtRopeArgs;
+int nexrt_rope_append(const NexrtRopeArgs* args, void* stream);
+
+typedef struct NexrtPagedAttnArgs {
+    uint64_t size;
+    const void *q, *k_pages, *v_pages, *table, *lens, *slopes;
+    void *out, *lse, *scratch, *status;               /* slopes, lse may be NULL; scratch: ctas times 32 (dim + 2) + 4 floats */
+    int64_t q_row, q_head, out_row, out_head, page, head, slot, table_row, lse_row;
+    int rows, q_heads, kv_heads, dim, width, slots, pages, window, type, ctas;   /* ctas: at most nexrt_paged_ctas of the call */
+    float scale, softcap;
+} NexrtPagedAttnArgs;
+int nexrt_paged_attn(const NexrtPagedAttnArgs* args, void* stream);
+int nexrt_paged_item_cost(void);                      /* chunks of 64 keys that an item counts in the split beside its own */
 int64_t nexrt_paged_slot(const int* table, int64_t stride, int rows, int width, int page, int pages, int row, int pos);   /* host: slot of the pool that holds a position, or -1 */
 int nexrt_paged_split(const int* lens, int seqs, int items, int64_t room, int window, int grid, int64_t* out, int most);   /* host: how the keys are split over CTAs */
-int nexrt_page_fork(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* table, int64_t table_stride, int rows, int width,
-                    const void* lens, const void* parents, const void* grow, int grow_all, void* table_out, int64_t out_stride, void* lens_out, void* refs,
-                    void* scratch, void* status, int rows_out, void* stream);   /* scratch: int[pages + 3 rows_out] */
-int nexrt_page_compact(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* table, int64_t table_stride, int rows, int width,
-                       const void* lens, void* table_out, int64_t out_stride, void* refs_out, void* remap, void* live, void* scratch, void* status,
-                       void* stream);   /* scratch: int[5 pages + 1] */
-int nexrt_page_copy(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* src, const void* dst, int n, void* scratch, void* status,
-                    void* stream);   /* scratch: int[3 n] */
+
+typedef struct NexrtPagesArgs {
+    uint64_t size;
+    void* pool;
+    const void *table, *lens, *parents, *grow;        /* parents, grow: of a fork; grow NULL: grow_all for all rows */
+    void *table_out, *lens_out, *refs, *remap, *live, *scratch, *status;
+    int64_t table_row, out_row;
+    int planes, pages, heads, slots, slot_bytes, rows, width, rows_out, grow_all, reserved;
+} NexrtPagesArgs;
+int nexrt_page_fork(const NexrtPagesArgs* args, void* stream);      /* scratch: int[pages + 3 rows_out] */
+int nexrt_page_compact(const NexrtPagesArgs* args, void* stream);   /* scratch: int[5 pages + 1] */
+int nexrt_page_copy(const NexrtPagesArgs* args, void* stream);      /* table: sources, lens: targets, rows of them; scratch: int[3 rows] */
 
 // ---- beam search (beam.cu) ------------------------------------------------------------------------------------------------
 int nexrt_beam_slices(int rows, int vocab, int type);   /* a call's scratch is batch * beams * slices * (k + 2) words of 8 bytes */
-int nexrt_beam_select(const void* logits, const void* scores, const void* finished, const int64_t* strides, void* scores_out, void* rows_out, void* tokens_out,
-                      void* scratch, void* status, int batch, int beams, int vocab, int k, int eos, int type, void* stream);   /* k <= 64, beams <= 256 */
-int nexrt_reorder_rows(const void* const* in, void* const* out, const int64_t* meta, int tensors, const void* rows, int64_t r_0, int64_t r_1, int cols, int n,
-                       int n_in, void* status, void* stream);   /* out[t][i] = in[t][rows[i]], at most 16 tensors */
+typedef struct NexrtBeamArgs {
+    uint64_t size;
+    const void *logits, *scores, *finished;           /* finished may be NULL */
+    void *scores_out, *rows_out, *tokens_out, *scratch, *status;
+    int64_t logits_request, logits_beam, scores_request, scores_beam, finished_request, finished_beam;
+    int batch, beams, vocab, k, eos, type, slices, reserved;   /* k <= 64, beams <= 256 */
+} NexrtBeamArgs;
+int nexrt_beam_select(const NexrtBeamArgs* args, void* stream);
+
+typedef struct NexrtReorderArgs {
+    uint64_t size;
+    const void* rows;
+    void* status;
+    int64_t rows_0, rows_1;
+    int cols, n, n_in, tensors;
+    const void* in[16];                               /* out[t][i] = in[t][rows[i]] */
+    void* out[16];
+    int64_t in_row[16], out_row[16], bytes[16];       /* bytes between rows, and of a row */
+} NexrtReorderArgs;
+int nexrt_reorder_rows(const NexrtReorderArgs* args, void* stream);
 
 #ifdef __cplusplus
 }

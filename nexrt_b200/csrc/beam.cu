@@ -546,51 +546,46 @@ using namespace nexrt;
 // Slices of a row: a call's scratch is batch * beams * slices * (k + 2) words of 8 bytes.
 extern "C" int nexrt_beam_slices(int rows, int vocab, int type) { return beam_slices(rows, vocab, type); }
 
-// type: 0 bf16, 1 fp16, 2 fp32; strides: logits (request, beam), scores, finished, in elements.
-extern "C" int nexrt_beam_select(const void* logits, const void* scores, const void* finished, const int64_t* strides, void* scores_out, void* rows_out, void* tokens_out,
-                                 void* scratch, void* status, int batch, int beams, int vocab, int k, int eos, int type, void* stream) {
-    if (batch < 0 || beams < 1 || beams > kBeamMaxWidth || vocab < 1 || vocab > kBeamMaxVocab || k < 1 || k > kBeamMaxK || static_cast<int64_t>(beams) * vocab < k ||
-        (finished != nullptr && (eos < 0 || eos >= vocab)) || static_cast<int64_t>(batch) * beams > 65535)
+extern "C" int nexrt_beam_select(const NexrtBeamArgs* x, void* stream) {
+    if (x->size != sizeof(*x) || x->batch < 0 || x->beams < 1 || x->beams > kBeamMaxWidth || x->vocab < 1 || x->vocab > kBeamMaxVocab || x->k < 1 || x->k > kBeamMaxK ||
+        static_cast<int64_t>(x->beams) * x->vocab < x->k || (x->finished != nullptr && (x->eos < 0 || x->eos >= x->vocab)) ||
+        static_cast<int64_t>(x->batch) * x->beams > 65535 || x->type < 0 || x->type > 2 || x->slices != beam_slices(x->batch * x->beams, x->vocab, x->type))
         return cudaErrorInvalidValue;
-    if (batch == 0) return 0;
+    if (x->batch == 0) return 0;
     BeamArgs a = {};
-    a.logits = logits; a.scores = static_cast<const float*>(scores); a.finished = static_cast<const unsigned char*>(finished);
-    a.l_b = strides[0]; a.l_w = strides[1]; a.s_b = strides[2]; a.s_w = strides[3]; a.f_b = strides[4]; a.f_w = strides[5];
-    a.batch = batch; a.beams = beams; a.vocab = vocab; a.k = k; a.eos = eos; a.slices = beam_slices(batch * beams, vocab, type);
-    const int64_t parts = static_cast<int64_t>(batch) * beams * a.slices;
-    a.keys = static_cast<u64*>(scratch);
-    a.sums = reinterpret_cast<double*>(a.keys + parts * k);
+    a.logits = x->logits; a.scores = static_cast<const float*>(x->scores); a.finished = static_cast<const unsigned char*>(x->finished);
+    a.l_b = x->logits_request; a.l_w = x->logits_beam; a.s_b = x->scores_request; a.s_w = x->scores_beam; a.f_b = x->finished_request; a.f_w = x->finished_beam;
+    a.batch = x->batch; a.beams = x->beams; a.vocab = x->vocab; a.k = x->k; a.eos = x->eos; a.slices = x->slices;
+    const int64_t parts = static_cast<int64_t>(x->batch) * x->beams * x->slices;
+    a.keys = static_cast<u64*>(x->scratch);
+    a.sums = reinterpret_cast<double*>(a.keys + parts * x->k);
     a.tops = reinterpret_cast<float*>(a.sums + parts);
-    a.scores_out = static_cast<float*>(scores_out); a.rows_out = static_cast<int*>(rows_out); a.tokens_out = static_cast<int*>(tokens_out);
-    a.status = static_cast<int*>(status);
+    a.scores_out = static_cast<float*>(x->scores_out); a.rows_out = static_cast<int*>(x->rows_out); a.tokens_out = static_cast<int*>(x->tokens_out);
+    a.status = static_cast<int*>(x->status);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const dim3 grid(a.slices, batch * beams);
-    int e = cudaErrorInvalidValue;
-    if (type == 0) e = launch(beam_slice_kernel<__nv_bfloat16>, grid, dim3(kSliceThreads), 0, st, a);
-    else if (type == 1) e = launch(beam_slice_kernel<__half>, grid, dim3(kSliceThreads), 0, st, a);
-    else if (type == 2) e = launch(beam_slice_kernel<float>, grid, dim3(kSliceThreads), 0, st, a);
+    const dim3 grid(a.slices, a.batch * a.beams), block(kSliceThreads);
+    const int e = x->type == 0 ? launch(beam_slice_kernel<__nv_bfloat16>, grid, block, 0, st, a)
+                               : (x->type == 1 ? launch(beam_slice_kernel<__half>, grid, block, 0, st, a) : launch(beam_slice_kernel<float>, grid, block, 0, st, a));
     if (e) return e;
-    return launch(beam_join_kernel, dim3(batch), dim3(kJoinThreads), 0, st, a);
+    return launch(beam_join_kernel, dim3(a.batch), dim3(kJoinThreads), 0, st, a);
 }
 
-// in, out, meta: arrays of `tensors` (at most 16) pointers and of 3 int64 each (row stride of in, of out, bytes of a row).
-extern "C" int nexrt_reorder_rows(const void* const* in, void* const* out, const int64_t* meta, int tensors, const void* rows, int64_t r_0, int64_t r_1, int cols, int n,
-                                  int n_in, void* status, void* stream) {
-    if (tensors < 0 || tensors > kReorderTensors || n < 0 || cols < 1 || n_in < 0) return cudaErrorInvalidValue;
+extern "C" int nexrt_reorder_rows(const NexrtReorderArgs* x, void* stream) {
+    if (x->size != sizeof(*x) || x->tensors < 0 || x->tensors > kReorderTensors || x->n < 0 || x->cols < 1 || x->n_in < 0) return cudaErrorInvalidValue;
     ReorderArgs a = {};
-    for (int t = 0; t < tensors; ++t) {
-        a.in[t] = static_cast<const char*>(in[t]);
-        a.out[t] = static_cast<char*>(out[t]);
-        a.in_stride[t] = meta[3 * t]; a.out_stride[t] = meta[3 * t + 1]; a.bytes[t] = meta[3 * t + 2];
+    for (int t = 0; t < x->tensors; ++t) {
+        a.in[t] = static_cast<const char*>(x->in[t]);
+        a.out[t] = static_cast<char*>(x->out[t]);
+        a.in_stride[t] = x->in_row[t]; a.out_stride[t] = x->out_row[t]; a.bytes[t] = x->bytes[t];
         if (a.bytes[t] < 0) return cudaErrorInvalidValue;
-        const uint64_t all = reinterpret_cast<uintptr_t>(in[t]) | reinterpret_cast<uintptr_t>(out[t]) | static_cast<uint64_t>(a.in_stride[t]) |
-                             static_cast<uint64_t>(a.out_stride[t]) | static_cast<uint64_t>(a.bytes[t]);
+        const uint64_t all = reinterpret_cast<uintptr_t>(x->in[t]) | reinterpret_cast<uintptr_t>(x->out[t]) | static_cast<uint64_t>(x->in_row[t]) |
+                             static_cast<uint64_t>(x->out_row[t]) | static_cast<uint64_t>(x->bytes[t]);
         a.width[t] = all % 16 == 0 ? 16 : (all % 4 == 0 ? 4 : 1);
         a.first[t + 1] = a.first[t] + (a.bytes[t] + kReorderPiece - 1) / kReorderPiece;
     }
-    a.rows = static_cast<const int*>(rows); a.r_0 = r_0; a.r_1 = r_1; a.cols = cols; a.n = n; a.n_in = n_in; a.tensors = tensors;
-    a.status = static_cast<int*>(status);
-    const int64_t units = a.first[tensors] * n, most = 8ll * sm_count();
+    a.rows = static_cast<const int*>(x->rows); a.r_0 = x->rows_0; a.r_1 = x->rows_1; a.cols = x->cols; a.n = x->n; a.n_in = x->n_in; a.tensors = x->tensors;
+    a.status = static_cast<int*>(x->status);
+    const int64_t units = a.first[x->tensors] * x->n, most = 8ll * sm_count();
     if (units == 0) return 0;
     return launch(reorder_kernel, dim3(static_cast<unsigned>(units < most ? units : most)), dim3(kReorderThreads), 0, static_cast<cudaStream_t>(stream), a);
 }

@@ -635,43 +635,34 @@ template <typename T> static int paged_dispatch(const PagedAttnArgs& a, int dim,
 
 using namespace nexrt;
 
-// CTAs of a call: its scratch is that many times 32 (dim + 2) + 4 floats.
-extern "C" int nexrt_paged_ctas(int seqs, int q_heads, int kv_heads, int width, int page, int window) {
-    if (seqs < 1 || kv_heads < 1 || q_heads < kv_heads) return 1;
-    const int64_t room = static_cast<int64_t>(width) * page;
-    const int64_t keys = window > 0 && window < room ? window + kChunk : room;
-    const int64_t most = (keys / kChunk + 1 + kItemCost) * seqs * kv_heads * ((q_heads / kv_heads + kPaRows - 1) / kPaRows);
-    const int64_t resident = 2ll * sm_count();
-    return static_cast<int>(most < resident ? most : (resident < kMaxCtas ? resident : kMaxCtas));
-}
+extern "C" int nexrt_paged_item_cost(void) { return kItemCost; }
 
-// type: 0 bf16, 1 fp16.  strides: q (sequence, head), out, pools (page, head, slot), table row, lse row - in elements.
-extern "C" int nexrt_paged_attn(const void* q, const void* k_pages, const void* v_pages, const void* table, const void* lens, const void* slopes, void* out, void* lse,
-                                void* scratch, void* status, const int64_t* strides, int seqs, int q_heads, int kv_heads, int dim, int width, int page, int pages,
-                                int window, int type, float scale, float softcap, int ctas, void* stream) {
-    if (seqs < 0 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads || width < 0 || page < 1 || pages < 0 || window < 0 || ctas < 1 || ctas > kMaxCtas || !(softcap >= 0.f))
+extern "C" int nexrt_paged_attn(const NexrtPagedAttnArgs* x, void* stream) {
+    if (x->size != sizeof(*x)) return cudaErrorInvalidValue;
+    if (x->rows < 0 || x->kv_heads < 1 || x->q_heads < 1 || x->q_heads % x->kv_heads || x->width < 0 || x->slots < 1 || x->pages < 0 || x->window < 0 || x->ctas < 1 ||
+        x->ctas > kMaxCtas || !(x->softcap >= 0.f))
         return cudaErrorInvalidValue;
-    if (seqs == 0) return 0;
-    PagedAttnArgs a = {};
-    a.q = q; a.k = k_pages; a.v = v_pages; a.out = out; a.lse = static_cast<float*>(lse);
-    a.q_b = strides[0]; a.q_h = strides[1]; a.o_b = strides[2]; a.o_h = strides[3];
-    a.head_s = strides[5]; a.lse_b = strides[8];
-    if (((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) || strides[4] % 8 || strides[5] % 8 || strides[6] % 8) return cudaErrorInvalidValue;
+    if (x->rows == 0) return 0;
+    if (((reinterpret_cast<uintptr_t>(x->k_pages) | reinterpret_cast<uintptr_t>(x->v_pages)) & 15) || x->page % 8 || x->head % 8 || x->slot % 8) return cudaErrorInvalidValue;
     // a row is named by its place in units of 16 bytes: pools of up to 64 GB
-    if (strides[4] < 0 || strides[6] < 0 || (pages > 0 ? pages - 1 : 0) * (strides[4] / 8) + (page - 1) * (strides[6] / 8) >= kNoRow) return cudaErrorInvalidValue;
-    a.page_s = static_cast<uint32_t>(strides[4] / 8); a.slot_s = static_cast<uint32_t>(strides[6] / 8);
-    a.table = {static_cast<const int*>(table), strides[7], seqs, width, page, pages};
-    a.lens = static_cast<const int*>(lens); a.slopes = static_cast<const float*>(slopes);
-    a.cuts = static_cast<int4*>(scratch);
-    a.ws_o = reinterpret_cast<float*>(a.cuts + ctas); a.ws_ml = a.ws_o + static_cast<int64_t>(2) * ctas * kPaRows * dim;
-    a.status = static_cast<int*>(status);
-    a.seqs = seqs; a.kv_heads = kv_heads; a.group = q_heads / kv_heads; a.head_groups = (a.group + kPaRows - 1) / kPaRows;
-    a.by_item = static_cast<int64_t>(seqs) * kv_heads * a.head_groups <= ctas;
-    a.window = window; a.grid = ctas; a.scale = scale; a.softcap = softcap;
+    if (x->page < 0 || x->slot < 0 || (x->pages > 0 ? x->pages - 1 : 0) * (x->page / 8) + (x->slots - 1) * (x->slot / 8) >= kNoRow) return cudaErrorInvalidValue;
+    PagedAttnArgs a = {};
+    a.q = x->q; a.k = x->k_pages; a.v = x->v_pages; a.out = x->out; a.lse = static_cast<float*>(x->lse);
+    a.q_b = x->q_row; a.q_h = x->q_head; a.o_b = x->out_row; a.o_h = x->out_head; a.head_s = x->head; a.lse_b = x->lse_row;
+    a.page_s = static_cast<uint32_t>(x->page / 8); a.slot_s = static_cast<uint32_t>(x->slot / 8);
+    a.table = {static_cast<const int*>(x->table), x->table_row, x->rows, x->width, x->slots, x->pages};
+    a.lens = static_cast<const int*>(x->lens); a.slopes = static_cast<const float*>(x->slopes);
+    a.cuts = static_cast<int4*>(x->scratch);
+    a.ws_o = reinterpret_cast<float*>(a.cuts + x->ctas); a.ws_ml = a.ws_o + static_cast<int64_t>(2) * x->ctas * kPaRows * x->dim;
+    a.status = static_cast<int*>(x->status);
+    a.seqs = x->rows; a.kv_heads = x->kv_heads; a.group = x->q_heads / x->kv_heads; a.head_groups = (a.group + kPaRows - 1) / kPaRows;
+    a.by_item = static_cast<int64_t>(x->rows) * x->kv_heads * a.head_groups <= x->ctas;
+    a.window = x->window; a.grid = x->ctas; a.scale = x->scale; a.softcap = x->softcap;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // with room for one chunk an item is never cut
-    const bool join = static_cast<int64_t>(width) * page > kChunk;
-    return type == 0 ? paged_dispatch<__nv_bfloat16>(a, dim, join, st) : (type == 1 ? paged_dispatch<__half>(a, dim, join, st) : static_cast<int>(cudaErrorInvalidValue));
+    const bool join = static_cast<int64_t>(x->width) * x->slots > kChunk;
+    if (x->type == 0) return paged_dispatch<__nv_bfloat16>(a, x->dim, join, st);
+    return x->type == 1 ? paged_dispatch<__half>(a, x->dim, join, st) : static_cast<int>(cudaErrorInvalidValue);
 }
 
 // Host forms of the index arithmetic above, for tests without a GPU.

@@ -364,91 +364,82 @@ __global__ void __launch_bounds__(kMoveThreads) page_move_kernel(const PageMove 
     }
 }
 
-static int move_launch(PageMove& a, void* pool, int planes, int pages, int heads, int slots, int slot_bytes, cudaStream_t st) {
-    a.pool = static_cast<char*>(pool);
-    a.planes = planes; a.heads = heads;
-    a.slot_bytes = slot_bytes; a.head_bytes = static_cast<int64_t>(slots) * slot_bytes;
-    a.page_bytes = a.head_bytes * heads; a.plane_bytes = a.page_bytes * pages;
-    const int64_t units = static_cast<int64_t>(a.n) * planes * heads * ((a.head_bytes + kMovePiece - 1) / kMovePiece);
+static int move_launch(PageMove& a, const NexrtPagesArgs& x, cudaStream_t st) {
+    a.pool = static_cast<char*>(x.pool);
+    a.planes = x.planes; a.heads = x.heads;
+    a.slot_bytes = x.slot_bytes; a.head_bytes = static_cast<int64_t>(x.slots) * x.slot_bytes;
+    a.page_bytes = a.head_bytes * x.heads; a.plane_bytes = a.page_bytes * x.pages;
+    const int64_t units = static_cast<int64_t>(a.n) * x.planes * x.heads * ((a.head_bytes + kMovePiece - 1) / kMovePiece);
     const int64_t most = 8ll * sm_count();
     int64_t grid = units < most ? units : most;
     if (a.table_out && grid < a.t.rows) grid = a.t.rows < most ? a.t.rows : most;
     return grid > 0 ? launch(page_move_kernel, dim3(static_cast<unsigned>(grid)), dim3(kMoveThreads), 0, st, a) : 0;
 }
 
-static bool pool_ok(const void* pool, int planes, int pages, int heads, int slots, int slot_bytes) {
-    return planes >= 0 && pages >= 0 && heads >= 1 && slots >= 1 && slot_bytes >= 16 && slot_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(pool) & 15) == 0;
+static bool pool_ok(const NexrtPagesArgs& x) {
+    return x.size == sizeof(x) && x.planes >= 0 && x.pages >= 0 && x.heads >= 1 && x.slots >= 1 && x.slot_bytes >= 16 && x.slot_bytes % 16 == 0 &&
+           (reinterpret_cast<uintptr_t>(x.pool) & 15) == 0 && x.rows >= 0 && x.width >= 0;
+}
+
+// Counts the pages that rows name, and writes the rows that go on.
+static int rows_launch(const NexrtPagesArgs& x, const PageTable& t, const int* parents, int* out, int* refs, int n, cudaStream_t st) {
+    if (x.pages > 0)
+        if (const cudaError_t e = cudaMemsetAsync(refs, 0, sizeof(int) * static_cast<size_t>(x.pages), st); e != cudaSuccess) return static_cast<int>(e);
+    if (n == 0 || x.width == 0) return 0;
+    const int cols = (x.width + 255) / 256;
+    return launch(fork_rows_kernel, dim3(cols < 64 ? cols : 64, n < 65535 ? n : 65535), dim3(256), 0, st, t, static_cast<const int*>(x.lens), parents, out, x.out_row, refs, n,
+                  static_cast<int*>(x.status));
 }
 
 }  // namespace nexrt
 
 using namespace nexrt;
 
-// scratch: int[pages + 3 rows_out].  grow: positions that every new row will append (null: grow_all for all).
-extern "C" int nexrt_page_fork(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* table, int64_t table_stride, int rows, int width,
-                               const void* lens, const void* parents, const void* grow, int grow_all, void* table_out, int64_t out_stride, void* lens_out, void* refs,
-                               void* scratch, void* status, int rows_out, void* stream) {
-    if (!pool_ok(pool, planes, pages, heads, slots, slot_bytes) || rows < 0 || width < 0 || rows_out < 0 || rows_out > kPlanRows) return cudaErrorInvalidValue;
+extern "C" int nexrt_page_fork(const NexrtPagesArgs* x, void* stream) {
+    if (!pool_ok(*x) || x->rows_out < 0 || x->rows_out > kPlanRows) return cudaErrorInvalidValue;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (pages > 0)
-        if (const cudaError_t e = cudaMemsetAsync(refs, 0, sizeof(int) * static_cast<size_t>(pages), st); e != cudaSuccess) return static_cast<int>(e);
-    if (rows_out == 0) return 0;
-    PageTable t = {static_cast<const int*>(table), table_stride, rows, width, slots, pages};
-    if (width > 0) {
-        const int cols = (width + 255) / 256;
-        const int e = launch(fork_rows_kernel, dim3(cols < 64 ? cols : 64, rows_out), dim3(256), 0, st, t, static_cast<const int*>(lens), static_cast<const int*>(parents),
-                             static_cast<int*>(table_out), out_stride, static_cast<int*>(refs), rows_out, static_cast<int*>(status));
-        if (e) return e;
-    }
+    const PageTable t = {static_cast<const int*>(x->table), x->table_row, x->rows, x->width, x->slots, x->pages};
+    if (const int e = rows_launch(*x, t, static_cast<const int*>(x->parents), static_cast<int*>(x->table_out), static_cast<int*>(x->refs), x->rows_out, st)) return e;
+    if (x->rows_out == 0) return 0;
     ForkPlan p = {};
-    p.t = t; p.lens = static_cast<const int*>(lens); p.parents = static_cast<const int*>(parents); p.grow = static_cast<const int*>(grow);
-    p.table = static_cast<int*>(table_out); p.table_stride = out_stride; p.lens_out = static_cast<int*>(lens_out); p.refs = static_cast<int*>(refs);
-    p.copies = static_cast<int*>(scratch) + pages; p.free_list = static_cast<int*>(scratch);
-    p.status = static_cast<int*>(status); p.n = rows_out; p.grow_all = grow_all; p.pages = pages;
-    if (const int e = launch(fork_plan_kernel, dim3(1), dim3(kPlanThreads), sizeof(int) * 2 * rows_out, st, p)) return e;
+    p.t = t; p.lens = static_cast<const int*>(x->lens); p.parents = static_cast<const int*>(x->parents); p.grow = static_cast<const int*>(x->grow);
+    p.table = static_cast<int*>(x->table_out); p.table_stride = x->out_row; p.lens_out = static_cast<int*>(x->lens_out); p.refs = static_cast<int*>(x->refs);
+    p.copies = static_cast<int*>(x->scratch) + x->pages; p.free_list = static_cast<int*>(x->scratch);
+    p.status = static_cast<int*>(x->status); p.n = x->rows_out; p.grow_all = x->grow_all; p.pages = x->pages;
+    if (const int e = launch(fork_plan_kernel, dim3(1), dim3(kPlanThreads), sizeof(int) * 2 * x->rows_out, st, p)) return e;
     PageMove m = {};
-    m.copies = p.copies; m.n = rows_out;
-    return move_launch(m, pool, planes, pages, heads, slots, slot_bytes, st);
+    m.copies = p.copies; m.n = x->rows_out;
+    return move_launch(m, *x, st);
 }
 
-// scratch: int[5 pages + 1].
-extern "C" int nexrt_page_compact(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* table, int64_t table_stride, int rows, int width,
-                                  const void* lens, void* table_out, int64_t out_stride, void* refs_out, void* remap, void* live, void* scratch, void* status,
-                                  void* stream) {
-    if (!pool_ok(pool, planes, pages, heads, slots, slot_bytes) || rows < 0 || width < 0) return cudaErrorInvalidValue;
+extern "C" int nexrt_page_compact(const NexrtPagesArgs* x, void* stream) {
+    if (!pool_ok(*x)) return cudaErrorInvalidValue;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    int* refs = static_cast<int*>(scratch);
-    if (pages > 0)
-        if (const cudaError_t e = cudaMemsetAsync(refs, 0, sizeof(int) * static_cast<size_t>(pages), st); e != cudaSuccess) return static_cast<int>(e);
-    PageTable t = {static_cast<const int*>(table), table_stride, rows, width, slots, pages};
-    if (rows > 0 && width > 0) {
-        const int cols = (width + 255) / 256;
-        const int e = launch(fork_rows_kernel, dim3(cols < 64 ? cols : 64, rows < 65535 ? rows : 65535), dim3(256), 0, st, t, static_cast<const int*>(lens),
-                             static_cast<const int*>(nullptr), static_cast<int*>(nullptr), out_stride, refs, rows, static_cast<int*>(status));
-        if (e) return e;
-    }
+    int* refs = static_cast<int*>(x->scratch);
+    const PageTable t = {static_cast<const int*>(x->table), x->table_row, x->rows, x->width, x->slots, x->pages};
+    if (const int e = rows_launch(*x, t, nullptr, nullptr, refs, x->rows, st)) return e;
+    const int64_t pages = x->pages;
     CompactPlan p = {};
-    p.refs = refs; p.refs_out = static_cast<int*>(refs_out); p.remap = static_cast<int*>(remap);
-    p.holes = refs + pages; p.copies = refs + 2 * static_cast<int64_t>(pages); p.n_copies = refs + 5 * static_cast<int64_t>(pages);
-    p.live = static_cast<int*>(live); p.pages = pages;
+    p.refs = refs; p.refs_out = static_cast<int*>(x->refs); p.remap = static_cast<int*>(x->remap);
+    p.holes = refs + pages; p.copies = refs + 2 * pages; p.n_copies = refs + 5 * pages;
+    p.live = static_cast<int*>(x->live); p.pages = x->pages;
     if (const int e = launch(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p)) return e;
     PageMove m = {};
-    m.copies = p.copies; m.n_copies = p.n_copies; m.n = pages;
-    m.t = t; m.lens = static_cast<const int*>(lens); m.remap = p.remap; m.table_out = static_cast<int*>(table_out); m.table_stride = out_stride;
-    return move_launch(m, pool, planes, pages, heads, slots, slot_bytes, st);
+    m.copies = p.copies; m.n_copies = p.n_copies; m.n = x->pages;
+    m.t = t; m.lens = static_cast<const int*>(x->lens); m.remap = p.remap; m.table_out = static_cast<int*>(x->table_out); m.table_stride = x->out_row;
+    return move_launch(m, *x, st);
 }
 
-// scratch: int[3 n].
-extern "C" int nexrt_page_copy(void* pool, int planes, int pages, int heads, int slots, int slot_bytes, const void* src, const void* dst, int n, void* scratch,
-                               void* status, void* stream) {
-    if (!pool_ok(pool, planes, pages, heads, slots, slot_bytes) || n < 0) return cudaErrorInvalidValue;
+extern "C" int nexrt_page_copy(const NexrtPagesArgs* x, void* stream) {
+    if (!pool_ok(*x)) return cudaErrorInvalidValue;
+    const int n = x->rows;
     if (n == 0) return 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    int* copies = static_cast<int*>(scratch);
-    if (const int e = launch(copy_list_kernel, dim3((n + 255) / 256), dim3(256), 0, st, static_cast<const int*>(src), static_cast<const int*>(dst), n, pages, copies,
-                             static_cast<int*>(status)))
+    int* copies = static_cast<int*>(x->scratch);
+    if (const int e = launch(copy_list_kernel, dim3((n + 255) / 256), dim3(256), 0, st, static_cast<const int*>(x->table), static_cast<const int*>(x->lens), n, x->pages, copies,
+                             static_cast<int*>(x->status)))
         return e;
     PageMove m = {};
     m.copies = copies; m.n = n;
-    return move_launch(m, pool, planes, pages, heads, slots, slot_bytes, st);
+    return move_launch(m, *x, st);
 }

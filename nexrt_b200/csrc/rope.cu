@@ -355,33 +355,31 @@ static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t
 
 using namespace nexrt;
 
-// in_type, out_type: 0 bf16, 1 fp16, 2 fp32.  table == NULL: q alone, kv_heads is 0.
-extern "C" int nexrt_rope_append(const void* q, const void* k, const void* v, const void* positions, const void* rows, void* q_out, void* k_out, void* v_out,
-                                 const void* table, const void* inv_freq, const void* q_norm, const void* k_norm, void* status, const int64_t* strides,
-                                 int tokens, int q_heads, int kv_heads, int dim, int rotary, int interleaved, int table_rows, int width, int page, int pages,
-                                 int in_type, int out_type, float scale, float eps, void* stream) {
-    if (tokens < 0 || q_heads < 0 || kv_heads < 0 || dim < 8 || dim > 256 || dim % 8 || rotary < 0 || rotary > dim || rotary % 2) return cudaErrorInvalidValue;
-    if (table != nullptr ? (page < 1 || width < 0 || pages < 0 || table_rows < 0) : kv_heads != 0) return cudaErrorInvalidValue;
-    if (tokens == 0 || q_heads + kv_heads == 0) return 0;
+extern "C" int nexrt_rope_append(const NexrtRopeArgs* x, void* stream) {
+    if (x->size != sizeof(*x)) return cudaErrorInvalidValue;
+    const bool paged = x->table != nullptr;
+    if (x->tokens < 0 || x->q_heads < 0 || x->kv_heads < 0 || x->dim < 8 || x->dim > 256 || x->dim % 8 || x->rotary < 0 || x->rotary > x->dim || x->rotary % 2) return cudaErrorInvalidValue;
+    if (paged ? (x->slots < 1 || x->width < 0 || x->pages < 0 || x->table_rows < 0) : x->kv_heads != 0) return cudaErrorInvalidValue;
+    if (x->tokens == 0 || x->q_heads + x->kv_heads == 0) return 0;
+    const int64_t head_strides[5] = {x->q_head, x->k_head, x->v_head, x->out_head, x->head};
+    for (const int64_t h : head_strides)
+        if (h < 0 || h > INT32_MAX) return cudaErrorInvalidValue;
     RopeArgs a = {};
-    a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.k_out = k_out; a.v_out = v_out;
-    for (const int i : {1, 3, 5, 7, 9})
-        if (strides[i] < 0 || strides[i] > INT32_MAX) return cudaErrorInvalidValue;
-    a.q_t = strides[0]; a.k_t = strides[2]; a.v_t = strides[4]; a.qo_t = strides[6]; a.page_s = strides[8]; a.slot_s = strides[10];
-    a.q_h = static_cast<int>(strides[1]); a.k_h = static_cast<int>(strides[3]); a.v_h = static_cast<int>(strides[5]);
-    a.qo_h = static_cast<int>(strides[7]); a.head_s = static_cast<int>(strides[9]);
-    a.positions = static_cast<const int*>(positions); a.rows = static_cast<const int*>(rows);
-    a.table = {static_cast<const int*>(table), strides[11], table_rows, width, page < 1 ? 1 : page, pages};
-    a.inv_freq = static_cast<const float*>(inv_freq); a.q_norm = static_cast<const float*>(q_norm); a.k_norm = static_cast<const float*>(k_norm);
-    a.status = static_cast<int*>(status);
-    a.tokens = tokens; a.q_heads = q_heads; a.kv_heads = kv_heads; a.dim = dim; a.rotary = rotary; a.interleaved = interleaved;
-    a.paged = table != nullptr; a.scale = scale; a.eps = eps;
+    a.q = x->q; a.k = x->k; a.v = x->v; a.q_out = x->q_out; a.k_out = x->k_pages; a.v_out = x->v_pages;
+    a.q_t = x->q_token; a.k_t = x->k_token; a.v_t = x->v_token; a.qo_t = x->out_token; a.page_s = x->page; a.slot_s = x->slot;
+    a.q_h = static_cast<int>(x->q_head); a.k_h = static_cast<int>(x->k_head); a.v_h = static_cast<int>(x->v_head);
+    a.qo_h = static_cast<int>(x->out_head); a.head_s = static_cast<int>(x->head);
+    a.positions = static_cast<const int*>(x->positions); a.rows = static_cast<const int*>(x->rows);
+    a.table = {static_cast<const int*>(x->table), x->table_row, x->table_rows, x->width, paged ? x->slots : 1, x->pages};
+    a.inv_freq = static_cast<const float*>(x->inv_freq); a.q_norm = static_cast<const float*>(x->q_norm); a.k_norm = static_cast<const float*>(x->k_norm);
+    a.status = static_cast<int*>(x->status);
+    a.tokens = x->tokens; a.q_heads = x->q_heads; a.kv_heads = x->kv_heads; a.dim = x->dim; a.rotary = x->rotary; a.interleaved = x->interleaved;
+    a.paged = paged; a.scale = x->scale; a.eps = x->eps;
     // 16-byte accesses where every head starts on such a boundary on both sides
-    bool vec = aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out) && aligned16(k_out) && aligned16(v_out);
-    for (int i = 0; i < 11; ++i) vec = vec && strides[i] % 8 == 0;
-    a.vec = vec;
+    const int64_t strides = x->q_token | x->q_head | x->k_token | x->k_head | x->v_token | x->v_head | x->out_token | x->out_head | x->page | x->head | x->slot;
+    a.vec = aligned16(x->q) && aligned16(x->k) && aligned16(x->v) && aligned16(x->q_out) && aligned16(x->k_pages) && aligned16(x->v_pages) && strides % 8 == 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    switch (in_type * 3 + out_type) {
+    switch (x->in_type * 3 + x->out_type) {
         case 0: return rope_launch<__nv_bfloat16, __nv_bfloat16>(a, st);
         case 4: return rope_launch<__half, __half>(a, st);
         case 6: return rope_launch<float, __nv_bfloat16>(a, st);

@@ -7,18 +7,21 @@ requests.  The rows that ``beam_select`` returns go to ``ops.paged.fork_pages`` 
 
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 
-from .lib import check_status, load as lib, longs, on_device, ptr, same_cuda_device
-from .rope import TYPES
+from .lib import address, check_status, load as lib, on_device, same_cuda_device
+from .rope import F32, I32, TYPES
 
 MAX_K = 64
 MAX_BEAMS = 256
 MAX_VOCAB = 1 << 24
-_TENSORS = 16      # tensors of one launch of the reorder kernel
+_TENSORS = 16                                   # of one launch of the reorder kernel
+_BEAM = struct.Struct("Q8P6q8i")                # NexrtBeamArgs
+_REORDER = struct.Struct("Q2P2q4i32P48q")       # NexrtReorderArgs
+_BOOL = torch.bool
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, finished: Optional[torch.Tensor] = None, eos: int = -1,
@@ -32,28 +35,31 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, finished:
     ``eos`` at its own score.  Where fewer than ``k`` candidates are above -inf the rest are at -inf.  A beam with a NaN or +inf among its
     logits, or as its score, has no candidate and latches ``NON_FINITE`` in ``status``."""
     what = "beam_select"
-    if logits.dim() != 3 or logits.dtype not in TYPES or (logits.shape[2] > 1 and logits.stride(2) != 1):
+    shape, l_s, kind = logits.shape, logits.stride(), logits.dtype
+    if len(shape) != 3 or kind not in TYPES or (shape[2] > 1 and l_s[2] != 1):
         raise ValueError(f"{what}: logits is [requests, beams, vocabulary] in bf16, fp16 or fp32 with a contiguous last dimension")
-    batch, beams, vocab = logits.shape
+    batch, beams, vocab = shape
     if not 1 <= beams <= MAX_BEAMS or not 1 <= vocab <= MAX_VOCAB or batch * beams > 65535:
         raise ValueError(f"{what}: at most {MAX_BEAMS} beams, 65535 in all, and a vocabulary of {MAX_VOCAB}")
     if not 1 <= k <= min(MAX_K, beams * vocab):
         raise ValueError(f"{what}: k is between 1 and {MAX_K} and no more than there are candidates")
-    if scores.dtype != torch.float32 or scores.shape != (batch, beams):
+    if scores.dtype is not F32 or scores.shape != (batch, beams):
         raise ValueError(f"{what}: scores is fp32 [requests, beams]")
-    if finished is not None and (finished.dtype != torch.bool or finished.shape != (batch, beams) or not 0 <= eos < vocab):
-        raise ValueError(f"{what}: finished is bool [requests, beams], with an end token of the vocabulary")
+    s_s, f_s = scores.stride(), (0, 0)
+    if finished is not None:
+        if finished.dtype is not _BOOL or finished.shape != (batch, beams) or not 0 <= eos < vocab:
+            raise ValueError(f"{what}: finished is bool [requests, beams], with an end token of the vocabulary")
+        f_s = finished.stride()
     check_status(what, status)
     device = same_cuda_device(what, logits, scores, finished, status)
-    best = scores.new_empty((batch, k))
-    rows, tokens = scores.new_empty((batch, k), dtype=torch.int32), scores.new_empty((batch, k), dtype=torch.int32)
+    best, rows, tokens = scores.new_empty(batch, k), scores.new_empty(batch, k, dtype=I32), scores.new_empty(batch, k, dtype=I32)
     if batch:
         L = lib()
-        scratch = scores.new_empty(batch * beams * L.nexrt_beam_slices(batch * beams, vocab, TYPES[logits.dtype]) * (k + 2), dtype=torch.int64)
-        strides = longs(*logits.stride()[:2], *scores.stride(), *(finished.stride() if finished is not None else (0, 0)))
-        on_device(device, lambda st: L.nexrt_beam_select(
-            logits.data_ptr(), scores.data_ptr(), ptr(finished), strides, best.data_ptr(), rows.data_ptr(), tokens.data_ptr(), scratch.data_ptr(), ptr(status), batch, beams,
-            vocab, k, eos, TYPES[logits.dtype], st), what)
+        slices = L.nexrt_beam_slices(batch * beams, vocab, TYPES[kind])
+        scratch = scores.new_empty(batch * beams * slices * (k + 2), dtype=torch.int64)
+        on_device(device, L.nexrt_beam_select, _BEAM.pack(
+            _BEAM.size, logits.data_ptr(), scores.data_ptr(), address(finished), best.data_ptr(), rows.data_ptr(), tokens.data_ptr(), scratch.data_ptr(), address(status),
+            l_s[0], l_s[1], s_s[0], s_s[1], f_s[0], f_s[1], batch, beams, vocab, k, eos, TYPES[kind], slices, 0), what)
     return best, rows, tokens
 
 
@@ -62,8 +68,10 @@ def _rows_of(what: str, t: torch.Tensor, n: int) -> Tuple[int, int, int]:
     shape = t.shape
     if len(shape) == 0 or shape[0] != n or not (t.is_contiguous() or n == 0 or t[0].is_contiguous()):
         raise ValueError(f"{what}: every tensor has {n} rows, each of them dense")
+    if n == 0:
+        return 0, 0, 0
     size = t.element_size()
-    return t.data_ptr(), t.stride()[0] * size, t.numel() // n * size if n else 0
+    return t.data_ptr(), t.stride()[0] * size, t.numel() // n * size
 
 
 def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Optional[Sequence[torch.Tensor]] = None, status: Optional[torch.Tensor] = None) -> List[torch.Tensor]:
@@ -71,7 +79,8 @@ def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Op
     one- or two-dimensional (the columns of ``beam_select``'s that go on), and may name a row several times.  ``out`` must not share
     memory with ``tensors``: keep two sets and change places.  A row that does not exist is left as it was and latches ``BAD_PAGE``."""
     what = "reorder_rows"
-    if rows.dtype != torch.int32 or rows.dim() not in (1, 2):
+    r_shape, r_s = rows.shape, rows.stride()
+    if rows.dtype is not I32 or len(r_shape) not in (1, 2):
         raise ValueError(f"{what}: rows is int32 with one or two dimensions")
     n = rows.numel()
     if not tensors:
@@ -86,7 +95,7 @@ def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Op
     for t, o in zip(tensors, out):
         src, src_row, size = _rows_of(what, t, n_in)
         dst, dst_row, out_size = _rows_of(what, o, n)
-        if o.dtype != t.dtype or o.shape[1:] != t.shape[1:]:
+        if o.dtype is not t.dtype or o.shape[1:] != t.shape[1:]:
             raise ValueError(f"{what}: out has the tensors' types and rows")
         if out_size:
             moves.append((src, dst, src_row, dst_row, out_size))
@@ -97,11 +106,12 @@ def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Op
         if first < ends[1 - side]:
             raise ValueError(f"{what}: out shares memory with the tensors")
         ends[side] = max(ends[side], end)
-    cols = max(1, rows.shape[1]) if rows.dim() == 2 else 1
-    r0, r1 = rows.stride() if rows.dim() == 2 else (rows.stride()[0], 0)
+    cols, r0, r1 = (max(1, r_shape[1]), r_s[0], r_s[1]) if len(r_shape) == 2 else (1, r_s[0], 0)
     for i in range(0, len(moves), _TENSORS):
         part = moves[i : i + _TENSORS]
-        pointers = ctypes.c_void_p * len(part)
-        ins, outs, meta = pointers(*[m[0] for m in part]), pointers(*[m[1] for m in part]), longs(*[x for m in part for x in m[2:]])
-        on_device(device, lambda st: lib().nexrt_reorder_rows(ins, outs, meta, len(part), rows.data_ptr(), r0, r1, cols, n, n_in, ptr(status), st), what)
+        none = [0] * (_TENSORS - len(part))
+        columns = []
+        for column in zip(*part):
+            columns += [*column, *none]
+        on_device(device, lib().nexrt_reorder_rows, _REORDER.pack(_REORDER.size, rows.data_ptr(), address(status), r0, r1, cols, n, n_in, len(part), *columns), what)
     return list(out)

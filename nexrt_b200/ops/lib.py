@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_float, c_int, c_int64, c_size_t, c_uint, c_ulonglong, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_uint, c_ulonglong, c_void_p
 from typing import Optional
 
 import torch
@@ -38,7 +38,6 @@ class LLChannelStruct(ctypes.Structure):
 
 
 CH = POINTER(LLChannelStruct)
-I64 = POINTER(c_int64)
 
 _PROTOTYPES = {
     "nexrt_set_pdl": [ci],
@@ -111,16 +110,16 @@ _PROTOTYPES = {
     "nexrt_attn_front_tail": [vp] * 6 + [ci] * 7 + [vp],
     "nexrt_tc_moe_l1": [vp] * 7 + [ci] * 6 + [cf, ci, vp, vp],
     "nexrt_tc_moe_l2_allreduce": [vp] * 8 + [ci] * 6 + [CH, cu, vp, vp],
-    "nexrt_rope_append": [vp] * 13 + [I64] + [ci] * 12 + [cf, cf, vp],
-    "nexrt_paged_ctas": [ci] * 6,
-    "nexrt_paged_attn": [vp] * 10 + [I64] + [ci] * 9 + [cf, cf, ci, vp],
+    "nexrt_rope_append": [c_char_p, vp],
+    "nexrt_paged_attn": [c_char_p, vp],
+    "nexrt_paged_item_cost": [],
     "nexrt_paged_split": [vp, ci, ci, c_int64, ci, ci, vp, ci],
-    "nexrt_page_fork": [vp] + [ci] * 5 + [vp, c_int64, ci, ci, vp, vp, vp, ci, vp, c_int64, vp, vp, vp, vp, ci, vp],
-    "nexrt_page_compact": [vp] + [ci] * 5 + [vp, c_int64, ci, ci, vp, vp, c_int64] + [vp] * 6,
-    "nexrt_page_copy": [vp] + [ci] * 5 + [vp, vp, ci, vp, vp, vp],
+    "nexrt_page_fork": [c_char_p, vp],
+    "nexrt_page_compact": [c_char_p, vp],
+    "nexrt_page_copy": [c_char_p, vp],
     "nexrt_beam_slices": [ci, ci, ci],
-    "nexrt_beam_select": [vp] * 3 + [I64] + [vp] * 5 + [ci] * 6 + [vp],
-    "nexrt_reorder_rows": [vp, vp, I64, ci, vp, c_int64, c_int64, ci, ci, ci, vp, vp],
+    "nexrt_beam_select": [c_char_p, vp],
+    "nexrt_reorder_rows": [c_char_p, vp],
     "nexrt_ipc_alloc": [c_size_t, POINTER(c_void_p)],
     "nexrt_ipc_get_handle": [vp, vp],
     "nexrt_ipc_open": [vp, POINTER(c_void_p)],
@@ -200,20 +199,31 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-def longs(*values: int):
-    """An ``int64_t[]`` argument."""
-    return (c_int64 * len(values))(*values)
-
-
-def on_device(device: int, call, what: str) -> None:
-    """``call(stream)`` on the current stream of CUDA device ``device``, with that device current: the operators' tensors may lie on another one."""
+def on_device(device: int, fn, block: bytes, what: str) -> None:
+    """``fn(block, stream)`` on the current stream of CUDA device ``device``, with that device current: the operators' tensors may lie
+    on another one.  ``block``: the entry point's arguments as csrc/api.h declares them (one packed block costs 0.7 us a call, 28
+    arguments by themselves 4.5)."""
     if device == torch.cuda.current_device():
-        err = call(torch._C._cuda_getCurrentRawStream(device))     # 0.1 us; torch.cuda.current_stream makes a Stream object, 2.2 us
+        err = fn(block, torch._C._cuda_getCurrentRawStream(device))     # 0.1 us; torch.cuda.current_stream makes a Stream object, 2.2 us
     else:
         with torch.cuda.device(device):
-            err = call(torch._C._cuda_getCurrentRawStream(device))
+            err = fn(block, torch._C._cuda_getCurrentRawStream(device))
     if err:
         check(err, what)
+
+
+def address(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+_SMS = {}
+
+
+def sm_count(device: int) -> int:
+    n = _SMS.get(device)
+    if n is None:
+        n = _SMS[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return n
 
 
 def same_cuda_device(what: str, *tensors: Optional[torch.Tensor]) -> int:

@@ -13,16 +13,22 @@ finds wrong (a page that does not exist, a full pool) is left out and latched in
 from __future__ import annotations
 
 import math
+import struct
 from typing import Optional, Tuple, Union
 
 import torch
 
 from ..runtime.control import Status
-from .lib import KernelError, check_status, load as lib, longs, on_device, ptr, same_cuda_device
-from .rope import TYPES, rope_append
+from .lib import KernelError, address, check_status, load as lib, on_device, same_cuda_device, sm_count
+from .rope import F32, I32, TYPES, rope_append
 
 HEAD_DIMS = (64, 128, 192, 256)
 MAX_ROWS = 4096
+_CHUNK = 64                                     # keys of a unit of the attention's work, and what an item counts beside them
+_ITEM_COST = 3
+_ATTN = struct.Struct("Q10P9q10i2f")            # NexrtPagedAttnArgs
+_PAGES = struct.Struct("Q12P2q10i")             # NexrtPagesArgs
+_POOL_TYPES = (torch.bfloat16, torch.float16)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, scale: Optional[float] = None,
@@ -38,11 +44,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     logarithm of the sum of exp of the scores.  Keys on a page that the table does not name count as masked and latch ``BAD_PAGE``."""
     what = "paged_attention"
     kind, shape, q_s = q.dtype, q.shape, q.stride()
-    if len(shape) != 3 or kind not in (torch.bfloat16, torch.float16) or q_s[2] != 1:
+    if len(shape) != 3 or kind not in _POOL_TYPES or q_s[2] != 1:
         raise ValueError(f"{what}: q is [rows, heads, dim] in bf16 or fp16 with a contiguous last dimension")
     rows, heads, dim = shape
     pool, pool_s = k_pages.shape, k_pages.stride()
-    if len(pool) != 4 or pool != v_pages.shape or pool_s != v_pages.stride() or pool_s[3] != 1 or k_pages.dtype != kind or v_pages.dtype != kind:
+    if len(pool) != 4 or pool != v_pages.shape or pool_s != v_pages.stride() or pool_s[3] != 1 or k_pages.dtype is not kind or v_pages.dtype is not kind:
         raise ValueError(f"{what}: k_pages and v_pages are [pages, kv heads, slots, dim] of q's type, with the same strides and a contiguous last dimension")
     pages, kv_heads, slots, pool_dim = pool
     if dim not in HEAD_DIMS or pool_dim != dim:
@@ -52,52 +58,58 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     k_ptr, v_ptr = k_pages.data_ptr(), v_pages.data_ptr()
     if (pool_s[0] | pool_s[1] | pool_s[2]) % 8 or (k_ptr | v_ptr) % 16:
         raise ValueError(f"{what}: rows of the pages start on 16-byte boundaries")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != rows or table.stride()[1] != 1:
+    if pages * pool_s[0] + slots * pool_s[2] > 2**35 - 8:
+        raise ValueError(f"{what}: one layer's keys or values take less than 64 GB")
+    t_shape, t_s = table.shape, table.stride()
+    if table.dtype is not I32 or len(t_shape) != 2 or t_shape[0] != rows or t_s[1] != 1:
         raise ValueError(f"{what}: table is int32 [rows, pages of a row] with contiguous rows")
-    if lens.dtype != torch.int32 or lens.shape != (rows,) or not lens.is_contiguous():
+    if lens.dtype is not I32 or lens.shape != (rows,) or not lens.is_contiguous():
         raise ValueError(f"{what}: lens is int32 [rows]")
-    if not (softcap >= 0.0 and math.isfinite(softcap)) or window < 0:
+    if not 0.0 <= softcap < math.inf or window < 0:
         raise ValueError(f"{what}: softcap and window are not negative")
-    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous()):
+    if slopes is not None and (slopes.dtype is not F32 or slopes.shape != (heads,) or not slopes.is_contiguous()):
         raise ValueError(f"{what}: slopes is fp32 [heads]")
     check_status(what, status)
     if out is None:
-        out = q.new_empty(shape)
-    elif out.shape != shape or out.dtype != kind or out.stride()[2] != 1:
-        raise ValueError(f"{what}: out is like q")
-    lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
+        out, o_s = q.new_empty(rows, heads, dim), (heads * dim, dim)
+    else:
+        o_s = out.stride()
+        if out.shape != shape or out.dtype is not kind or o_s[2] != 1:
+            raise ValueError(f"{what}: out is like q")
+    lse = q.new_empty(rows, heads, dtype=F32) if return_lse else None
     device = same_cuda_device(what, q, k_pages, v_pages, table, lens, slopes, out, status)
     if rows:
-        L = lib()
-        width, o_s = table.shape[1], out.stride()
-        window = min(window, 2**31 - 1)
-        ctas = L.nexrt_paged_ctas(rows, heads, kv_heads, width, slots, window)
-        scratch = q.new_empty(ctas * (32 * (dim + 2) + 4), dtype=torch.float32)
-        strides = longs(q_s[0], q_s[1], o_s[0], o_s[1], pool_s[0], pool_s[1], pool_s[2], table.stride()[0], heads)
-        on_device(device, lambda st: L.nexrt_paged_attn(
-            q.data_ptr(), k_ptr, v_ptr, table.data_ptr(), lens.data_ptr(), ptr(slopes), out.data_ptr(), ptr(lse), scratch.data_ptr(), ptr(status), strides, rows, heads,
-            kv_heads, dim, width, slots, pages, window, TYPES[kind], dim**-0.5 if scale is None else scale, softcap, ctas, st), what)
+        # as many CTAs as are resident (two on an SM), no more than there can be units of work
+        width, window = t_shape[1], min(window, 2**31 - 1)
+        keys = min(width * slots, window + _CHUNK) if window else width * slots
+        ctas = min(2 * sm_count(device), 1024, (keys // _CHUNK + 1 + _ITEM_COST) * rows * kv_heads * -(-heads // (16 * kv_heads)))
+        scratch = q.new_empty(ctas * (32 * (dim + 2) + 4), dtype=F32)
+        on_device(device, lib().nexrt_paged_attn, _ATTN.pack(
+            _ATTN.size, q.data_ptr(), k_ptr, v_ptr, table.data_ptr(), lens.data_ptr(), address(slopes), out.data_ptr(), address(lse), scratch.data_ptr(), address(status),
+            q_s[0], q_s[1], o_s[0], o_s[1], pool_s[0], pool_s[1], pool_s[2], t_s[0], heads,
+            rows, heads, kv_heads, dim, width, slots, pages, window, TYPES[kind], ctas, dim**-0.5 if scale is None else scale, softcap), what)
     return (out, lse) if return_lse else out
 
 
 def _pool(what: str, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor):
-    """Arguments of the page kernels: base, planes, pages, heads, slots, bytes of a slot."""
+    """Base of the pool; planes, pages, heads, slots, bytes of a slot, rows and width of the table; its row stride."""
     shape = kv.shape
     if len(shape) != 6 or shape[1] != 2 or not kv.is_contiguous():
         raise ValueError(f"{what}: kv is a contiguous [layers, 2, pages, kv heads, slots, dim]")
     base, slot = kv.data_ptr(), shape[5] * kv.element_size()
     if shape[3] < 1 or shape[4] < 1 or slot < 16 or slot % 16 or base % 16:
         raise ValueError(f"{what}: a slot of the pool takes a multiple of 16 bytes and starts on such a boundary")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.stride()[1] != 1:
+    t_shape, t_s = table.shape, table.stride()
+    if table.dtype is not I32 or len(t_shape) != 2 or t_s[1] != 1:
         raise ValueError(f"{what}: table is int32 [rows, pages of a row] with contiguous rows")
-    if lens.dtype != torch.int32 or lens.shape != table.shape[:1] or not lens.is_contiguous():
+    if lens.dtype is not I32 or lens.shape != (t_shape[0],) or not lens.is_contiguous():
         raise ValueError(f"{what}: lens is int32 [rows]")
-    return base, 2 * shape[0], shape[2], shape[3], shape[4], slot
+    return base, (2 * shape[0], shape[2], shape[3], shape[4], slot, t_shape[0], t_shape[1]), t_s[0]
 
 
 def _fresh(what: str, name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor, *old: torch.Tensor) -> torch.Tensor:
     if t is None:
-        return like.new_empty(shape)
+        return like.new_empty(*shape)
     if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or (t.numel() and t.stride(-1) != 1) or (t.dim() == 1 and not t.is_contiguous()):
         raise ValueError(f"{what}: {name} is int32 {list(shape)} with contiguous rows")
     for o in old:
@@ -117,12 +129,12 @@ def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent
     which there is no page, or no column in the table, keeps its length and latches ``NO_PAGES``; a page or parent that does not
     exist latches ``BAD_PAGE``.  The outputs must not share memory with ``table`` or ``lens``."""
     what = "fork_pages"
-    pool = _pool(what, kv, table, lens)
-    if parents.dtype != torch.int32 or parents.dim() != 1 or not parents.is_contiguous() or parents.numel() > MAX_ROWS:
+    base, sizes, row = _pool(what, kv, table, lens)
+    n, width, pages = parents.numel(), sizes[6], sizes[1]
+    if parents.dtype is not I32 or parents.dim() != 1 or not parents.is_contiguous() or n > MAX_ROWS:
         raise ValueError(f"{what}: parents is int32 [rows], at most {MAX_ROWS}")
-    n, width, pages = parents.numel(), table.shape[1], kv.shape[2]
     each = grow if isinstance(grow, torch.Tensor) else None
-    if each is not None and (each.dtype != torch.int32 or each.shape != (n,) or not each.is_contiguous()):
+    if each is not None and (each.dtype is not I32 or each.shape != (n,) or not each.is_contiguous()):
         raise ValueError(f"{what}: grow is an int or int32 [rows]")
     if each is None and not 0 <= grow < 2**31:
         raise ValueError(f"{what}: grow is not negative")
@@ -132,9 +144,9 @@ def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent
     refs = _fresh(what, "refs", refs, (pages,), table, lens, parents, each, table)
     device = same_cuda_device(what, kv, table, lens, parents, each, table_out, lens_out, refs, status)
     scratch = table.new_empty(pages + 3 * n)
-    on_device(device, lambda st: lib().nexrt_page_fork(
-        *pool, table.data_ptr(), table.stride()[0], table.shape[0], width, lens.data_ptr(), parents.data_ptr(), ptr(each), 0 if each is not None else grow, table_out.data_ptr(),
-        table_out.stride()[0], lens_out.data_ptr(), refs.data_ptr(), scratch.data_ptr(), ptr(status), n, st), what)
+    on_device(device, lib().nexrt_page_fork, _PAGES.pack(
+        _PAGES.size, base, table.data_ptr(), lens.data_ptr(), parents.data_ptr(), address(each), table_out.data_ptr(), lens_out.data_ptr(), refs.data_ptr(), 0, 0,
+        scratch.data_ptr(), address(status), row, table_out.stride()[0], *sizes, n, 0 if each is not None else grow, 0), what)
     return table_out, lens_out, refs
 
 
@@ -144,17 +156,17 @@ def compact_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, 
     places go, in order, into the holes in front.  Returns ``(table, refs, remap, live)``: the renamed table, rows per page, new
     place of every page (-1: it was free) and ``live`` int32 ``[1]``.  What lies in the pool from ``live`` on is free."""
     what = "compact_pages"
-    pool = _pool(what, kv, table, lens)
-    pages = kv.shape[2]
+    base, sizes, row = _pool(what, kv, table, lens)
+    pages = sizes[1]
     check_status(what, status)
     table_out = _fresh(what, "table_out", table_out, tuple(table.shape), table, table)
     refs = _fresh(what, "refs", refs, (pages,), table, lens, table)
     remap, live = table.new_empty(pages), table.new_empty(1)
     device = same_cuda_device(what, kv, table, lens, table_out, refs, status)
     scratch = table.new_empty(5 * pages + 1)
-    on_device(device, lambda st: lib().nexrt_page_compact(
-        *pool, table.data_ptr(), table.stride()[0], table.shape[0], table.shape[1], lens.data_ptr(), table_out.data_ptr(), table_out.stride()[0], refs.data_ptr(),
-        remap.data_ptr(), live.data_ptr(), scratch.data_ptr(), ptr(status), st), what)
+    on_device(device, lib().nexrt_page_compact, _PAGES.pack(
+        _PAGES.size, base, table.data_ptr(), lens.data_ptr(), 0, 0, table_out.data_ptr(), 0, refs.data_ptr(), remap.data_ptr(), live.data_ptr(), scratch.data_ptr(),
+        address(status), row, table_out.stride()[0], *sizes, 0, 0, 0), what)
     return table_out, refs, remap, live
 
 
@@ -165,11 +177,11 @@ def copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *, status
     for t in (src, dst):
         if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() != src.numel():
             raise ValueError(f"{what}: src and dst are int32 lists of the same length")
-    pool = _pool(what, kv, src.view(-1, 1), src)
+    base, sizes, _ = _pool(what, kv, src.view(-1, 1), src)
     check_status(what, status)
     device = same_cuda_device(what, kv, src, dst, status)
     scratch = src.new_empty(3 * src.numel())
-    on_device(device, lambda st: lib().nexrt_page_copy(*pool, src.data_ptr(), dst.data_ptr(), src.numel(), scratch.data_ptr(), ptr(status), st), what)
+    on_device(device, lib().nexrt_page_copy, _PAGES.pack(_PAGES.size, base, src.data_ptr(), dst.data_ptr(), 0, 0, 0, 0, 0, 0, 0, scratch.data_ptr(), address(status), 1, 0, *sizes, 0, 0, 0), what)
 
 
 class PagedCache:

@@ -9,14 +9,17 @@ Pair ``i`` of a head at position ``p`` turns by ``p * inv_freq[i]``; ``scale`` m
 from __future__ import annotations
 
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
 
-from .lib import check_status, load as lib, longs, on_device, ptr, same_cuda_device
+from .lib import address, check_status, load as lib, on_device, same_cuda_device
 
+I32, F32 = torch.int32, torch.float32
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_DIM = 256
+_POOL_TYPES = (torch.bfloat16, torch.float16)
 
 
 def rope_frequencies(rotary: int, theta: float, scaling: Optional[str] = None, factor: float = 1.0, trained: int = 0, fast: float = 32.0,
@@ -48,48 +51,51 @@ def rope_frequencies(rotary: int, theta: float, scaling: Optional[str] = None, f
     return torch.tensor(inv, dtype=torch.float32), scale
 
 
-def _heads(what: str, x: torch.Tensor, tokens: int, dim: int, dtype: torch.dtype) -> Tuple[int, int, int]:
-    """(heads, stride of a token, stride of a head) of a tensor of heads."""
-    if x.dim() == 3 and x.dtype == dtype:
-        shape, strides = x.shape, x.stride()
-        if shape[0] == tokens and shape[2] == dim and strides[2] == 1:
-            return shape[1], strides[0], strides[1]
-    raise ValueError(f"{what}: tensors of heads are [tokens, heads, dim] of one type with a contiguous last dimension")
+_ARGS = struct.Struct("Q13P12q12i2f")      # NexrtRopeArgs
 
 
 def _common(what, q, positions, inv_freq, norms):
-    if q.dim() != 3 or q.dtype not in TYPES or q.stride()[2] != 1:
+    """(tokens, heads, dim, rotary, strides of q)."""
+    shape, strides = q.shape, q.stride()
+    if len(shape) != 3 or q.dtype not in TYPES or strides[2] != 1:
         raise ValueError(f"{what}: q is [tokens, heads, dim] in bf16, fp16 or fp32 with a contiguous last dimension")
-    tokens, _, dim = q.shape
+    tokens, heads, dim = shape
     if dim < 8 or dim > MAX_DIM or dim % 8:
         raise ValueError(f"{what}: head dimensions are multiples of 8 up to {MAX_DIM}, not {dim}")
-    if positions.dtype != torch.int32 or positions.shape != (tokens,) or not positions.is_contiguous():
+    if positions.dtype is not I32 or positions.shape != (tokens,) or not positions.is_contiguous():
         raise ValueError(f"{what}: positions is int32 [tokens]")
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or 2 * inv_freq.numel() > dim:
+    rotary = 2 * inv_freq.numel()
+    if inv_freq.dtype is not F32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or rotary > dim:
         raise ValueError(f"{what}: inv_freq is fp32 [rotary / 2] with rotary at most the head dimension")
     for w in norms:
-        if w is not None and (w.dtype != torch.float32 or w.shape != (dim,) or not w.is_contiguous()):
+        if w is not None and (w.dtype is not F32 or w.shape != (dim,) or not w.is_contiguous()):
             raise ValueError(f"{what}: norm multipliers are fp32 [dim]")
-    return tokens, dim, 2 * inv_freq.numel()
+    return tokens, heads, dim, rotary, strides
+
+
+def _out(what, out, q, tokens, heads, dim, kind):
+    """``out``, or a new one, and its strides."""
+    if out is None:
+        out = q.new_empty(tokens, heads, dim, dtype=kind)
+        return out, (heads * dim, dim)
+    strides = out.stride()
+    if out.shape != (tokens, heads, dim) or out.dtype is not kind or strides[2] != 1:
+        raise ValueError(f"{what}: out is [tokens, heads, dim] of {kind} with a contiguous last dimension")
+    return out, strides
 
 
 def rope(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0, norm: Optional[torch.Tensor] = None,
          eps: float = 1e-6, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``q [tokens, heads, dim]`` at ``positions`` int32 ``[tokens]``, rotated (after an RMSNorm with the multiplier ``norm``, if given); ``out`` may be ``q``."""
-    tokens, dim, rotary = _common("rope", q, positions, inv_freq, (norm,))
-    if out is None:
-        out = q.new_empty(q.shape)
-    hq, q_t, q_h = _heads("rope", q, tokens, dim, q.dtype)
-    ho, o_t, o_h = _heads("rope", out, tokens, dim, q.dtype)
-    if ho != hq:
-        raise ValueError("rope: out has other heads than q")
+    tokens, heads, dim, rotary, q_s = _common("rope", q, positions, inv_freq, (norm,))
+    out, o_s = _out("rope", out, q, tokens, heads, dim, q.dtype)
     device = same_cuda_device("rope", q, positions, inv_freq, norm, out)
-    if q.numel() == 0:
-        return out
-    strides = longs(q_t, q_h, 0, 0, 0, 0, o_t, o_h, 0, 0, 0, 0)
-    kind = TYPES[q.dtype]
-    on_device(device, lambda st: lib().nexrt_rope_append(q.data_ptr(), None, None, positions.data_ptr(), None, out.data_ptr(), None, None, None, inv_freq.data_ptr(), ptr(norm),
-                                                         None, None, strides, tokens, hq, 0, dim, rotary, interleaved, 0, 0, 1, 0, kind, kind, scale, eps, st), "rope")
+    if tokens and heads:
+        kind = TYPES[q.dtype]
+        on_device(device, lib().nexrt_rope_append, _ARGS.pack(
+            _ARGS.size, q.data_ptr(), 0, 0, positions.data_ptr(), 0, out.data_ptr(), 0, 0, 0, inv_freq.data_ptr(), address(norm), 0, 0,
+            q_s[0], q_s[1], 0, 0, 0, 0, o_s[0], o_s[1], 0, 0, 0, 0,
+            tokens, heads, 0, dim, rotary, interleaved, 0, 0, 1, 0, kind, kind, scale, eps), "rope")
     return out
 
 
@@ -103,37 +109,31 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     A negative ``rows[i]`` is padding: its q is rotated, nothing is stored.  A position whose page the table does not name is left out
     and latches ``BAD_PAGE`` in ``status``.  Two tokens of a call with the same slot leave it undefined."""
     what = "rope_append"
-    tokens, dim, rotary = _common(what, q, positions, inv_freq, (q_norm, k_norm))
+    tokens, hq, dim, rotary, q_s = _common(what, q, positions, inv_freq, (q_norm, k_norm))
     kind, pool_kind = q.dtype, k_pages.dtype
-    hq, q_t, q_h = _heads(what, q, tokens, dim, kind)
-    hk, k_t, k_h = _heads(what, k, tokens, dim, kind)
-    hv, v_t, v_h = _heads(what, v, tokens, dim, kind)
-    if hk != hv:
-        raise ValueError(f"{what}: k and v have the same heads")
-    if rows.dtype != torch.int32 or rows.shape != (tokens,) or not rows.is_contiguous():
+    k_shape, k_s, v_s = k.shape, k.stride(), v.stride()
+    if len(k_shape) != 3 or k_shape != v.shape or k_shape[0] != tokens or k_shape[2] != dim or k.dtype is not kind or v.dtype is not kind or k_s[2] != 1 or v_s[2] != 1:
+        raise ValueError(f"{what}: k and v are [tokens, kv heads, dim] like q, with contiguous last dimensions")
+    if rows.dtype is not I32 or rows.shape != (tokens,) or not rows.is_contiguous():
         raise ValueError(f"{what}: rows is int32 [tokens]")
     pool, pool_s = k_pages.shape, k_pages.stride()
-    if len(pool) != 4 or pool != v_pages.shape or pool_s != v_pages.stride() or v_pages.dtype != pool_kind or pool_s[3] != 1:
+    if len(pool) != 4 or pool != v_pages.shape or pool_s != v_pages.stride() or v_pages.dtype is not pool_kind or pool_s[3] != 1:
         raise ValueError(f"{what}: k_pages and v_pages are [pages, kv heads, slots, dim] with the same strides and a contiguous last dimension")
-    if pool[1] != hk or pool[3] != dim or pool[2] < 1:
+    pages, hk, slots, pool_dim = pool
+    if k_shape[1] != hk or pool_dim != dim or slots < 1:
         raise ValueError(f"{what}: the pages have other heads than k")
-    if pool_kind not in (torch.bfloat16, torch.float16) or kind not in (pool_kind, torch.float32):
+    if pool_kind not in _POOL_TYPES or (kind is not pool_kind and kind is not F32):
         raise ValueError(f"{what}: pages are bf16 or fp16, q, k and v the same or fp32")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.stride()[1] != 1:
+    t_shape, t_s = table.shape, table.stride()
+    if table.dtype is not I32 or len(t_shape) != 2 or t_s[1] != 1:
         raise ValueError(f"{what}: table is int32 [rows, pages of a row] with contiguous rows")
     check_status(what, status)
-    if out is None:
-        out = q.new_empty(q.shape, dtype=pool_kind)
-    ho, o_t, o_h = _heads(what, out, tokens, dim, pool_kind)
-    if ho != hq:
-        raise ValueError(f"{what}: out has other heads than q")
+    out, o_s = _out(what, out, q, tokens, hq, dim, pool_kind)
     device = same_cuda_device(what, q, k, v, positions, rows, k_pages, v_pages, table, inv_freq, q_norm, k_norm, out, status)
-    if tokens == 0:
-        return out
-    table_rows, width = table.shape
-    strides = longs(q_t, q_h, k_t, k_h, v_t, v_h, o_t, o_h, pool_s[0], pool_s[1], pool_s[2], table.stride()[0])
-    on_device(device, lambda st: lib().nexrt_rope_append(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), rows.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
-        inv_freq.data_ptr(), ptr(q_norm), ptr(k_norm), ptr(status), strides, tokens, hq, hk, dim, rotary, interleaved, table_rows, width, pool[2], pool[0], TYPES[kind],
-        TYPES[pool_kind], scale, eps, st), what)
+    if tokens:
+        on_device(device, lib().nexrt_rope_append, _ARGS.pack(
+            _ARGS.size, q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), rows.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+            table.data_ptr(), inv_freq.data_ptr(), address(q_norm), address(k_norm), address(status),
+            q_s[0], q_s[1], k_s[0], k_s[1], v_s[0], v_s[1], o_s[0], o_s[1], pool_s[0], pool_s[1], pool_s[2], t_s[0],
+            tokens, hq, hk, dim, rotary, interleaved, t_shape[0], t_shape[1], slots, pages, TYPES[kind], TYPES[pool_kind], scale, eps), what)
     return out

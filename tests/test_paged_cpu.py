@@ -160,6 +160,13 @@ def test_no_rows_no_launch():
     assert reorder_rows([], _i32(2)) == []
 
 
+def test_split_constants_match():
+    """What the caller sizes its launch by is what the kernel splits by."""
+    from nexrt_b200.ops import paged
+
+    assert L.load().nexrt_paged_item_cost() == paged._ITEM_COST
+
+
 def test_slot_of_a_position():
     """The device's page lookup, run on the host: entries that name no page of the pool, and places outside the table, give -1."""
     lib = L.load()
