@@ -228,11 +228,12 @@ typedef struct NexrtPagedAttnArgs {
     const void *q, *k_pages, *v_pages, *table, *lens, *slopes;
     void *out, *lse, *scratch, *status;               /* slopes, lse may be NULL; scratch: ctas times 32 (dim + 2) + 4 floats */
     int64_t q_row, q_head, out_row, out_head, page, head, slot, table_row, lse_row;
-    int rows, q_heads, kv_heads, dim, width, slots, pages, window, type, ctas;   /* ctas: at most nexrt_paged_ctas of the call */
+    int rows, q_heads, kv_heads, dim, width, slots, pages, window, type, ctas;   /* ctas: at most 1024 */
     float scale, softcap;
 } NexrtPagedAttnArgs;
 int nexrt_paged_attn(const NexrtPagedAttnArgs* args, void* stream);
 int nexrt_paged_item_cost(void);                      /* chunks of 64 keys that an item counts in the split beside its own */
+int nexrt_paged_resident(int dim);                    /* CTAs of the kernel on an SM */
 int64_t nexrt_paged_slot(const int* table, int64_t stride, int rows, int width, int page, int pages, int row, int pos);   /* host: slot of the pool that holds a position, or -1 */
 int nexrt_paged_split(const int* lens, int seqs, int items, int64_t room, int window, int grid, int64_t* out, int most);   /* host: how the keys are split over CTAs */
 

@@ -45,7 +45,9 @@ struct PagedAttnArgs {
     float scale, softcap;
 };
 
-template <int D> constexpr int ring_depth() { return D == 256 ? 3 : (D == 192 ? 4 : (D == 128 ? 6 : 8)); }
+// CTAs on an SM, and half tiles of a warp's ring: what registers and shared memory hold.
+constexpr int resident_ctas(int dim) { return dim == 64 ? 3 : 2; }
+template <int D> constexpr int ring_depth() { return D == 256 ? 3 : (D == 64 ? 6 : 4); }
 template <int D> constexpr int half_bytes() { return kTile * (D * 2 + 16); }
 template <int D> constexpr size_t ring_bytes() { return static_cast<size_t>(kPaWarps) * ring_depth<D>() * half_bytes<D>(); }
 template <int D> constexpr size_t merge_bytes() { return sizeof(float) * kPaWarps * kPaRows * (D + 4); }
@@ -172,7 +174,7 @@ __device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t phase, bool& lat
 }
 
 template <typename T, int D, int NTR, bool MODS>
-__global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(kPaThreads, resident_ctas(D)) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int KS = D / 16, R = ring_depth<D>(), PITCH = D * 2 + 16, HALF = half_bytes<D>(), CPR = D / 8;
     extern __shared__ __align__(128) unsigned char pa_smem[];
     uint4* const qf = reinterpret_cast<uint4*>(pa_smem);                           // query fragments, 512 bytes a k step
@@ -636,6 +638,7 @@ template <typename T> static int paged_dispatch(const PagedAttnArgs& a, int dim,
 using namespace nexrt;
 
 extern "C" int nexrt_paged_item_cost(void) { return kItemCost; }
+extern "C" int nexrt_paged_resident(int dim) { return resident_ctas(dim); }
 
 extern "C" int nexrt_paged_attn(const NexrtPagedAttnArgs* x, void* stream) {
     if (x->size != sizeof(*x)) return cudaErrorInvalidValue;

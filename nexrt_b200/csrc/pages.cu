@@ -15,6 +15,9 @@ namespace nexrt {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanRows = 4096;         // rows whose plan one CTA holds in shared memory
 constexpr int kPagesPerThread = 8;
+// Entries of a table that the planning CTA counts itself (8 rows of 130 entries: a fork 14.4 -> 9.6 us on the device; a CTA takes
+// about 1 us a thousand entries, a launch and a memset 5 us).
+constexpr int kSmallTable = 4096;
 
 // Sum of `v` over the threads before this one; `total` gets the sum over all.  red: 33 ints.
 __device__ __forceinline__ int block_prefix(int v, int* red, int& total) {
@@ -54,25 +57,36 @@ __device__ __forceinline__ int kept_len(const PageTable& t, const int* lens, int
     return n < 0 ? 0 : (n > room ? static_cast<int>(room) : n);
 }
 
-// new table[r] = old table[parents[r]] (-1 behind its last page), refs[page] = rows that name it.  refs comes in as zero.
+// new table[r] = old table[parents[r]] (-1 behind its last page), refs[page] += rows that name it; columns [j0, width) by steps of `step`.
+__device__ __forceinline__ void go_on(const PageTable& t, const int* lens, const int* parents, int* out, int64_t out_stride, int* refs, int r, int j0, int step, int* status) {
+    const int p = parents ? parents[r] : r;
+    if (j0 == 0 && (p >= t.rows || (p >= 0 && lens[p] > static_cast<int64_t>(t.width) * t.page))) latch(status, kStatusBadPage);
+    const int used = pages_of(kept_len(t, lens, p), t.page);
+    for (int j = j0; j < t.width; j += step) {
+        int page = -1;
+        if (j < used) {
+            page = page_at(t, p, j);
+            if (page < 0) latch(status, kStatusBadPage);
+            else atomicAdd(refs + page, 1);
+        }
+        if (out) out[r * out_stride + j] = page;
+    }
+}
+
+// A table of more than kSmallTable entries; refs comes in as zero.
 __global__ void __launch_bounds__(256) fork_rows_kernel(PageTable t, const int* lens, const int* parents, int* out, int64_t out_stride, int* refs, int n,
                                                         int* status) {
     pdl_launch_dependents();
     pdl_wait();
-    for (int r = blockIdx.y; r < n; r += gridDim.y) {
-        const int p = parents ? parents[r] : r;
-        if (threadIdx.x == 0 && blockIdx.x == 0 && (p >= t.rows || (p >= 0 && lens[p] > static_cast<int64_t>(t.width) * t.page))) latch(status, kStatusBadPage);
-        const int used = pages_of(kept_len(t, lens, p), t.page);
-        for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < t.width; j += gridDim.x * blockDim.x) {
-            int page = -1;
-            if (j < used) {
-                page = page_at(t, p, j);
-                if (page < 0) latch(status, kStatusBadPage);
-                else atomicAdd(refs + page, 1);
-            }
-            if (out) out[r * out_stride + j] = page;
-        }
-    }
+    for (int r = blockIdx.y; r < n; r += gridDim.y) go_on(t, lens, parents, out, out_stride, refs, r, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x, status);
+}
+
+// The same by the CTA that plans: a launch and a memset less where there is little to count.
+__device__ __forceinline__ void count_here(const PageTable& t, const int* lens, const int* parents, int* out, int64_t out_stride, int* refs, int n, int* status) {
+    for (int p = threadIdx.x; p < t.pages; p += blockDim.x) refs[p] = 0;
+    __syncthreads();
+    for (int r = threadIdx.x >> 5; r < n; r += blockDim.x >> 5) go_on(t, lens, parents, out, out_stride, refs, r, threadIdx.x & 31, 32, status);
+    __syncthreads();
 }
 
 struct ForkPlan {
@@ -85,6 +99,7 @@ struct ForkPlan {
     int* free_list;             // [pages] scratch
     int* status;
     int n, grow_all, pages;
+    int count;                  // the table has not been copied and counted yet
 };
 
 // One CTA.  A row with g more positions needs pages for them, and, if it goes on writing in a begun page that other rows hold
@@ -96,6 +111,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkPlan 
     __shared__ int red[33];
     pdl_launch_dependents();
     pdl_wait();
+    if (a.count) count_here(a.t, a.lens, a.parents, a.table, a.table_stride, a.refs, a.n, a.status);
     constexpr int kCopy = 1 << 30;
     for (int r = threadIdx.x; r < a.n; r += blockDim.x) {
         const int p = a.parents[r], len = kept_len(a.t, a.lens, p);
@@ -196,19 +212,24 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkPlan 
 }
 
 struct CompactPlan {
-    const int* refs;            // [pages] rows that name a page
+    PageTable t;
+    const int* lens;
+    int* refs;                  // [pages] rows that name a page
     int *refs_out, *remap;      // of the moved pages; new place of a page, -1: free
     int* copies;                // [pages][3]
     int* n_copies;
     int* live;
     int* holes;                 // [pages] scratch
     int pages;
+    int count;                  // the table has not been counted yet
+    int* status;
 };
 
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const CompactPlan a) {
     __shared__ int red[33];
     pdl_launch_dependents();
     pdl_wait();
+    if (a.count) count_here(a.t, a.lens, nullptr, nullptr, 0, a.refs, a.t.rows, a.status);
     constexpr int kStep = kPlanThreads * kPagesPerThread;
     int live = 0;
     for (int p0 = 0; p0 < a.pages; p0 += kStep) {
@@ -381,8 +402,11 @@ static bool pool_ok(const NexrtPagesArgs& x) {
            (reinterpret_cast<uintptr_t>(x.pool) & 15) == 0 && x.rows >= 0 && x.width >= 0;
 }
 
-// Counts the pages that rows name, and writes the rows that go on.
+static bool counts_here(const NexrtPagesArgs& x, int n) { return static_cast<int64_t>(n) * x.width <= kSmallTable && x.pages <= 16 * kSmallTable; }
+
+// Counts the pages that rows name, and writes the rows that go on, where the planning CTA does not.
 static int rows_launch(const NexrtPagesArgs& x, const PageTable& t, const int* parents, int* out, int* refs, int n, cudaStream_t st) {
+    if (counts_here(x, n) && n > 0) return 0;
     if (x.pages > 0)
         if (const cudaError_t e = cudaMemsetAsync(refs, 0, sizeof(int) * static_cast<size_t>(x.pages), st); e != cudaSuccess) return static_cast<int>(e);
     if (n == 0 || x.width == 0) return 0;
@@ -405,7 +429,7 @@ extern "C" int nexrt_page_fork(const NexrtPagesArgs* x, void* stream) {
     p.t = t; p.lens = static_cast<const int*>(x->lens); p.parents = static_cast<const int*>(x->parents); p.grow = static_cast<const int*>(x->grow);
     p.table = static_cast<int*>(x->table_out); p.table_stride = x->out_row; p.lens_out = static_cast<int*>(x->lens_out); p.refs = static_cast<int*>(x->refs);
     p.copies = static_cast<int*>(x->scratch) + x->pages; p.free_list = static_cast<int*>(x->scratch);
-    p.status = static_cast<int*>(x->status); p.n = x->rows_out; p.grow_all = x->grow_all; p.pages = x->pages;
+    p.status = static_cast<int*>(x->status); p.n = x->rows_out; p.grow_all = x->grow_all; p.pages = x->pages; p.count = counts_here(*x, x->rows_out);
     if (const int e = launch(fork_plan_kernel, dim3(1), dim3(kPlanThreads), sizeof(int) * 2 * x->rows_out, st, p)) return e;
     PageMove m = {};
     m.copies = p.copies; m.n = x->rows_out;
@@ -423,6 +447,7 @@ extern "C" int nexrt_page_compact(const NexrtPagesArgs* x, void* stream) {
     p.refs = refs; p.refs_out = static_cast<int*>(x->refs); p.remap = static_cast<int*>(x->remap);
     p.holes = refs + pages; p.copies = refs + 2 * pages; p.n_copies = refs + 5 * pages;
     p.live = static_cast<int*>(x->live); p.pages = x->pages;
+    p.t = t; p.lens = static_cast<const int*>(x->lens); p.count = x->rows > 0 && counts_here(*x, x->rows); p.status = static_cast<int*>(x->status);
     if (const int e = launch(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p)) return e;
     PageMove m = {};
     m.copies = p.copies; m.n_copies = p.n_copies; m.n = x->pages;

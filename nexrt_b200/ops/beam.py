@@ -63,15 +63,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, finished:
     return best, rows, tokens
 
 
-def _rows_of(what: str, t: torch.Tensor, n: int) -> Tuple[int, int, int]:
-    """(address, bytes between rows, bytes of a row) of a tensor of ``n`` dense rows."""
-    shape = t.shape
-    if len(shape) == 0 or shape[0] != n or not (t.is_contiguous() or n == 0 or t[0].is_contiguous()):
-        raise ValueError(f"{what}: every tensor has {n} rows, each of them dense")
-    if n == 0:
-        return 0, 0, 0
-    size = t.element_size()
-    return t.data_ptr(), t.stride()[0] * size, t.numel() // n * size
+def _row_stride(what: str, t: torch.Tensor, size: int) -> int:
+    """Bytes between the rows of a tensor whose rows are ``size`` bytes each."""
+    if t.is_contiguous():
+        return size
+    if not t[0].is_contiguous():
+        raise ValueError(f"{what}: rows are dense")
+    return t.stride()[0] * t.element_size()
 
 
 def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Optional[Sequence[torch.Tensor]] = None, status: Optional[torch.Tensor] = None) -> List[torch.Tensor]:
@@ -93,13 +91,15 @@ def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Op
     check_status(what, status)
     moves, spans = [], []
     for t, o in zip(tensors, out):
-        src, src_row, size = _rows_of(what, t, n_in)
-        dst, dst_row, out_size = _rows_of(what, o, n)
-        if o.dtype is not t.dtype or o.shape[1:] != t.shape[1:]:
-            raise ValueError(f"{what}: out has the tensors' types and rows")
-        if out_size:
-            moves.append((src, dst, src_row, dst_row, out_size))
-            spans += ((dst, dst + (n - 1) * dst_row + out_size, 1), (src, src + max(n_in - 1, 0) * src_row + size, 0))
+        t_shape, o_shape = t.shape, o.shape
+        if len(t_shape) == 0 or len(o_shape) == 0 or t_shape[0] != n_in or o_shape[0] != n or t_shape[1:] != o_shape[1:] or o.dtype is not t.dtype:
+            raise ValueError(f"{what}: tensors have the same number of rows, and out the same rows of the same types")
+        values = o.numel()
+        if values:
+            size = values // n * o.element_size()
+            src, dst, src_row, dst_row = t.data_ptr(), o.data_ptr(), _row_stride(what, t, size) if n_in else size, _row_stride(what, o, size)
+            moves.append((src, dst, src_row, dst_row, size))
+            spans += ((dst, dst + (n - 1) * dst_row + size, 1), (src, src + (n_in - 1) * src_row + size, 0))
     device = same_cuda_device(what, *tensors, *out, rows, status)
     ends = [0, 0]
     for first, end, side in sorted(spans):

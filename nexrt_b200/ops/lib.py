@@ -113,6 +113,7 @@ _PROTOTYPES = {
     "nexrt_rope_append": [c_char_p, vp],
     "nexrt_paged_attn": [c_char_p, vp],
     "nexrt_paged_item_cost": [],
+    "nexrt_paged_resident": [ci],
     "nexrt_paged_split": [vp, ci, ci, c_int64, ci, ci, vp, ci],
     "nexrt_page_fork": [c_char_p, vp],
     "nexrt_page_compact": [c_char_p, vp],

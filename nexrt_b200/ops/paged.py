@@ -31,6 +31,11 @@ _PAGES = struct.Struct("Q12P2q10i")             # NexrtPagesArgs
 _POOL_TYPES = (torch.bfloat16, torch.float16)
 
 
+def _resident(dim: int) -> int:
+    """CTAs of the attention kernel on an SM."""
+    return 3 if dim == 64 else 2
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, scale: Optional[float] = None,
                     softcap: float = 0.0, window: int = 0, slopes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, return_lse: bool = False,
                     status: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
@@ -79,10 +84,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     lse = q.new_empty(rows, heads, dtype=F32) if return_lse else None
     device = same_cuda_device(what, q, k_pages, v_pages, table, lens, slopes, out, status)
     if rows:
-        # as many CTAs as are resident (two on an SM), no more than there can be units of work
+        # as many CTAs as are resident, no more than there can be units of work
         width, window = t_shape[1], min(window, 2**31 - 1)
         keys = min(width * slots, window + _CHUNK) if window else width * slots
-        ctas = min(2 * sm_count(device), 1024, (keys // _CHUNK + 1 + _ITEM_COST) * rows * kv_heads * -(-heads // (16 * kv_heads)))
+        ctas = min(_resident(dim) * sm_count(device), 1024, (keys // _CHUNK + 1 + _ITEM_COST) * rows * kv_heads * -(-heads // (16 * kv_heads)))
         scratch = q.new_empty(ctas * (32 * (dim + 2) + 4), dtype=F32)
         on_device(device, lib().nexrt_paged_attn, _ATTN.pack(
             _ATTN.size, q.data_ptr(), k_ptr, v_ptr, table.data_ptr(), lens.data_ptr(), address(slopes), out.data_ptr(), address(lse), scratch.data_ptr(), address(status),

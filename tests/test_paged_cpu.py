@@ -165,6 +165,7 @@ def test_split_constants_match():
     from nexrt_b200.ops import paged
 
     assert L.load().nexrt_paged_item_cost() == paged._ITEM_COST
+    assert all(L.load().nexrt_paged_resident(d) == paged._resident(d) for d in paged.HEAD_DIMS)
 
 
 def test_slot_of_a_position():
