@@ -25,7 +25,8 @@ constexpr int kPieces = 4;                  // 16-byte pieces of a thread and st
 constexpr int kStepBytes = kSliceThreads * kPieces * 16;
 constexpr int kBeamGroups = 128;            // at most
 constexpr int kBeamKeep = 1024;             // values that are ranked by counting; more (ties) take the search below
-constexpr int kJoinThreads = 1024;
+constexpr int kJoinThreads = 512;
+constexpr int kJoinHold = 4;               // candidates of a thread that it keeps in registers
 constexpr int kBeamMaxWidth = 256;          // beams of a request
 constexpr int kBeamMaxVocab = 1 << 24;      // (beam, logit, token) in one 64-bit word
 
@@ -80,6 +81,23 @@ template <typename T> struct Piece {
         else return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w[i / 2] >> 16 : w[i / 2])));
     }
     __device__ __forceinline__ void operator=(const uint4& v) { w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+    // Bit i: value i >= bound, a value of the same type (16-bit types are compared two at a time).
+    __device__ __forceinline__ uint32_t at_least(float bound) const {
+        uint32_t bits = 0;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bits |= static_cast<uint32_t>(value(i) >= bound) << i;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t m;
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) m = __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), __float2bfloat162_rn(bound));
+                else m = __hge2_mask(*reinterpret_cast<const __half2*>(&w[i]), __float2half2_rn(bound));
+                bits |= ((m & 1u) | (m >> 15 & 2u)) << (2 * i);
+            }
+        }
+        return bits;
+    }
     __device__ __forceinline__ float top() const {
         if constexpr (sizeof(T) == 4) {
             return fmaxf(fmaxf(value(0), value(1)), fmaxf(value(2), value(3)));
@@ -206,16 +224,12 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (piece_top[j] >= bound) {
-                uint32_t there = 0;
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) there |= static_cast<uint32_t>(x[j].value(i) >= bound) << i;
                 const int first = (p0 + j * kSliceThreads + static_cast<int>(threadIdx.x)) * VEC - off, end = min(a.vocab, hi * VEC - off);
-                for (; there; there &= there - 1) {
-                    const int i = __ffs(there) - 1, token = first + i;
+#pragma unroll 1
+                for (uint32_t there = x[j].at_least(bound); there; there &= there - 1) {
+                    const int token = first + __ffs(there) - 1;
                     if (token < 0 || token >= end) continue;
-                    float v = x[j].value(0);
-#pragma unroll
-                    for (int n = 1; n < VEC; ++n) v = n == i ? x[j].value(n) : v;
+                    const float v = static_cast<float>(base[token]);
                     const int to = atomicAdd(&count_s, 1);
                     if (to < kBeamKeep) keep[to] = (static_cast<u64>(ord32(v)) << 32) | static_cast<unsigned int>(~token);
                 }
@@ -314,31 +328,45 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
 
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamArgs a) {
     __shared__ double lse[kBeamMaxWidth];           // of a live beam
+    __shared__ float score_s[kBeamMaxWidth];
     __shared__ int kind[kBeamMaxWidth];             // 0 live, 1 finished, 2 closed without a candidate above -infinity
-    __shared__ u64 group_top[kJoinThreads / 8], keep[kBeamKeep], keep_tie[kBeamKeep];
+    __shared__ u64 group_top[kJoinThreads / 4], keep[kBeamKeep], keep_tie[kBeamKeep];
     __shared__ u64 bound_s;
     __shared__ int count_s, red[32];
     pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.beams, S = a.slices, k = a.k;
+    const int per = S * k, total_n = W * per;
+    const u64* const keys = a.keys + static_cast<int64_t>(b) * total_n;
+    // the first candidates are on their way while the beams' sums are made (what belongs to a closed beam was not written and is not used)
+    u64 raw[kJoinHold];
+#pragma unroll
+    for (int i = 0; i < kJoinHold; ++i) {
+        const int n = i * kJoinThreads + threadIdx.x;
+        raw[i] = n < total_n ? keys[n] : 0;
+    }
     for (int w = warp; w < W; w += kJoinThreads / 32) {
+        const int64_t at = (static_cast<int64_t>(b) * W + w) * S;
+        const float score = a.scores[b * a.s_b + w * a.s_w];
+        const bool done = a.finished && a.finished[b * a.f_b + w * a.f_w];
+        float ms = lane < S ? a.tops[at + lane] : -INFINITY;
+        double part = lane < S ? a.sums[at + lane] : 0.0;
         int what = 0;
         double value = 0.0;
-        if (a.finished && a.finished[b * a.f_b + w * a.f_w]) {
-            what = 1;
-            if (!(a.scores[b * a.s_b + w * a.s_w] < INFINITY)) what = 2;
-        } else if (beam_is_closed(a, b, w)) {
-            what = 2;
+        if (done || !(score > -INFINITY && score < INFINITY)) {
+            what = done && score < INFINITY ? 1 : 2;
+            if (lane == 0 && a.status && (score != score || score == INFINITY)) atomicCAS(a.status, 0, static_cast<int>(kStatusNonFinite));
         } else {
-            const int64_t at = (static_cast<int64_t>(b) * W + w) * S;
-            float m = -INFINITY;
-            for (int s = lane; s < S; s += 32) m = fmaxf(m, a.tops[at + s]);
+            float m = ms;
+            for (int s = lane + 32; s < S; s += 32) m = fmaxf(m, a.tops[at + s]);
             m = warp_max(m);
             double sum = 0.0;
             for (int s = lane; s < S; s += 32) {
-                const float ms = a.tops[at + s];
-                const double part = a.sums[at + s];
-                sum += ms == m ? part : part * exp(static_cast<double>(ms) - static_cast<double>(m));
+                if (s != lane) {
+                    ms = a.tops[at + s];
+                    part = a.sums[at + s];
+                }
+                sum += ms == m ? part : part * static_cast<double>(exp2_down((ms - m) * 1.4426950408889634f));
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -351,12 +379,9 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamArgs 
                 if (lane == 0 && a.status) atomicCAS(a.status, 0, static_cast<int>(kStatusNonFinite));
             }
         }
-        if (what == 2 && lane == 0 && a.status) {
-            const float s = a.scores[b * a.s_b + w * a.s_w];
-            if (s != s || s == INFINITY) atomicCAS(a.status, 0, static_cast<int>(kStatusNonFinite));
-        }
         if (lane == 0) {
             lse[w] = value;
+            score_s[w] = score;
             kind[w] = what;
         }
     }
@@ -364,13 +389,11 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamArgs 
     __syncthreads();
 
     // candidate n of the request: its total in order (0: none), and the word that orders equal totals
-    const int per = S * k, total_n = W * per;
-    auto candidate = [&](int n, u64& tie) -> u64 {
+    auto candidate = [&](int n, u64 key, u64& tie) -> u64 {
         const int w = n / per, i = n - w * per;
         const u64 beam = static_cast<u64>(kBeamMaxWidth - 1 - w) << 56;
-        const double score = a.scores[b * a.s_b + w * a.s_w];
+        const double score = score_s[w];
         if (kind[w] == 0) {
-            const u64 key = a.keys[(static_cast<int64_t>(b) * W + w) * per + i];
             if (key == 0) return 0;
             const unsigned int logit = static_cast<unsigned int>(key >> 32), token = ~static_cast<unsigned int>(key);
             tie = beam | (static_cast<u64>(logit) << 24) | (kBeamMaxVocab - 1 - token);
@@ -384,44 +407,53 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamArgs 
         tie = beam | (kBeamMaxVocab - 1 - token);
         return ord64(kind[w] == 1 && i == 0 ? score : -INFINITY);
     };
+    auto reload = [&](int n, u64& tie) { return candidate(n, keys[n], tie); };
 
-    u64 top = 0, tie = 0;
-    for (int n = threadIdx.x; n < total_n; n += kJoinThreads) {
-        const u64 key = candidate(n, tie);
+    u64 held[kJoinHold], held_tie[kJoinHold], top = 0, tie = 0;
+#pragma unroll
+    for (int i = 0; i < kJoinHold; ++i) {
+        const int n = i * kJoinThreads + threadIdx.x;
+        held_tie[i] = 0;
+        held[i] = n < total_n ? candidate(n, raw[i], held_tie[i]) : 0;
+        top = held[i] > top ? held[i] : top;
+    }
+    for (int n = kJoinHold * kJoinThreads + threadIdx.x; n < total_n; n += kJoinThreads) {
+        const u64 key = reload(n, tie);
         top = key > top ? key : top;
     }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
+    for (int o = 1; o < 4; o <<= 1) {
         const u64 other = __shfl_xor_sync(0xffffffffu, top, o);
         top = other > top ? other : top;
     }
-    if ((lane & 7) == 0) group_top[threadIdx.x >> 3] = top;
+    if ((lane & 3) == 0) group_top[threadIdx.x >> 2] = top;
+    if (threadIdx.x == 0) bound_s = ~0ull;
     __syncthreads();
     {
-        const int mine_i = threadIdx.x >> 3;                       // eight threads a group
-        const u64 mine = group_top[mine_i];
-        int rank = 0;
-#pragma unroll
-        for (int i = 0; i < kJoinThreads / 64; ++i) {
-            const int other = 8 * i + (lane & 7);
-            const u64 g = group_top[other];
-            rank += g > mine || (g == mine && other < mine_i);
-        }
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-        if ((lane & 7) == 0 && rank == k - 1) bound_s = mine;
+        // the k-th largest of the groups' maxima: four threads a group
+        int above = 0;
+#pragma unroll 8
+        for (int i = threadIdx.x & 3; i < kJoinThreads / 4; i += 4) above += group_top[i] > top;
+        above += __shfl_xor_sync(0xffffffffu, above, 1);
+        above += __shfl_xor_sync(0xffffffffu, above, 2);
+        if ((lane & 3) == 0 && above < k) atomicMin(&bound_s, top);
     }
     __syncthreads();
     const u64 bound = bound_s;
-    for (int n = threadIdx.x; n < total_n; n += kJoinThreads) {
-        const u64 key = candidate(n, tie);
+    auto collect = [&](u64 key, u64 key_tie) {
         if (key != 0 && key >= bound) {
             const int at = atomicAdd(&count_s, 1);
             if (at < kBeamKeep) {
                 keep[at] = key;
-                keep_tie[at] = tie;
+                keep_tie[at] = key_tie;
             }
         }
+    };
+#pragma unroll
+    for (int i = 0; i < kJoinHold; ++i) collect(held[i], held_tie[i]);
+    for (int n = kJoinHold * kJoinThreads + threadIdx.x; n < total_n; n += kJoinThreads) {
+        const u64 key = reload(n, tie);
+        collect(key, tie);
     }
     __syncthreads();
     int count = count_s;
@@ -431,23 +463,23 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamArgs 
         for (int bit = 63; bit >= 0; --bit) {
             const u64 next = edge | (1ull << bit);
             int n = 0;
-            for (int i = threadIdx.x; i < total_n; i += kJoinThreads) n += candidate(i, tie) >= next;
+            for (int i = threadIdx.x; i < total_n; i += kJoinThreads) n += reload(i, tie) >= next;
             if (cta_sum(n, red) >= k) edge = next;
         }
         int above = 0;
-        for (int i = threadIdx.x; i < total_n; i += kJoinThreads) above += candidate(i, tie) > edge;
+        for (int i = threadIdx.x; i < total_n; i += kJoinThreads) above += reload(i, tie) > edge;
         above = cta_sum(above, red);
         for (int bit = 63; bit >= 0; --bit) {
             const u64 next = edge_tie | (1ull << bit);
             int n = 0;
-            for (int i = threadIdx.x; i < total_n; i += kJoinThreads) n += candidate(i, tie) == edge && tie >= next;
+            for (int i = threadIdx.x; i < total_n; i += kJoinThreads) n += reload(i, tie) == edge && tie >= next;
             if (above + cta_sum(n, red) >= k) edge_tie = next;
         }
         __syncthreads();
         if (threadIdx.x == 0) count_s = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < total_n; i += kJoinThreads) {
-            const u64 key = candidate(i, tie);
+            const u64 key = reload(i, tie);
             if (key != 0 && (key > edge || (key == edge && tie >= edge_tie))) {
                 const int at = atomicAdd(&count_s, 1);
                 if (at < kBeamKeep) {
