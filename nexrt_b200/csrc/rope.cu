@@ -92,7 +92,7 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float2 
 }
 
 constexpr int kRopeThreads = 128;
-constexpr int kRopeResident = 6;        // CTAs on an SM
+constexpr int kRopeResident = 4;        // CTAs on an SM
 constexpr int kRopeWarps = kRopeThreads / 32;
 
 // How a value meets the other one of its pair: (2 i, 2 i + 1) are in one lane; the rotated dims lie in the first halves of the lanes'
