@@ -10,7 +10,7 @@
 // registers as they came, the next step's loads in flight.  The k largest: the k-th largest of 64 or 128 maxima of the first step bounds them from below, the few values
 // at or above it are collected and at the end ranked by counting (equal values in masses are found by bisection instead).  A second
 // kernel, one CTA a request, joins the slices.  Bound by the logits' bytes, and for one request by the two launches.  Measured: 117 live
-// rows of 248320 bf16 logits (58 MB) 35 us, 18 instructions a value on schedulers that are 63 % busy; four rows of fp32 11 us.
+// rows of 248320 bf16 logits (58 MB) 33 us, 16 instructions a value; four rows of fp32 11 us.
 #include <type_traits>
 
 #include "api.h"
@@ -82,6 +82,9 @@ template <typename T> struct Piece {
         else return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w[i / 2] >> 16 : w[i / 2])));
     }
     __device__ __forceinline__ void operator=(const uint4& v) { w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+    __device__ __forceinline__ void clear() {          // to -infinity
+        w[0] = w[1] = w[2] = w[3] = sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __nv_bfloat16>::value ? 0xff80ff80u : 0xfc00fc00u);
+    }
     // Bit i: value i >= bound, a value of the same type (16-bit types are compared two at a time).
     __device__ __forceinline__ uint32_t at_least(float bound) const {
         uint32_t bits = 0;
@@ -154,7 +157,11 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
     // the row in 16-byte pieces: piece c holds values [c VEC - off, (c + 1) VEC - off)
     const int off = static_cast<int>(reinterpret_cast<uintptr_t>(base) / sizeof(T) % VEC);
     const int pieces = (a.vocab + off + VEC - 1) / VEC;
-    const int lo = static_cast<int>(static_cast<int64_t>(pieces) * slice / a.slices), hi = static_cast<int>(static_cast<int64_t>(pieces) * (slice + 1) / a.slices);
+    // a slice is whole steps: only a row's last one is ragged
+    const int steps = (pieces + kSliceThreads * NV - 1) / (kSliceThreads * NV);
+    const unsigned int slices = a.slices;                              // (no more than there are steps, at most 4097: 32 bits will do)
+    const int lo = static_cast<int>(static_cast<unsigned int>(steps * slice) / slices) * kSliceThreads * NV;
+    const int hi = min(pieces, static_cast<int>(static_cast<unsigned int>(steps * (slice + 1)) / slices) * kSliceThreads * NV);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t at_slice = static_cast<int64_t>(row) * a.slices + slice;
     u64* out = a.keys + at_slice * a.k;
@@ -177,7 +184,8 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
         for (int j = 0; j < NV; ++j) {
             const int c = p0 + j * kSliceThreads + threadIdx.x, at = c * VEC - off;
             if (c < hi && at >= 0 && at + VEC <= a.vocab) ahead[j] = ld_stream16(base + at);
-            else ahead[j] = edge_piece(base, at, c < hi ? a.vocab : 0);
+            else if (c < hi) ahead[j] = edge_piece(base, at, a.vocab);
+            else ahead[j].clear();
         }
     };
     fetch(lo);
@@ -207,18 +215,18 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
         top = new_top;
         if (p0 == lo) {
             // the k-th largest maximum of 64 groups of lanes (of 128 for many beams) bounds the k-th largest value of the slice from below
-            const int lanes = a.k > 16 ? 2 : 4, groups = kSliceThreads / lanes, mine_i = threadIdx.x / lanes;
+            const int wide = a.k > 16 ? 1 : 2, lanes = 1 << wide, groups = kSliceThreads >> wide, part = threadIdx.x & (lanes - 1);
             float group = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             if (lanes == 4) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, 2));
-            if (threadIdx.x % lanes == 0) group_top[mine_i] = group;
+            if (part == 0) group_top[threadIdx.x >> wide] = group;
             if (threadIdx.x == 0) bound_s = 0xffffffffu;
             __syncthreads();
             int above = 0;
 #pragma unroll 16
-            for (int i = threadIdx.x % lanes; i < groups; i += lanes) above += group_top[i] > group;
+            for (int i = part; i < groups; i += lanes) above += group_top[i] > group;
             above += __shfl_xor_sync(0xffffffffu, above, 1);
             if (lanes == 4) above += __shfl_xor_sync(0xffffffffu, above, 2);
-            if (threadIdx.x % lanes == 0 && above < a.k) atomicMin(&bound_s, ord32(group));
+            if (part == 0 && above < a.k) atomicMin(&bound_s, ord32(group));
             __syncthreads();
             bound = unord32(bound_s);
         }

@@ -232,3 +232,55 @@ def test_beam_search_over_a_paged_cache():
             cache.compact()
     cache.check()
     assert len({tuple(b[1]) for b in beams}) == W
+
+
+def test_a_captured_beam_step_goes_on_like_an_eager_one():
+    """Fork, append, attend, select and reorder as one graph, replayed, against the same step called eagerly on a second cache; a row of the batch is padding."""
+    W, hq, hk, dim, V, page = 4, 6, 2, 128, 700, 8
+    g = torch.Generator(device=DEV).manual_seed(3)
+    embed, wq, wo = (torch.randn(*n, device=DEV, generator=g) * 0.1 for n in ((V, 64), (64, (hq + 2 * hk) * dim), (hq * dim, V)))
+    inv = rope_frequencies(dim, 1e4)[0].to(DEV)
+
+    class Run:
+        def __init__(self):
+            self.cache = PagedCache(1, 60, hk, page, dim, W + 1, 96)
+            self.parents, self.tokens = ints([0, 0, 0, 0, -1]), torch.full((W,), 5, device=DEV)
+            self.scores = torch.tensor([[0.0, -math.inf, -math.inf, -math.inf]], device=DEV)
+            self.state, self.other = torch.zeros(W, 33, device=DEV), torch.zeros(W, 33, device=DEV)
+
+        def step(self):
+            c = self.cache
+            c.fork(self.parents, 1)
+            x = torch.zeros(W + 1, 64, device=DEV)
+            x[:W] = embed[self.tokens]
+            h = (x @ wq).view(W + 1, -1, dim)
+            rows = torch.where(c.lens > 0, c.same, -1)                         # the last row is empty: nothing is stored for it
+            q = c.append(0, h[:, :hq], h[:, hq : hq + hk], h[:, hq + hk :], c.lens - 1, rows, inv)
+            y = c.attend(0, q, softcap=20.0).float()
+            assert y.shape == (W + 1, hq, dim)
+            s, r, t = beam_select((y[:W].flatten(1) @ wo)[None], self.scores, W)
+            reorder_rows([self.state], r, out=[self.other])
+            self.state.copy_(self.other)
+            self.state[:, 0] += t[0].float()
+            self.scores.copy_(s)
+            self.tokens.copy_(t[0])
+            self.parents[:W].copy_(r[0])
+
+    a, b = Run(), Run()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        a.step()
+    torch.cuda.current_stream().wait_stream(st)
+    graph = torch.cuda.CUDAGraph()
+    with graph_capture(graph, st):
+        a.step()
+    b.step()
+    for _ in range(20):
+        graph.replay()
+        b.step()
+        for x, y in ((a.cache.table, b.cache.table), (a.cache.lens, b.cache.lens), (a.cache.refs, b.cache.refs), (a.scores, b.scores), (a.tokens, b.tokens), (a.state, b.state)):
+            assert torch.equal(x, y)
+    a.cache.check()
+    b.cache.check()
+    assert a.cache.lens.tolist() == [21] * W + [0] and torch.equal(a.cache.kv, b.cache.kv)

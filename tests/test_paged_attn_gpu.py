@@ -219,3 +219,19 @@ def test_captured_graphs_follow_their_inputs():
         side = paged_attention(q, kv[0], kv[1], table, lens)
     st.synchronize()
     assert torch.equal(side, paged_attention(q, kv[0], kv[1], table, lens))
+
+
+def test_two_streams_at_once():
+    """Calls that overlap have scratch of their own."""
+    cases = [build([9000, 3, 700], 16, 2, 256, 32, torch.bfloat16, seed=i) for i in range(2)]
+    want = [paged_attention(q, kv[0], kv[1], table, lens) for q, kv, table, lens in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                q, kv, table, lens = cases[i]
+                got[i].append(paged_attention(q, kv[0], kv[1], table, lens))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
