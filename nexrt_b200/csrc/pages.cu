@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkPlan 
         const int used = pages_of(len, a.t.page);
         int want = 0, open = -1;
         if (g > 0) {
-            if (static_cast<int64_t>(len) + g > static_cast<int64_t>(a.t.width) * a.t.page) {
+            const int64_t room = static_cast<int64_t>(a.t.width) * a.t.page;
+            if (static_cast<int64_t>(len) + g > (room < INT32_MAX ? room : INT32_MAX)) {
                 latch(a.status, kStatusNoPages);
                 g = 0;
             } else if (len % a.t.page) {

@@ -127,10 +127,10 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const
     // ---- this warp's steps, of all tokens' (kHeads heads of one token each)
     const int64_t total = static_cast<int64_t>(a.tokens) * steps;
     const int n = gridDim.x * kRopeWarps, w_id = blockIdx.x * kRopeWarps + warp;
-    const int64_t begin = total * w_id / n;
-    int left = static_cast<int>(total * (w_id + 1) / n - begin), ahead = left;
+    const int64_t begin = range_begin(total, w_id, n);
+    int left = static_cast<int>(range_begin(total, w_id + 1, n) - begin), ahead = left;
     if (left == 0) return;
-    int t = static_cast<int>(begin / steps), i = static_cast<int>(begin - static_cast<int64_t>(t) * steps);
+    int t = static_cast<int>(quotient(begin, steps)), i = static_cast<int>(begin - static_cast<int64_t>(t) * steps);
 
     uint4 (*const ring)[2 * kWide][32] = ring_s[kVec ? warp : 0];
     int ft = t, fi = i;                                  // the step that is fetched next
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int j = 0; j < kWide; ++j)
-                    cp16(static_cast<uint32_t>(__cvta_generic_to_shared(&ring[at][c * kWide + j][lane])), src + (e0 + c * kFar < a.dim ? c * kFar + j * 4 : 0), e0 + c * kFar < a.dim);
+                    cp16(static_cast<uint32_t>(__cvta_generic_to_shared(&ring[at][c * kWide + j][lane])), e0 + c * kFar < a.dim ? src + c * kFar + j * 4 : src - e0, e0 + c * kFar < a.dim);
         }
         cp_commit();
         --ahead;

@@ -130,6 +130,16 @@ def test_fork_reports_and_survives_bad_input():
     assert run([[0, 1, 2, 3, 4, 5], [-1] * 6], [24, 0], [0, 1], ints([0, 1]))[1:] == ([24, 0], [1] * 6, Status.NO_PAGES)   # the pool is full
 
 
+def test_a_length_that_32_bits_do_not_hold_is_refused():
+    """A table with room for more positions than an int32 counts."""
+    kv = torch.zeros(1, 2, 3, 1, 65536, 16, dtype=torch.int8, device=DEV)
+    table, status = torch.zeros(1, 40000, dtype=torch.int32, device=DEV), ints([0])
+    t, l, refs = fork_pages(kv, table, ints([2**31 - 65536]), ints([0]), 65535, status=status)
+    assert l.tolist() == [2**31 - 1] and int(status) == 0 and refs.tolist() == [32767, 1, 0]
+    t, l, refs = fork_pages(kv, table, ints([2**31 - 65536]), ints([0]), 65536, status=status)
+    assert l.tolist() == [2**31 - 65536] and int(status) == Status.NO_PAGES and refs.tolist() == [32767, 0, 0]
+
+
 @pytest.mark.parametrize("seed", range(16))
 def test_compact_is_its_statement(seed):
     r = random.Random(100 + seed)
