@@ -51,7 +51,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, finished:
             raise ValueError(f"{what}: finished is bool [requests, beams], with an end token of the vocabulary")
         f_s = finished.stride()
     check_status(what, status)
-    device = same_cuda_device(what, logits, scores, finished, status)
+    device = same_cuda_device(what, {logits.get_device(), scores.get_device()}, finished, status)
     best, rows, tokens = scores.new_empty(batch, k), scores.new_empty(batch, k, dtype=I32), scores.new_empty(batch, k, dtype=I32)
     if batch:
         L = lib()
@@ -63,10 +63,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, finished:
     return best, rows, tokens
 
 
-def _row_stride(what: str, t: torch.Tensor, size: int) -> int:
-    """Bytes between the rows of a tensor whose rows are ``size`` bytes each."""
-    if t.is_contiguous():
-        return size
+def _row_stride(what: str, t: torch.Tensor) -> int:
+    """Bytes between the rows of a tensor that is not contiguous, but whose rows are."""
     if not t[0].is_contiguous():
         raise ValueError(f"{what}: rows are dense")
     return t.stride()[0] * t.element_size()
@@ -92,20 +90,27 @@ def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Op
     moves, spans = [], []
     for t, o in zip(tensors, out):
         t_shape, o_shape = t.shape, o.shape
-        if len(t_shape) == 0 or len(o_shape) == 0 or t_shape[0] != n_in or o_shape[0] != n or t_shape[1:] != o_shape[1:] or o.dtype is not t.dtype:
+        if len(t_shape) == 0 or len(o_shape) == 0 or t_shape[0] != n_in or o_shape[0] != n or (t_shape != o_shape and t_shape[1:] != o_shape[1:]) or o.dtype is not t.dtype:
             raise ValueError(f"{what}: tensors have the same number of rows, and out the same rows of the same types")
         values = o.numel()
         if values:
             size = values // n * o.element_size()
-            src, dst, src_row, dst_row = t.data_ptr(), o.data_ptr(), _row_stride(what, t, size) if n_in else size, _row_stride(what, o, size)
+            src, dst, src_row, dst_row = t.data_ptr(), o.data_ptr(), size, size
+            if not o.is_contiguous():
+                dst_row = _row_stride(what, o)
+            if n_in and not t.is_contiguous():
+                src_row = _row_stride(what, t)
             moves.append((src, dst, src_row, dst_row, size))
-            spans += ((dst, dst + (n - 1) * dst_row + size, 1), (src, src + (n_in - 1) * src_row + size, 0))
-    device = same_cuda_device(what, *tensors, *out, rows, status)
+            spans.append((dst, dst + (n - 1) * dst_row + size, 1))
+            spans.append((src, src + (n_in - 1) * src_row + size, 0))
+    device = same_cuda_device(what, {rows.get_device()}, *tensors, *out, status)
     ends = [0, 0]
-    for first, end, side in sorted(spans):
+    spans.sort()
+    for first, end, side in spans:
         if first < ends[1 - side]:
             raise ValueError(f"{what}: out shares memory with the tensors")
-        ends[side] = max(ends[side], end)
+        if end > ends[side]:
+            ends[side] = end
     cols, r0, r1 = (max(1, r_shape[1]), r_s[0], r_s[1]) if len(r_shape) == 2 else (1, r_s[0], 0)
     for i in range(0, len(moves), _TENSORS):
         part = moves[i : i + _TENSORS]

@@ -204,7 +204,7 @@ def on_device(device: int, fn, block: bytes, what: str) -> None:
     """``fn(block, stream)`` on the current stream of CUDA device ``device``, with that device current: the operators' tensors may lie
     on another one.  ``block``: the entry point's arguments as csrc/api.h declares them (one packed block costs 0.7 us a call, 28
     arguments by themselves 4.5)."""
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():
         err = fn(block, torch._C._cuda_getCurrentRawStream(device))     # 0.1 us; torch.cuda.current_stream makes a Stream object, 2.2 us
     else:
         with torch.cuda.device(device):
@@ -227,14 +227,17 @@ def sm_count(device: int) -> int:
     return n
 
 
-def same_cuda_device(what: str, *tensors: Optional[torch.Tensor]) -> int:
-    """Index of the CUDA device that all the tensors given lie on; a ``ValueError`` where there is none."""
-    device = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != device:
-            raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
+def same_cuda_device(what: str, devices: set, *optional: Optional[torch.Tensor]) -> int:
+    """Index of the one CUDA device in ``devices`` (the ``get_device()`` of an operator's tensors; those in ``optional`` may be ``None``); a
+    ``ValueError`` where there are several or none."""
+    for t in optional:
+        if t is not None:
+            devices.add(t.get_device())
+    if len(devices) != 1:
+        raise ValueError(f"{what}: tensors on several devices ({sorted(devices)}, -1 is the CPU)")
+    device = devices.pop()
     if device < 0:
-        raise ValueError(f"{what} runs on a CUDA device, the tensors are on {tensors[0].device}")
+        raise ValueError(f"{what} runs on a CUDA device, the tensors are on the CPU")
     return device
 
 

@@ -82,7 +82,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if out.shape != shape or out.dtype is not kind or o_s[2] != 1:
             raise ValueError(f"{what}: out is like q")
     lse = q.new_empty(rows, heads, dtype=F32) if return_lse else None
-    device = same_cuda_device(what, q, k_pages, v_pages, table, lens, slopes, out, status)
+    device = same_cuda_device(what, {q.get_device(), k_pages.get_device(), v_pages.get_device(), table.get_device(), lens.get_device(), out.get_device()}, slopes, status)
     if rows:
         # as many CTAs as are resident, no more than there can be units of work
         width, window = t_shape[1], min(window, 2**31 - 1)
@@ -114,7 +114,7 @@ def _pool(what: str, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor):
 
 def _fresh(what: str, name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor, *old: torch.Tensor) -> torch.Tensor:
     if t is None:
-        return like.new_empty(*shape)
+        return like.new_empty(*shape)        # (ints cost half of what a tuple does)
     if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or (t.numel() and t.stride(-1) != 1) or (t.dim() == 1 and not t.is_contiguous()):
         raise ValueError(f"{what}: {name} is int32 {list(shape)} with contiguous rows")
     for o in old:
@@ -147,7 +147,8 @@ def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent
     table_out = _fresh(what, "table_out", table_out, (n, width), table, table)
     lens_out = _fresh(what, "lens_out", lens_out, (n,), table, lens, parents, each)
     refs = _fresh(what, "refs", refs, (pages,), table, lens, parents, each, table)
-    device = same_cuda_device(what, kv, table, lens, parents, each, table_out, lens_out, refs, status)
+    device = same_cuda_device(what, {kv.get_device(), table.get_device(), lens.get_device(), parents.get_device(), table_out.get_device(), lens_out.get_device(),
+                                     refs.get_device()}, each, status)
     scratch = table.new_empty(pages + 3 * n)
     on_device(device, lib().nexrt_page_fork, _PAGES.pack(
         _PAGES.size, base, table.data_ptr(), lens.data_ptr(), parents.data_ptr(), address(each), table_out.data_ptr(), lens_out.data_ptr(), refs.data_ptr(), 0, 0,
@@ -167,7 +168,7 @@ def compact_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, 
     table_out = _fresh(what, "table_out", table_out, tuple(table.shape), table, table)
     refs = _fresh(what, "refs", refs, (pages,), table, lens, table)
     remap, live = table.new_empty(pages), table.new_empty(1)
-    device = same_cuda_device(what, kv, table, lens, table_out, refs, status)
+    device = same_cuda_device(what, {kv.get_device(), table.get_device(), lens.get_device(), table_out.get_device(), refs.get_device()}, status)
     scratch = table.new_empty(5 * pages + 1)
     on_device(device, lib().nexrt_page_compact, _PAGES.pack(
         _PAGES.size, base, table.data_ptr(), lens.data_ptr(), 0, 0, table_out.data_ptr(), 0, refs.data_ptr(), remap.data_ptr(), live.data_ptr(), scratch.data_ptr(),
@@ -184,7 +185,7 @@ def copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *, status
             raise ValueError(f"{what}: src and dst are int32 lists of the same length")
     base, sizes, _ = _pool(what, kv, src.view(-1, 1), src)
     check_status(what, status)
-    device = same_cuda_device(what, kv, src, dst, status)
+    device = same_cuda_device(what, {kv.get_device(), src.get_device(), dst.get_device()}, status)
     scratch = src.new_empty(3 * src.numel())
     on_device(device, lib().nexrt_page_copy, _PAGES.pack(_PAGES.size, base, src.data_ptr(), dst.data_ptr(), 0, 0, 0, 0, 0, 0, 0, scratch.data_ptr(), address(status), 1, 0, *sizes, 0, 0, 0), what)
 

@@ -76,8 +76,7 @@ def _common(what, q, positions, inv_freq, norms):
 def _out(what, out, q, tokens, heads, dim, kind):
     """``out``, or a new one, and its strides."""
     if out is None:
-        out = q.new_empty(tokens, heads, dim, dtype=kind)
-        return out, (heads * dim, dim)
+        return q.new_empty(tokens, heads, dim) if q.dtype is kind else q.new_empty(tokens, heads, dim, dtype=kind), (heads * dim, dim)
     strides = out.stride()
     if out.shape != (tokens, heads, dim) or out.dtype is not kind or strides[2] != 1:
         raise ValueError(f"{what}: out is [tokens, heads, dim] of {kind} with a contiguous last dimension")
@@ -89,7 +88,7 @@ def rope(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, in
     """``q [tokens, heads, dim]`` at ``positions`` int32 ``[tokens]``, rotated (after an RMSNorm with the multiplier ``norm``, if given); ``out`` may be ``q``."""
     tokens, heads, dim, rotary, q_s = _common("rope", q, positions, inv_freq, (norm,))
     out, o_s = _out("rope", out, q, tokens, heads, dim, q.dtype)
-    device = same_cuda_device("rope", q, positions, inv_freq, norm, out)
+    device = same_cuda_device("rope", {q.get_device(), positions.get_device(), inv_freq.get_device(), out.get_device()}, norm)
     if tokens and heads:
         kind = TYPES[q.dtype]
         on_device(device, lib().nexrt_rope_append, _ARGS.pack(
@@ -129,7 +128,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
         raise ValueError(f"{what}: table is int32 [rows, pages of a row] with contiguous rows")
     check_status(what, status)
     out, o_s = _out(what, out, q, tokens, hq, dim, pool_kind)
-    device = same_cuda_device(what, q, k, v, positions, rows, k_pages, v_pages, table, inv_freq, q_norm, k_norm, out, status)
+    device = same_cuda_device(what, {q.get_device(), k.get_device(), v.get_device(), positions.get_device(), rows.get_device(), k_pages.get_device(), v_pages.get_device(),
+                                     table.get_device(), inv_freq.get_device(), out.get_device()}, q_norm, k_norm, status)
     if tokens:
         on_device(device, lib().nexrt_rope_append, _ARGS.pack(
             _ARGS.size, q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), rows.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
