@@ -10,7 +10,7 @@
 // registers as they came, the next step's loads in flight.  The k largest: the k-th largest of 64 or 128 maxima of the first step bounds them from below, the few values
 // at or above it are collected and at the end ranked by counting (equal values in masses are found by bisection instead).  A second
 // kernel, one CTA a request, joins the slices.  Bound by the logits' bytes, and for one request by the two launches.  Measured: 117 live
-// rows of 248320 bf16 logits (58 MB) 33 us, 16 instructions a value; four rows of fp32 11 us.
+// rows of 248320 bf16 logits (58 MB) 30 us, about 14 instructions a value; four rows of fp32 10 us.
 #include <type_traits>
 
 #include "api.h"
@@ -57,9 +57,9 @@ struct BeamArgs {
 
 // A beam with no candidates of its own vocabulary: finished, or with a score that nothing can follow.
 __device__ __forceinline__ bool beam_is_closed(const BeamArgs& a, int b, int w) {
-    if (a.finished && a.finished[b * a.f_b + w * a.f_w]) return true;
+    const bool done = a.finished && a.finished[b * a.f_b + w * a.f_w];
     const float s = a.scores[b * a.s_b + w * a.s_w];
-    return !(s > -INFINITY) || s == INFINITY;
+    return done || !(s > -INFINITY) || s == INFINITY;
 }
 
 // sum of an int over the CTA, for all threads; red: 32 ints
@@ -84,6 +84,16 @@ template <typename T> struct Piece {
     __device__ __forceinline__ void operator=(const uint4& v) { w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
     __device__ __forceinline__ void clear() {          // to -infinity
         w[0] = w[1] = w[2] = w[3] = sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __nv_bfloat16>::value ? 0xff80ff80u : 0xfc00fc00u);
+    }
+    // value(i) of an i that is not known when this is compiled
+    __device__ __forceinline__ float value_at(int i) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(i & 2 ? (i & 1 ? w[3] : w[2]) : (i & 1 ? w[1] : w[0]));
+        } else {
+            const uint32_t u = i & 4 ? (i & 2 ? w[3] : w[2]) : (i & 2 ? w[1] : w[0]);
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
+            else return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? u >> 16 : u)));
+        }
     }
     // Bit i: value i >= bound, a value of the same type (16-bit types are compared two at a time).
     __device__ __forceinline__ uint32_t at_least(float bound) const {
@@ -152,7 +162,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
     pdl_launch_dependents();
     pdl_wait();
     const int row = blockIdx.y, slice = blockIdx.x, b = row / a.beams, w = row - b * a.beams;
-    if (beam_is_closed(a, b, w)) return;
+    const bool closed = beam_is_closed(a, b, w);        // looked at when the first loads are on their way
     const T* base = static_cast<const T*>(a.logits) + b * a.l_b + w * a.l_w;
     // the row in 16-byte pieces: piece c holds values [c VEC - off, (c + 1) VEC - off)
     const int off = static_cast<int>(reinterpret_cast<uintptr_t>(base) / sizeof(T) % VEC);
@@ -189,6 +199,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
         }
     };
     fetch(lo);
+    if (closed) return;
     int step = 0;
     for (int p0 = lo; p0 < hi; p0 += kSliceThreads * NV, ++step) {
         Piece<T> x[NV];
@@ -236,9 +247,9 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
                 const int first = (p0 + j * kSliceThreads + static_cast<int>(threadIdx.x)) * VEC - off, end = min(a.vocab, hi * VEC - off);
 #pragma unroll 1
                 for (uint32_t there = x[j].at_least(bound); there; there &= there - 1) {
-                    const int token = first + __ffs(there) - 1;
+                    const int i = __ffs(there) - 1, token = first + i;
                     if (token < 0 || token >= end) continue;
-                    const float v = static_cast<float>(base[token]);
+                    const float v = x[j].value_at(i);
                     const int to = atomicAdd(&count_s, 1);
                     if (to < kBeamKeep) keep[to] = (static_cast<u64>(ord32(v)) << 32) | static_cast<unsigned int>(~token);
                 }
