@@ -134,26 +134,37 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const
 
     uint4 (*const ring)[2 * kWide][32] = ring_s[kVec ? warp : 0];
     int ft = t, fi = i;                                  // the step that is fetched next
-    auto source = [&](int t_, int h) -> const TI* {
+    auto source = [&](int64_t t_, int h) -> const TI* {
         if (h < a.q_heads) return static_cast<const TI*>(a.q) + t_ * a.q_t + static_cast<int64_t>(h) * a.q_h + e0;
         if (h < qk) return static_cast<const TI*>(a.k) + t_ * a.k_t + static_cast<int64_t>(h - a.q_heads) * a.k_h + e0;
         return static_cast<const TI*>(a.v) + t_ * a.v_t + static_cast<int64_t>(h - qk) * a.v_h + e0;
     };
+    // steps whose heads are all of q, the most there are, need no choice: a pointer runs along
+    const int q_steps = a.q_heads / kHeads;
+    const int64_t q_step = static_cast<int64_t>(kHeads) * a.q_h, out_step = static_cast<int64_t>(kHeads) * a.qo_h;
+    const TI* q_from = static_cast<const TI*>(a.q) + ft * a.q_t + static_cast<int64_t>(fi * kHeads + lane / LPH) * a.q_h + e0;
+    const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(&ring_s[kVec ? warp : 0][0][0][lane]));
+    const bool in0 = e0 < a.dim, in1 = e0 + kFar < a.dim;
+    const int far = in1 ? kFar : 0;
     auto fetch = [&](int at) {
         const int h = fi * kHeads + lane / LPH;
         if (ahead > 0 && h < heads) {
-            const TI* src = source(ft, h);
+            const TI* src = fi < q_steps ? q_from : source(ft, h);
+            if (!in0) src -= e0;                         // (a lane without dims copies nothing, from a valid place)
+            const uint32_t dst = ring_at + at * (2 * kWide * 512);
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int j = 0; j < kWide; ++j)
-                    cp16(static_cast<uint32_t>(__cvta_generic_to_shared(&ring[at][c * kWide + j][lane])), e0 + c * kFar < a.dim ? src + c * kFar + j * 4 : src - e0, e0 + c * kFar < a.dim);
+            for (int j = 0; j < kWide; ++j) {
+                cp16(dst + j * 512, src + (in0 ? j * 4 : 0), in0);
+                cp16(dst + (kWide + j) * 512, src + far + (in1 ? j * 4 : 0), in1);
+            }
         }
         cp_commit();
         --ahead;
+        q_from += q_step;
         if (++fi == steps) {
             fi = 0;
             ++ft;
+            q_from = static_cast<const TI*>(a.q) + ft * a.q_t + static_cast<int64_t>(lane / LPH) * a.q_h + e0;
         }
     };
     if (kVec) {
@@ -162,8 +173,10 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const
     }
 
     // ---- a token: its angles, and the entry of the table that its k and v need; the next one's position and row are on their way
+    TO* q_to = nullptr;                                  // head lane / LPH of the token's q
     int pos = 0, row = -1, entry = -1, next_pos = a.positions[t], next_row = a.paged ? a.rows[t] : -1;
     auto begin_token = [&]() {
+        q_to = static_cast<TO*>(a.q_out) + t * a.qo_t + static_cast<int64_t>(lane / LPH) * a.qo_h + e0;
         pos = next_pos;
         row = next_row;
         if (t + 1 < a.tokens) {
@@ -225,6 +238,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const
             kind = -1;
             begin_token();
         }
+        const bool all_q = i < q_steps;                  // the same for all lanes
         const int h = i++ * kHeads + lane / LPH;
         Eight<TI> raw[2];
         if (kVec) {
@@ -275,16 +289,16 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const
             float ss = sq.x + sq.y;
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if ((h < a.q_heads ? a.q_norm : a.k_norm) != nullptr) r = rsqrtf(fmaf(ss, inv_dim, a.eps));
+            if ((all_q || h < a.q_heads ? a.q_norm : a.k_norm) != nullptr) r = rsqrtf(fmaf(ss, inv_dim, a.eps));
         }
         if (kVec) {
             __syncwarp();
             fetch(at);                               // into the place that was just read
         }
-        if (h >= heads) continue;
-        if (h < qk) {
-            if (kind != (h < a.q_heads ? 0 : 1)) {
-                kind = h < a.q_heads ? 0 : 1;
+        if (!all_q && h >= heads) continue;
+        if (all_q || h < qk) {
+            if (kind != (all_q || h < a.q_heads ? 0 : 1)) {
+                kind = all_q || h < a.q_heads ? 0 : 1;
                 factors(kind ? a.k_norm : a.q_norm);
             }
             const float2 rr = make_float2(r, r);
@@ -319,8 +333,8 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const
             }
         }
         TO* dst;
-        if (h < a.q_heads) {
-            dst = static_cast<TO*>(a.q_out) + t * a.qo_t + static_cast<int64_t>(h) * a.qo_h + e0;
+        if (all_q || h < a.q_heads) {
+            dst = q_to + (i - 1) * out_step;
         } else {
             if (row < 0) continue;                   // padding: nothing is stored for it
             if (entry < 0 || entry >= a.table.pages) {
@@ -330,8 +344,8 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const
             dst = static_cast<TO*>(h < qk ? a.k_out : a.v_out) + entry * a.page_s + static_cast<int64_t>(pos % a.table.page) * a.slot_s +
                   static_cast<int64_t>(h < qk ? h - a.q_heads : h - qk) * a.head_s + e0;
         }
-        if (e0 < a.dim) store8(dst, x[0], vec);
-        if (e0 + kFar < a.dim) store8(dst + kFar, x[1], vec);
+        if (in0) store8(dst, x[0], vec);
+        if (in1) store8(dst + kFar, x[1], vec);
     }
 }
 
