@@ -15,18 +15,15 @@ struct PageTable {
     int pages;           // pages of the pool
 };
 
-// Entry `j` of a row's pages, or -1 where it names no page of the pool.
-__host__ __device__ __forceinline__ int page_at(const PageTable& t, int row, int j) {
-    if (row < 0 || row >= t.rows || j < 0 || j >= t.width) return -1;
-    const int p = t.table[row * t.stride + j];
-    return p >= 0 && p < t.pages ? p : -1;
+// Entry `j` of a row as the table has it, -1 outside the table.
+__host__ __device__ __forceinline__ int page_entry(const PageTable& t, int row, int j) {
+    return row < 0 || row >= t.rows || j < 0 || j >= t.width ? -1 : t.table[row * t.stride + j];
 }
 
-// Slot of the pool (page * slots + slot) that holds position `pos` of `row`, or -1.
-__host__ __device__ __forceinline__ int64_t page_slot(const PageTable& t, int row, int pos) {
-    if (pos < 0) return -1;
-    const int j = pos / t.page, p = page_at(t, row, j);
-    return p < 0 ? -1 : static_cast<int64_t>(p) * t.page + (pos - j * t.page);
+// The same, -1 also where it names no page of the pool.
+__host__ __device__ __forceinline__ int page_at(const PageTable& t, int row, int j) {
+    const int p = page_entry(t, row, j);
+    return p >= 0 && p < t.pages ? p : -1;
 }
 
 // Pages that `len` positions take.

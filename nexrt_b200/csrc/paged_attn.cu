@@ -677,7 +677,8 @@ extern "C" int nexrt_paged_attn(const NexrtPagedAttnArgs* x, void* stream) {
 
 // Host forms of the index arithmetic above, for tests without a GPU.
 extern "C" int64_t nexrt_paged_slot(const int* table, int64_t stride, int rows, int width, int page, int pages, int row, int pos) {
-    return page_slot({table, stride, rows, width, page, pages}, row, pos);
+    const int p = pos < 0 ? -1 : page_at({table, stride, rows, width, page, pages}, row, pos / page);
+    return p < 0 ? -1 : static_cast<int64_t>(p) * page + pos % page;
 }
 // out [parts][5]: CTA, sequence, item, first chunk, chunks - the walk of every CTA; returns the number of parts (at most `most` are written).
 extern "C" int nexrt_paged_split(const int* lens, int seqs, int items, int64_t room, int window, int grid, int64_t* out, int most) {

@@ -183,9 +183,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const
             next_pos = a.positions[t + 1];
             if (a.paged) next_row = a.rows[t + 1];
         }
-        const int j = pos / a.table.page;
-        const bool named = row >= 0 && row < a.table.rows && pos >= 0 && j < a.table.width;
-        entry = named ? a.table.table[row * a.table.stride + j] : -1;
+        entry = pos < 0 ? -1 : page_entry(a.table, row, pos / a.table.page);     // (checked where it is used: the load is not waited for here)
         __syncwarp();
         for (int p = lane; p < half; p += 32) {
             double turns = static_cast<double>(pos) * static_cast<double>(a.inv_freq[p]) * 0.15915494309189533577;
