@@ -21,7 +21,7 @@
 // batch's lengths cut an item).
 //
 // Measured: 200K keys, 2 key heads of 256, 32 query heads: 76 us, 5.4 TB/s of keys and values, 0.83 of copy rate (the rings alone fill in
-// 64); 48 sequences of 0 to 16384 keys, 8 heads of 128: 95 us, 0.84; one sequence of 1100 keys: 9.2 us, two launches and their chains.
+// 64); 48 sequences of 0 to 16384 keys, 8 heads of 128: 92 us, 0.87; one sequence of 1100 keys: 9.2 us, two launches and their chains.
 #include "api.h"
 #include "paged.cuh"
 
@@ -544,10 +544,9 @@ __global__ void __launch_bounds__(kPaThreads, resident_ctas(D)) paged_attn_kerne
 
 // One CTA per (cut, row): joins the parts of an item that was cut.  The parts' maxima and sums first, then their accumulators with
 // D / 4 lanes of four dims side by side and the parts shared out over the groups of lanes.
-constexpr int kJoinThreads = 512;
 constexpr int kMaxCtas = 1024;
 
-template <typename T, int D>
+template <typename T, int D, int kJoinThreads>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int LANES = D / 4, GROUPS = kJoinThreads / LANES;
     __shared__ float weight[kMaxCtas], top_s[kJoinThreads / 32], sum_s[kJoinThreads / 32];
@@ -626,8 +625,11 @@ template <typename T, int D> static int paged_launch(const PagedAttnArgs& a, boo
     if (a.group <= 8) e = mods ? launch(paged_attn_kernel<T, D, 1, true>, grid, block, smem, st, a) : launch(paged_attn_kernel<T, D, 1, false>, grid, block, smem, st, a);
     else e = mods ? launch(paged_attn_kernel<T, D, 2, true>, grid, block, smem, st, a) : launch(paged_attn_kernel<T, D, 2, false>, grid, block, smem, st, a);
     if (e || !join) return e;
-    const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads * a.head_groups;
-    return launch(paged_join_kernel<T, D>, dim3(a.by_item ? static_cast<unsigned>(items) : a.grid, a.group < kPaRows ? a.group : kPaRows), dim3(kJoinThreads), 0, st, a);
+    const int rows = a.group < kPaRows ? a.group : kPaRows, items = a.seqs * a.kv_heads * a.head_groups;
+    // items cut into dozens of parts are few and want many threads (200K keys in 148 parts: 75.5 us, with 256 threads 80.3), items cut once
+    // or twice are many and want many CTAs (a ragged batch 91.9, with 1024 threads where it may 95.0; 1100 keys 9.2 and 10.0)
+    if (a.by_item && a.grid >= 32 * items) return launch(paged_join_kernel<T, D, 1024>, dim3(items, rows), dim3(1024), 0, st, a);
+    return launch(paged_join_kernel<T, D, 256>, dim3(a.by_item ? items : a.grid, rows), dim3(256), 0, st, a);
 }
 
 template <typename T> static int paged_dispatch(const PagedAttnArgs& a, int dim, bool join, cudaStream_t st) {
