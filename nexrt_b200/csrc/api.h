@@ -245,7 +245,7 @@ typedef struct NexrtPagesArgs {
     int64_t table_row, out_row;
     int planes, pages, heads, slots, slot_bytes, rows, width, rows_out, grow_all, reserved;
 } NexrtPagesArgs;
-int nexrt_page_fork(const NexrtPagesArgs* args, void* stream);      /* scratch: int[pages + 3 rows_out] */
+int nexrt_page_fork(const NexrtPagesArgs* args, void* stream);      /* scratch: int[pages + 3 rows_out + 1] */
 int nexrt_page_compact(const NexrtPagesArgs* args, void* stream);   /* scratch: int[5 pages + 1] */
 int nexrt_page_copy(const NexrtPagesArgs* args, void* stream);      /* table: sources, lens: targets, rows of them; scratch: int[3 rows] */
 

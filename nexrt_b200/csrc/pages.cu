@@ -7,8 +7,8 @@
 // the table names; the lowest go first, to the rows in their order.
 //
 // Bound by the bytes of the copied pages; for a table without copies by the launches and the plan's few round trips.  Measured: 360
-// pages of 15 layers (708 MB both ways) compacted in 132 us, 0.83 of copy rate (the move itself 117); eight beams of 8191 keys
-// forked in 9.6 us, 128 of up to 20000 in 17.5.
+// pages of 15 layers (708 MB both ways) compacted in 124 us, 0.88 of copy rate; eight beams of 8191 keys forked in 9.8 us, 128 of up to
+// 20000 in 15.
 #include "api.h"
 #include "paged.cuh"
 
@@ -97,7 +97,8 @@ struct ForkPlan {
     int* table;                 // the new one, as fork_rows_kernel left it
     int64_t table_stride;
     int *lens_out, *refs;
-    int* copies;                // [n][3]: source page, target page, positions to copy (0: none)
+    int* copies;                // [n][3]: source page, target page, positions to copy
+    int* n_copies;
     int* free_list;             // [pages] scratch
     int* status;
     int n, grow_all, pages;
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkPlan 
         need += total;
     }
     int found = 0;
-    for (int p0 = 0; p0 < a.pages && found < need; p0 += kPlanThreads * kPagesPerThread) {
+    for (int p0 = 0; p0 < a.pages && found < need; p0 += blockDim.x * kPagesPerThread) {
         const int base = p0 + threadIdx.x * kPagesPerThread;
         int mask = 0;
 #pragma unroll
@@ -177,15 +178,14 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkPlan 
     }
     __syncthreads();
 
-    int before = 0;
+    int before = 0, copied = 0;
     for (int r0 = 0; r0 < a.n; r0 += blockDim.x) {
         const int r = r0 + threadIdx.x;
         const int f = r < a.n ? fresh[r] : 0, k = f & (kCopy - 1);
         int total;
         const int at = before + block_prefix(k, red, total);
         before += total;
-        if (r >= a.n) continue;
-        const int p = a.parents[r], len = kept_len(a.t, a.lens, p);
+        const int p = k > 0 ? a.parents[r] : -1, len = kept_len(a.t, a.lens, p);
         int src = 0, dst = 0, fill = 0;
         if (k > 0 && at + k > found) {
             latch(a.status, kStatusNoPages);                     // the pool is full: the row keeps what it has and does not grow
@@ -208,10 +208,16 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkPlan 
                 a.refs[page] = 1;
             }
         }
-        a.copies[3 * r] = src;
-        a.copies[3 * r + 1] = dst;
-        a.copies[3 * r + 2] = fill;
+        // only what is copied is listed
+        const int place = copied + block_prefix(fill > 0, red, total);
+        copied += total;
+        if (fill > 0) {
+            a.copies[3 * place] = src;
+            a.copies[3 * place + 1] = dst;
+            a.copies[3 * place + 2] = fill;
+        }
     }
+    if (threadIdx.x == 0) *a.n_copies = copied;
 }
 
 struct CompactPlan {
@@ -343,9 +349,10 @@ struct PageMove {
 };
 
 constexpr int kMoveThreads = 256;
-constexpr int kMovePiece = kMoveThreads * 16 * 4;     // bytes that a CTA moves at a time: four 16-byte loads a thread in flight
+constexpr int kMoveLoads = 4;                         // 16-byte loads of a thread in flight (with eight a compaction gains nothing, small copies lose)
+constexpr int kMovePiece = kMoveThreads * 16 * kMoveLoads;
 
-__global__ void __launch_bounds__(kMoveThreads) page_move_kernel(const PageMove a) {
+__global__ void __launch_bounds__(kMoveThreads, 6) page_move_kernel(const PageMove a) {
     pdl_launch_dependents();
     pdl_wait();
     const int n = a.n_copies ? *a.n_copies : a.n;
@@ -361,40 +368,45 @@ __global__ void __launch_bounds__(kMoveThreads) page_move_kernel(const PageMove 
     // a piece never crosses a head, so that copies of a begun page move its written positions only
     const int per_head = static_cast<int>((a.head_bytes + kMovePiece - 1) / kMovePiece);
     const int64_t units = static_cast<int64_t>(n) * a.planes * a.heads * per_head;
+    struct Unit {
+        const char* src;
+        int64_t step, bytes;        // from source to target; of this piece, 0: nothing
+    };
+    auto unit = [&](int64_t u) -> Unit {
+        if (u >= units) return {nullptr, 0, 0};
+        const int64_t run = quotient(u, per_head), page = quotient(run, a.heads), i = quotient(page, a.planes);
+        const int piece = static_cast<int>(u - run * per_head), head = static_cast<int>(run - page * a.heads), plane = static_cast<int>(page - i * a.planes);
+        const int from = a.copies[3 * i], to = a.copies[3 * i + 1], fill = a.copies[3 * i + 2];
+        const int64_t begin = static_cast<int64_t>(piece) * kMovePiece, bytes = fill < 0 ? a.head_bytes : fill * a.slot_bytes;
+        return {a.pool + plane * a.plane_bytes + from * a.page_bytes + head * a.head_bytes + begin, static_cast<int64_t>(to - from) * a.page_bytes, bytes - begin};
+    };
+    // the next piece is looked up while this one's loads are on their way
+    Unit now = unit(blockIdx.x);
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int piece = static_cast<int>(u % per_head);
-        int64_t rest = u / per_head;
-        const int head = static_cast<int>(rest % a.heads);
-        rest /= a.heads;
-        const int plane = static_cast<int>(rest % a.planes), i = static_cast<int>(rest / a.planes);
-        const int fill = a.copies[3 * i + 2];
-        if (fill == 0) continue;
-        const int64_t bytes = fill < 0 ? a.head_bytes : fill * a.slot_bytes;
-        const int64_t begin = static_cast<int64_t>(piece) * kMovePiece;
-        char* base = a.pool + plane * a.plane_bytes + head * a.head_bytes;
-        const char* src = base + a.copies[3 * i] * a.page_bytes;
-        char* dst = base + a.copies[3 * i + 1] * a.page_bytes;
-        uint4 v[4];
+        uint4 v[kMoveLoads];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int64_t o = begin + (k * kMoveThreads + threadIdx.x) * 16;
-            if (o < bytes) v[k] = *reinterpret_cast<const uint4*>(src + o);
+        for (int k = 0; k < kMoveLoads; ++k) {
+            const int o = (k * kMoveThreads + threadIdx.x) * 16;
+            if (o < now.bytes) v[k] = *reinterpret_cast<const uint4*>(now.src + o);
         }
+        const Unit next = unit(u + gridDim.x);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int64_t o = begin + (k * kMoveThreads + threadIdx.x) * 16;
-            if (o < bytes) *reinterpret_cast<uint4*>(dst + o) = v[k];
+        for (int k = 0; k < kMoveLoads; ++k) {
+            const int o = (k * kMoveThreads + threadIdx.x) * 16;
+            if (o < now.bytes) *reinterpret_cast<uint4*>(const_cast<char*>(now.src) + now.step + o) = v[k];
         }
+        now = next;
     }
 }
 
-static int move_launch(PageMove& a, const NexrtPagesArgs& x, cudaStream_t st) {
+// whole: every copy is of a whole page, whose heads then are one run.
+static int move_launch(PageMove& a, const NexrtPagesArgs& x, bool whole, cudaStream_t st) {
     a.pool = static_cast<char*>(x.pool);
-    a.planes = x.planes; a.heads = x.heads;
-    a.slot_bytes = x.slot_bytes; a.head_bytes = static_cast<int64_t>(x.slots) * x.slot_bytes;
-    a.page_bytes = a.head_bytes * x.heads; a.plane_bytes = a.page_bytes * x.pages;
-    const int64_t units = static_cast<int64_t>(a.n) * x.planes * x.heads * ((a.head_bytes + kMovePiece - 1) / kMovePiece);
-    const int64_t most = 8ll * sm_count();
+    a.planes = x.planes; a.heads = whole ? 1 : x.heads;
+    a.slot_bytes = x.slot_bytes; a.head_bytes = static_cast<int64_t>(x.slots) * x.slot_bytes * (whole ? x.heads : 1);
+    a.page_bytes = a.head_bytes * a.heads; a.plane_bytes = a.page_bytes * x.pages;
+    const int64_t units = static_cast<int64_t>(a.n) * a.planes * a.heads * ((a.head_bytes + kMovePiece - 1) / kMovePiece);
+    const int64_t most = 16ll * sm_count();
     int64_t grid = units < most ? units : most;
     if (a.table_out && grid < a.t.rows) grid = a.t.rows < most ? a.t.rows : most;
     return grid > 0 ? launch(page_move_kernel, dim3(static_cast<unsigned>(grid)), dim3(kMoveThreads), 0, st, a) : 0;
@@ -431,12 +443,14 @@ extern "C" int nexrt_page_fork(const NexrtPagesArgs* x, void* stream) {
     ForkPlan p = {};
     p.t = t; p.lens = static_cast<const int*>(x->lens); p.parents = static_cast<const int*>(x->parents); p.grow = static_cast<const int*>(x->grow);
     p.table = static_cast<int*>(x->table_out); p.table_stride = x->out_row; p.lens_out = static_cast<int*>(x->lens_out); p.refs = static_cast<int*>(x->refs);
-    p.copies = static_cast<int*>(x->scratch) + x->pages; p.free_list = static_cast<int*>(x->scratch);
+    p.free_list = static_cast<int*>(x->scratch); p.copies = p.free_list + x->pages; p.n_copies = p.copies + 3 * x->rows_out;
     p.status = static_cast<int*>(x->status); p.n = x->rows_out; p.grow_all = x->grow_all; p.pages = x->pages; p.count = counts_here(*x, x->rows_out);
-    if (const int e = launch(fork_plan_kernel, dim3(1), dim3(kPlanThreads), sizeof(int) * 2 * x->rows_out, st, p)) return e;
+    // up to a row a warp few threads plan sooner, barriers are what it waits for: 8 rows 9.8 us, by 1024 threads 10.6 (24 rows 10.0 and 9.1)
+    const bool few = x->rows_out <= 8 && x->pages <= 8 * kSmallTable;
+    if (const int e = launch(fork_plan_kernel, dim3(1), dim3(few ? 256 : kPlanThreads), sizeof(int) * 2 * x->rows_out, st, p)) return e;
     PageMove m = {};
-    m.copies = p.copies; m.n = x->rows_out;
-    return move_launch(m, *x, st);
+    m.copies = p.copies; m.n_copies = p.n_copies; m.n = x->rows_out;
+    return move_launch(m, *x, false, st);
 }
 
 extern "C" int nexrt_page_compact(const NexrtPagesArgs* x, void* stream) {
@@ -455,7 +469,7 @@ extern "C" int nexrt_page_compact(const NexrtPagesArgs* x, void* stream) {
     PageMove m = {};
     m.copies = p.copies; m.n_copies = p.n_copies; m.n = x->pages;
     m.t = t; m.lens = static_cast<const int*>(x->lens); m.remap = p.remap; m.table_out = static_cast<int*>(x->table_out); m.table_stride = x->out_row;
-    return move_launch(m, *x, st);
+    return move_launch(m, *x, true, st);
 }
 
 extern "C" int nexrt_page_copy(const NexrtPagesArgs* x, void* stream) {
@@ -469,5 +483,5 @@ extern "C" int nexrt_page_copy(const NexrtPagesArgs* x, void* stream) {
         return e;
     PageMove m = {};
     m.copies = copies; m.n = n;
-    return move_launch(m, *x, st);
+    return move_launch(m, *x, true, st);
 }

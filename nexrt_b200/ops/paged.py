@@ -149,7 +149,7 @@ def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent
     refs = _fresh(what, "refs", refs, (pages,), table, lens, parents, each, table)
     device = same_cuda_device(what, {kv.get_device(), table.get_device(), lens.get_device(), parents.get_device(), table_out.get_device(), lens_out.get_device(),
                                      refs.get_device()}, each, status)
-    scratch = table.new_empty(pages + 3 * n)
+    scratch = table.new_empty(pages + 3 * n + 1)
     on_device(device, lib().nexrt_page_fork, _PAGES.pack(
         _PAGES.size, base, table.data_ptr(), lens.data_ptr(), parents.data_ptr(), address(each), table_out.data_ptr(), lens_out.data_ptr(), refs.data_ptr(), 0, 0,
         scratch.data_ptr(), address(status), row, table_out.stride()[0], *sizes, n, 0 if each is not None else grow, 0), what)
