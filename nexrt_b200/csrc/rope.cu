@@ -12,7 +12,7 @@
 // norm's multipliers - stay in registers for all its heads.  A head lies over 4, 8 or 16 lanes, 16 values a lane: its sum of
 // squares is two to four shuffles for several heads at once; sums and products go two values an instruction.
 //
-// Measured: 4099 tokens of 36 heads of 256 (151 MB) 34 us, 0.69 of copy rate: 135 instructions a head keep the schedulers half busy, with
+// Measured: 4099 tokens of 36 heads of 256 (151 MB) 34 us, 0.69 of copy rate: 130 instructions a head keep the schedulers half busy, with
 // four warps each to hide their latencies (six CTAs an SM have to spill: 37 us).  Eight tokens of six heads: 3.9 us, the chain from
 // the position to the stores.
 #include "api.h"
