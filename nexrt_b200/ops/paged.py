@@ -220,6 +220,15 @@ class PagedCache:
     def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, rows: torch.Tensor, inv_freq: torch.Tensor, **how) -> torch.Tensor:
         return rope_append(q, k, v, positions, rows, self.kv[layer, 0], self.kv[layer, 1], self.table, inv_freq, status=self.status, **how)
 
+    def load_kv(self, layer: int, row: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Install ``k, v [kv heads][positions][dim]`` (already normalised and rotated, as ``DecodeEngine.export_state`` gives them) as the first
+        positions of ``row``, which has room for them (``fork`` with ``grow``)."""
+        if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or not 0 <= row < self.lens.numel():
+            raise ValueError("PagedCache.load_kv: k and v are [kv heads, positions, dim] for a row of the cache")
+        k, v = k.transpose(0, 1), v.transpose(0, 1)
+        at = torch.arange(k.shape[0], dtype=I32, device=k.device)
+        self.append(layer, k[:, :0], k, v, at, torch.full_like(at, row), torch.empty(0, device=k.device))
+
     def attend(self, layer: int, q: torch.Tensor, **how) -> torch.Tensor:
         return paged_attention(q, self.kv[layer, 0], self.kv[layer, 1], self.table, self.lens, status=self.status, **how)
 

@@ -263,3 +263,35 @@ def test_a_captured_step_goes_on_from_replay_to_replay():
         twin.fork(parents, 1)
         assert torch.equal(cache.table, twin.table) and torch.equal(cache.lens, twin.lens) and torch.equal(cache.refs, twin.refs)
     cache.check()
+
+
+def test_an_engine_prefill_becomes_rows_of_a_cache():
+    """The engine prefills one prompt; its keys and values go into a paged row, three beams fork it, and each attends like the engine's own cache."""
+    from nexrt_b200.models.reference import synthetic_prompt
+    from nexrt_b200.ops.paged import paged_attention
+    from nexrt_b200.testing import make_engine, shrunk_checkpoint
+
+    cfg, ckpt = shrunk_checkpoint(0)
+    eng = make_engine(cfg, ckpt)
+    prompt = synthetic_prompt(cfg.vocab, 37, seed=3)
+    eng.prefill(prompt)
+    state = eng.export_state()
+    full = [x for x in state["layers"].values() if x["kind"] == "full"]
+    L, nk, hd = state["L"], cfg.n_kv_heads, cfg.head_dim
+    cache = PagedCache(len(full), 30, nk, 8, hd, 3, 64)
+    cache.fork(grow=ints([L, 0, 0]))
+    for i, x in enumerate(full):
+        cache.load_kv(i, 0, x["k_cache"], x["v_cache"])
+    cache.fork(ints([0, 0, 0]))
+    cache.check()
+    assert cache.lens.tolist() == [L] * 3 and int((cache.refs > 0).sum()) == -(-L // 8)
+    q = torch.randn(3, cfg.n_q_heads, hd, device=DEV).to(torch.bfloat16)
+    for i, x in enumerate(full):
+        assert torch.equal(cache.kv[i, 0][cache.table[1, : -(-L // 8)].long()].transpose(0, 1).reshape(nk, -1, hd)[:, :L], x["k_cache"])
+        whole = torch.stack([x["k_cache"], x["v_cache"]])[:, None].contiguous()       # the engine's cache as one page of L slots
+        want = paged_attention(q, whole[0], whole[1], torch.zeros(3, 1, dtype=torch.int32, device=DEV), cache.lens)
+        got = cache.attend(i, q)
+        # both are within half a step (2^-8) and the sums' own error of the same numbers; the two splits of the keys differ
+        assert torch.all((got.float() - want.float()).abs() <= 2.0**-7 * want.float().abs() + 2.0**-10)
+    with pytest.raises(ValueError):
+        cache.load_kv(0, 3, full[0]["k_cache"], full[0]["v_cache"])
