@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kPaThreads, resident_ctas(D)) paged_attn_kerne
         auto find = [&](int tile) -> uint32_t {
             const int p = key0 + tile * kChunk + (lane & 15);
             if (tile >= tiles || p < lo || p >= hi) return kNoRow;
-            const int j = p / a.table.page, page = page_at(a.table, b, j);
+            const int j = static_cast<int>(static_cast<uint32_t>(p) / static_cast<uint32_t>(a.table.page)), page = page_at(a.table, b, j);
             if (page < 0) {
                 if (a.status) atomicCAS(a.status, 0, static_cast<int>(kStatusBadPage));
                 return kNoRow;
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kPaThreads, resident_ctas(D)) paged_attn_kerne
             sum[r] = 0.f;
             slope[r] = MODS && a.slopes && g + 8 * r < rows ? a.slopes[h0 + g + 8 * r] * 1.4426950408889634f : 0.f;
         }
-        const float scale2 = a.scale * 1.4426950408889634f;
+        const float scale2 = a.scale * 1.4426950408889634f, to_cap = a.scale / a.softcap, cap2 = a.softcap * 1.4426950408889634f;
         // with few registers' worth of queries they stay there
         constexpr bool kHold = KS * NTR <= 16;
         uint32_t qr[kHold ? KS : 1][4];
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kPaThreads, resident_ctas(D)) paged_attn_kerne
             // ---- mask and running softmax: row g + 8 r has its 16 scores in the four lanes of a g
             uint32_t ph[NTR][2], pl[NTR][2];
             float corr[NTR];
-            const int tile0 = key0 + i * kChunk;
+            const float dist = static_cast<float>(hi - 1 - (key0 + i * kChunk) - 2 * t);   // of the lane's first key (exact up to 2^24)
 #pragma unroll
             for (int r = 0; r < NTR; ++r) {
                 float v[4] = {s[0][2 * r], s[0][2 * r + 1], s[1][2 * r], s[1][2 * r + 1]};
@@ -402,9 +402,8 @@ __global__ void __launch_bounds__(kPaThreads, resident_ctas(D)) paged_attn_kerne
                 for (int u = 0; u < 4; ++u) {
                     const int key = (u >> 1) * 8 + 2 * t + (u & 1);
                     if (MODS) {
-                        float y = v[u] * a.scale;
-                        if (a.softcap > 0.f) y = a.softcap * tanhf(y / a.softcap);
-                        v[u] = y * 1.4426950408889634f - slope[r] * static_cast<float>(hi - 1 - tile0 - key);
+                        const float y = a.softcap > 0.f ? cap2 * tanhf(v[u] * to_cap) : v[u] * scale2;
+                        v[u] = y - slope[r] * (dist - static_cast<float>((u >> 1) * 8 + (u & 1)));
                     } else {
                         v[u] *= scale2;
                     }
