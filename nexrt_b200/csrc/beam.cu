@@ -144,13 +144,6 @@ template <typename T> __device__ __noinline__ uint4 edge_piece(const T* base, in
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 2^x for x <= 0, to 2^-22 of the value; below 2^-126 zero
-__device__ __forceinline__ float exp2_down(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const BeamArgs a) {
     constexpr int VEC = Piece<T>::kValues, NV = kPieces, kWarps = kSliceThreads / 32;

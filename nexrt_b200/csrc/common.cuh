@@ -193,6 +193,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return r;
 }
 
+// 2^x for x <= 0, to 2^-22 of the value; below 2^-126 zero
+__device__ __forceinline__ float exp2_down(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Block-wide sum for blockDim.x <= 1024; `red` is 32 floats of shared memory.
 __device__ __forceinline__ float block_sum(float v, float* red) {
     v = warp_sum(v);

@@ -414,10 +414,10 @@ __global__ void __launch_bounds__(kPaThreads, resident_ctas(D)) paged_attn_kerne
                 m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 m = max_nan(m, mx[r]);
                 const float shift = m == -INFINITY ? 0.f : m;
-                corr[r] = mx[r] == m ? 1.f : exp2f(mx[r] - shift);
+                corr[r] = mx[r] == m ? 1.f : exp2_down(mx[r] - shift);
                 mx[r] = m;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = exp2f(v[u] - shift);
+                for (int u = 0; u < 4; ++u) v[u] = exp2_down(v[u] - shift);
                 sum[r] = fmaf(sum[r], corr[r], (v[0] + v[1]) + (v[2] + v[3]));
                 split2(v[0], v[1], ph[r][0], pl[r][0], T());
                 split2(v[2], v[3], ph[r][1], pl[r][1], T());
