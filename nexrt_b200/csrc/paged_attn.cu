@@ -21,7 +21,8 @@
 // batch's lengths cut an item).
 //
 // Measured: 200K keys, 2 key heads of 256, 32 query heads: 75 us, 5.4 TB/s of keys and values, 0.84 of copy rate (the rings alone fill in
-// 64); 48 sequences of 0 to 16384 keys, 8 heads of 128: 93 us, 0.86; one sequence of 1100 keys: 9.2 us, two launches and their chains.
+// 64); 48 sequences of 0 to 16384 keys, 8 heads of 128: 93 us, 0.86; 16 sequences of up to
+// 4097 keys, 8 heads of 64, capped and biased: 16 us; one sequence of 1100 keys: 9.2 us, two launches and their chains.
 #include "api.h"
 #include "paged.cuh"
 
@@ -51,8 +52,8 @@ struct PagedAttnArgs {
     float scale, softcap;
 };
 
-// CTAs on an SM, and half tiles of a warp's ring: what registers and shared memory hold.  (64 dims: three CTAs 20.7 us where two take
-// 25.8; 128 dims: two with rings of four 94.9, three 99.9, two with rings of six 96.4.)
+// CTAs on an SM, and half tiles of a warp's ring: what registers and shared memory hold.  (64 dims: three CTAs take 0.8 of the time of
+// two; 128 dims: two with rings of four 94.9, three 99.9, two with rings of six 96.4.)
 constexpr int resident_ctas(int dim) { return dim == 64 ? 3 : 2; }
 template <int D> constexpr int ring_depth() { return D == 256 ? 3 : (D == 64 ? 6 : 4); }
 template <int D> constexpr int half_bytes() { return kTile * (D * 2 + 16); }
