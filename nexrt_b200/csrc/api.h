@@ -250,7 +250,7 @@ int nexrt_page_compact(const NexrtPagesArgs* args, void* stream);   /* scratch: 
 int nexrt_page_copy(const NexrtPagesArgs* args, void* stream);      /* table: sources, lens: targets, rows of them; scratch: int[3 rows] */
 
 // ---- beam search (beam.cu) ------------------------------------------------------------------------------------------------
-int nexrt_beam_slices(int rows, int vocab, int type);   /* a call's scratch is batch * beams * slices * (k + 2) words of 8 bytes */
+int nexrt_beam_slices(int rows, int beams, int vocab, int k, int type);   /* a call's scratch is batch * beams * slices * (k + 2) words of 8 bytes */
 typedef struct NexrtBeamArgs {
     uint64_t size;
     const void *logits, *scores, *finished;           /* finished may be NULL */

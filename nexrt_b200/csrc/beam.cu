@@ -7,10 +7,12 @@
 //
 // Within a beam the order of the totals is that of the logits, so one pass over a slice of a row gives everything that is
 // needed of it: its maximum, its sum of exp and its k largest logits.  A CTA walks its slice in steps of 16 KB, 64 bytes a thread in
-// registers as they came, the next step's loads in flight.  The k largest: the k-th largest of 64 or 128 maxima of the first step bounds them from below, the few values
-// at or above it are collected and at the end ranked by counting (equal values in masses are found by bisection instead).  A second
-// kernel, one CTA a request, joins the slices.  Bound by the logits' bytes, and for one request by the two launches.  Measured: 117 live
-// rows of 248320 bf16 logits (58 MB) 30 us, about 14 instructions a value; four rows of fp32 10 us.
+// registers as they came, the next step's loads in flight.  The k largest: the k-th largest of 64 or 128 maxima of the first step bounds
+// them from below; the few values of that step at or above it, and of the later ones above it (an equal one comes behind k with lower
+// tokens), are collected and at the end ranked by counting.  Equal values in masses, as masked vocabularies have them, are taken in the
+// order of their tokens, k of them at most; what still does not fit is selected digit by digit.  A second kernel, one CTA a request, joins
+// the slices.  Bound by the logits' bytes, and for one request by the two launches.  Measured: 117 live rows of 248320 bf16 logits
+// (58 MB) 30 us, about 14 instructions a value, 128 rows with all but ten values masked 28; four rows of fp32 11 us.
 #include <type_traits>
 
 #include "api.h"
@@ -62,14 +64,42 @@ __device__ __forceinline__ bool beam_is_closed(const BeamArgs& a, int b, int w) 
     return done || !(s > -INFINITY) || s == INFINITY;
 }
 
-// sum of an int over the CTA, for all threads; red: 32 ints
-__device__ __forceinline__ int cta_sum(int v, int* red) {
-    v = __reduce_add_sync(0xffffffffu, v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    const int n = blockDim.x >> 5, lane = threadIdx.x & 31;
-    return __reduce_add_sync(0xffffffffu, lane < n ? red[lane] : 0);
+// The threshold of the k largest of n keys, a digit of eight bits at a time; 0 is no key.  Taken are keys above `edge`, and of those equal to
+// it `ties` (-1: all; equal keys are told apart by the caller).  hist: 258 ints.
+template <typename Key> __device__ __forceinline__ u64 largest_edge(Key key_of, int n, int k, int* hist, int& ties) {
+    u64 edge = 0;
+    ties = -1;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < 258; i += blockDim.x) hist[i] = 0;
+        __syncthreads();
+        for (int i0 = 0; i0 < n; i0 += blockDim.x) {
+            const int i = i0 + threadIdx.x;
+            const u64 key = i < n ? key_of(i) : 0;
+            const int digit = key != 0 && (shift == 56 || key >> (shift + 8) == edge >> (shift + 8)) ? static_cast<int>(key >> shift & 255) : -1;
+            int same;
+            __match_all_sync(0xffffffffu, digit, &same);           // (equal keys in masses: one addition a warp)
+            if (digit >= 0 && (!same || (threadIdx.x & 31) == 0)) atomicAdd(hist + digit, same ? 32 : 1);
+        }
+        __syncthreads();
+        if (threadIdx.x < 256) {
+            int above = 0;
+#pragma unroll 8
+            for (int i = threadIdx.x + 1; i < 256; ++i) above += hist[i];
+            if (above < k && above + hist[threadIdx.x] >= k) {
+                hist[256] = static_cast<int>(threadIdx.x) + 1;
+                hist[257] = above;
+            }
+        }
+        __syncthreads();
+        if (hist[256] == 0) return 0;                              // fewer than k
+        const int digit = hist[256] - 1;
+        edge |= static_cast<u64>(digit) << shift;
+        k -= hist[257];
+        if (hist[digit] == k) return edge;
+    }
+    ties = k;
+    return edge;
 }
 
 // 16 bytes of a row as they came; `top` takes maxNum over two or four such pieces' words without unpacking 16-bit types.
@@ -112,6 +142,13 @@ template <typename T> struct Piece {
         }
         return bits;
     }
+    // The smallest value of the type above v (NaN above infinity: nothing is at least that).
+    static __device__ __forceinline__ float above(float v) {
+        auto up = [](unsigned int bits, unsigned int sign) { return bits & sign ? (bits == sign ? 1u : bits - 1u) : bits + 1u; };
+        if constexpr (sizeof(T) == 4) return __uint_as_float(up(__float_as_uint(v), 0x80000000u));
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(up(__float_as_uint(v) >> 16, 0x8000u) << 16);
+        else return __half2float(__ushort_as_half(static_cast<unsigned short>(up(__half_as_ushort(__float2half_rn(v)), 0x8000u))));
+    }
     __device__ __forceinline__ float top() const {
         if constexpr (sizeof(T) == 4) {
             return fmaxf(fmaxf(value(0), value(1)), fmaxf(value(2), value(3)));
@@ -151,7 +188,9 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
     __shared__ double warp_part[kWarps];
     __shared__ u64 keep[kBeamKeep];
     __shared__ unsigned int bound_s;
-    __shared__ int count_s, red[32];
+    __shared__ float equal_s;
+    __shared__ int count_s, tied_s, red[32];
+    static_assert(sizeof(keep) >= 258 * sizeof(int), "the digits' counts lie where the candidates did");
     pdl_launch_dependents();
     pdl_wait();
     const int row = blockIdx.y, slice = blockIdx.x, b = row / a.beams, w = row - b * a.beams;
@@ -168,7 +207,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t at_slice = static_cast<int64_t>(row) * a.slices + slice;
     u64* out = a.keys + at_slice * a.k;
-    if (threadIdx.x == 0) count_s = 0;
+    if (threadIdx.x == 0) count_s = tied_s = 0;
 
     // the thread's maximum and its sum of exp below it, in 64 bits from 32 values on
     float top = -INFINITY, bound = 0.f;
@@ -226,13 +265,28 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
             if (threadIdx.x == 0) bound_s = 0xffffffffu;
             __syncthreads();
             int above = 0;
+            float least = group;
 #pragma unroll 16
-            for (int i = part; i < groups; i += lanes) above += group_top[i] > group;
+            for (int i = part; i < groups; i += lanes) {
+                above += group_top[i] > group;
+                least = fminf(least, group_top[i]);
+            }
             above += __shfl_xor_sync(0xffffffffu, above, 1);
-            if (lanes == 4) above += __shfl_xor_sync(0xffffffffu, above, 2);
-            if (part == 0 && above < a.k) atomicMin(&bound_s, ord32(group));
+            least = fminf(least, __shfl_xor_sync(0xffffffffu, least, 1));
+            if (lanes == 4) {
+                above += __shfl_xor_sync(0xffffffffu, above, 2);
+                least = fminf(least, __shfl_xor_sync(0xffffffffu, least, 2));
+            }
+            if (part == 0 && above < a.k) {
+                atomicMin(&bound_s, ord32(group));
+                if (group == least) {                    // even the smallest reaches the bound: values equal to it in masses, a masked slice
+                    tied_s = 1;
+                    equal_s = group;
+                }
+            }
             __syncthreads();
             bound = unord32(bound_s);
+            if (tied_s) bound = Piece<T>::above(bound);
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -247,6 +301,8 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
                     if (to < kBeamKeep) keep[to] = (static_cast<u64>(ord32(v)) << 32) | static_cast<unsigned int>(~token);
                 }
             }
+        // what equals the bound comes behind the k of the first step, whose tokens are lower
+        if (p0 == lo && !tied_s) bound = Piece<T>::above(bound);
         if ((step & 3) == 3 && p0 + kSliceThreads * NV < hi) {
             // half full: only the k largest so far go on, and what follows has to reach the last of them
             __syncthreads();
@@ -275,7 +331,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
                 }
                 if (threadIdx.x == 0) count_s = a.k;
                 __syncthreads();
-                bound = unord32(bound_s);
+                bound = Piece<T>::above(unord32(bound_s));
             }
             __syncthreads();
         }
@@ -303,6 +359,30 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
         a.sums[at_slice] = t;
         a.tops[at_slice] = m;
     }
+    const int first = max(lo * VEC - off, 0), last = min(hi * VEC - off, a.vocab);
+    if (tied_s) {
+        // of the first step's values equal to its bound the k lowest tokens
+        const float equal = equal_s;
+        const int end = min(last, (lo + kSliceThreads * NV) * VEC - off);
+        for (int t0 = first, taken = 0; t0 < end && taken < a.k; t0 += kSliceThreads) {
+            const int token = t0 + threadIdx.x;
+            const bool here = token < end && static_cast<float>(base[token]) == equal;
+            const unsigned int mask = __ballot_sync(0xffffffffu, here);
+            if (lane == 0) red[warp] = __popc(mask);
+            __syncthreads();
+            int place = taken + __popc(mask & ((1u << lane) - 1u));
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) {
+                if (i < warp) place += red[i];
+                taken += red[i];
+            }
+            if (here && place < a.k) {
+                const int to = atomicAdd(&count_s, 1);
+                if (to < kBeamKeep) keep[to] = (static_cast<u64>(ord32(equal)) << 32) | static_cast<unsigned int>(~token);
+            }
+            __syncthreads();
+        }
+    }
     const int count = count_s;
     if (!over && count <= kBeamKeep) {
         for (int i = threadIdx.x; i < count; i += kSliceThreads) {
@@ -314,21 +394,13 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
         for (int i = count + threadIdx.x; i < a.k; i += kSliceThreads) out[i] = 0;
         return;
     }
-    // many equal values: the k-th largest key bit by bit (keys differ, so exactly k are at or above it), the slice read again each time
-    const int first = max(lo * VEC - off, 0), last = min(hi * VEC - off, a.vocab);
+    // more than there is room for (keys differ, so exactly k are at or above the edge); the slice is read again for each digit
     auto key_at = [&](int token) -> u64 {
         const float v = static_cast<float>(base[token]);
         return v != v ? 0 : (static_cast<u64>(ord32(v)) << 32) | static_cast<unsigned int>(~token);
     };
-    u64 edge = 0;
-#pragma unroll 1
-    for (int bit = 63; bit >= 0; --bit) {
-        const u64 next = edge | (1ull << bit);
-        int n = 0;
-        for (int i = first + threadIdx.x; i < last; i += kSliceThreads) n += key_at(i) >= next;
-        if (cta_sum(n, red) >= a.k) edge = next;
-    }
-    __syncthreads();
+    int ties;
+    const u64 edge = largest_edge([&](int i) { return key_at(first + i); }, last - first, a.k, reinterpret_cast<int*>(keep), ties);
     if (threadIdx.x == 0) count_s = 0;
     __syncthreads();
     for (int i = first + threadIdx.x; i < last; i += kSliceThreads) {
@@ -343,19 +415,23 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamArgs 
     __shared__ double lse[kBeamMaxWidth];           // of a live beam
     __shared__ float score_s[kBeamMaxWidth];
     __shared__ int kind[kBeamMaxWidth];             // 0 live, 1 finished, 2 closed without a candidate above -infinity
-    __shared__ u64 group_top[kJoinThreads / 4], keep[kBeamKeep], keep_tie[kBeamKeep];
-    __shared__ u64 bound_s;
-    __shared__ int count_s, red[32];
+    __shared__ u64 group_top[kJoinThreads / 4], group_tie[kJoinThreads / 4], keep[kBeamKeep], keep_tie[kBeamKeep];
+    __shared__ u64 bound_s, bound_tie_s;
+    __shared__ int count_s;
     pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.beams, S = a.slices, k = a.k;
     const int per = S * k, total_n = W * per;
     const u64* const keys = a.keys + static_cast<int64_t>(b) * total_n;
+    // Candidate `i` of this thread.  Lists of 64 would put all their first ones with the same threads, and too many would reach the bound that
+    // the groups below give (8 beams of 61 slices, k = 64: 2.2 ms); turned round by round, every group has some of the largest.
+    auto index = [&](int i) { return i * kJoinThreads + static_cast<int>((threadIdx.x + i * 199u) % kJoinThreads); };
+    const int rounds = (total_n + kJoinThreads - 1) / kJoinThreads;
     // the first candidates are on their way while the beams' sums are made (what belongs to a closed beam was not written and is not used)
     u64 raw[kJoinHold];
 #pragma unroll
     for (int i = 0; i < kJoinHold; ++i) {
-        const int n = i * kJoinThreads + threadIdx.x;
+        const int n = index(i);
         raw[i] = n < total_n ? keys[n] : 0;
     }
     for (int w = warp; w < W; w += kJoinThreads / 32) {
@@ -422,39 +498,57 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamArgs 
     };
     auto reload = [&](int n, u64& tie) { return candidate(n, keys[n], tie); };
 
-    u64 held[kJoinHold], held_tie[kJoinHold], top = 0, tie = 0;
+    u64 held[kJoinHold], held_tie[kJoinHold], top = 0, top_tie = 0, tie = 0;
+    auto larger = [](u64 x, u64 x_tie, u64 y, u64 y_tie) { return x > y || (x == y && x_tie > y_tie); };
+    auto raise = [&](u64 key, u64 key_tie) {
+        if (larger(key, key_tie, top, top_tie)) {
+            top = key;
+            top_tie = key_tie;
+        }
+    };
 #pragma unroll
     for (int i = 0; i < kJoinHold; ++i) {
-        const int n = i * kJoinThreads + threadIdx.x;
+        const int n = index(i);
         held_tie[i] = 0;
         held[i] = n < total_n ? candidate(n, raw[i], held_tie[i]) : 0;
-        top = held[i] > top ? held[i] : top;
+        if (held[i]) raise(held[i], held_tie[i]);
     }
-    for (int n = kJoinHold * kJoinThreads + threadIdx.x; n < total_n; n += kJoinThreads) {
-        const u64 key = reload(n, tie);
-        top = key > top ? key : top;
+    for (int i = kJoinHold; i < rounds; ++i) {
+        const int n = index(i);
+        if (const u64 key = n < total_n ? reload(n, tie) : 0) raise(key, tie);
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-        const u64 other = __shfl_xor_sync(0xffffffffu, top, o);
-        top = other > top ? other : top;
+        const u64 other = __shfl_xor_sync(0xffffffffu, top, o), other_tie = __shfl_xor_sync(0xffffffffu, top_tie, o);
+        raise(other, other_tie);
     }
-    if ((lane & 3) == 0) group_top[threadIdx.x >> 2] = top;
-    if (threadIdx.x == 0) bound_s = ~0ull;
+    if ((lane & 3) == 0) {
+        group_top[threadIdx.x >> 2] = top;
+        group_tie[threadIdx.x >> 2] = top_tie;
+    }
+    if (threadIdx.x == 0) bound_s = bound_tie_s = 0;
     __syncthreads();
     {
-        // the k-th largest of the groups' maxima: four threads a group
-        int above = 0;
+        // the k-th largest of the groups' maxima, which all differ where there is one: four threads a group
+        int above = 0, same = 0;
 #pragma unroll 8
-        for (int i = threadIdx.x & 3; i < kJoinThreads / 4; i += 4) above += group_top[i] > top;
+        for (int i = threadIdx.x & 3; i < kJoinThreads / 4; i += 4) {
+            above += group_top[i] > top;
+            same += group_top[i] == top;
+        }
+        if (same > ((threadIdx.x >> 2 & 3) == (threadIdx.x & 3)))        // others than the group itself
+            for (int i = threadIdx.x & 3; i < kJoinThreads / 4; i += 4) above += group_top[i] == top && group_tie[i] > top_tie;
         above += __shfl_xor_sync(0xffffffffu, above, 1);
         above += __shfl_xor_sync(0xffffffffu, above, 2);
-        if ((lane & 3) == 0 && above < k) atomicMin(&bound_s, top);
+        if ((lane & 3) == 0 && above == k - 1 && top != 0) {
+            bound_s = top;
+            bound_tie_s = top_tie;
+        }
     }
     __syncthreads();
-    const u64 bound = bound_s;
+    const u64 bound = bound_s, bound_tie = bound_tie_s;
     auto collect = [&](u64 key, u64 key_tie) {
-        if (key != 0 && key >= bound) {
+        if (key != 0 && !larger(bound, bound_tie, key, key_tie)) {
             const int at = atomicAdd(&count_s, 1);
             if (at < kBeamKeep) {
                 keep[at] = key;
@@ -464,30 +558,19 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamArgs 
     };
 #pragma unroll
     for (int i = 0; i < kJoinHold; ++i) collect(held[i], held_tie[i]);
-    for (int n = kJoinHold * kJoinThreads + threadIdx.x; n < total_n; n += kJoinThreads) {
-        const u64 key = reload(n, tie);
-        collect(key, tie);
+    for (int i = kJoinHold; i < rounds; ++i) {
+        const int n = index(i);
+        if (const u64 key = n < total_n ? reload(n, tie) : 0) collect(key, tie);
     }
     __syncthreads();
     int count = count_s;
     if (count > kBeamKeep) {
-        // the k-th largest total bit by bit, then the last of its equals that is still among the k
-        u64 edge = 0, edge_tie = 0;
-        for (int bit = 63; bit >= 0; --bit) {
-            const u64 next = edge | (1ull << bit);
-            int n = 0;
-            for (int i = threadIdx.x; i < total_n; i += kJoinThreads) n += reload(i, tie) >= next;
-            if (cta_sum(n, red) >= k) edge = next;
-        }
-        int above = 0;
-        for (int i = threadIdx.x; i < total_n; i += kJoinThreads) above += reload(i, tie) > edge;
-        above = cta_sum(above, red);
-        for (int bit = 63; bit >= 0; --bit) {
-            const u64 next = edge_tie | (1ull << bit);
-            int n = 0;
-            for (int i = threadIdx.x; i < total_n; i += kJoinThreads) n += reload(i, tie) == edge && tie >= next;
-            if (above + cta_sum(n, red) >= k) edge_tie = next;
-        }
+        // the k-th largest total, then the last of its equals that is still among the k
+        int ties, none;
+        u64 edge_tie = 0;
+        const u64 edge = largest_edge([&](int n) { return reload(n, tie); }, total_n, k, reinterpret_cast<int*>(keep), ties);
+        if (ties >= 0)
+            edge_tie = largest_edge([&](int n) { const u64 key = reload(n, tie); return key == edge ? tie : 0; }, total_n, ties, reinterpret_cast<int*>(keep), none);
         __syncthreads();
         if (threadIdx.x == 0) count_s = 0;
         __syncthreads();
@@ -577,10 +660,13 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
 }
 
 // Slices of a row: no more than there are steps, and together about two waves of CTAs (four on an SM at a time).  A CTA's first step
-// finds its bound, which costs as much as the step; those behind it are cheap.
-static int beam_slices(int rows, int vocab, int type) {
+// finds its bound, which costs as much as the step; those behind it are cheap.  One CTA joins a request's k of every slice: with large k
+// and many beams no more of them than it reads in a few microseconds (8 beams of 248320, k = 64: 61 slices 80 us, 16 slices 39).
+constexpr int kJoinMost = 8192;
+static int beam_slices(int rows, int beams, int vocab, int k, int type) {
     const int64_t bytes = (static_cast<int64_t>(vocab) + 8) * (type == 2 ? 4 : 2);
-    const int most = static_cast<int>((bytes + kStepBytes - 1) / kStepBytes), share = 8 * sm_count() / (rows > 0 ? rows : 1);
+    const int most = static_cast<int>((bytes + kStepBytes - 1) / kStepBytes), wave = 8 * sm_count() / (rows > 0 ? rows : 1), join = kJoinMost / (beams * k);
+    const int share = wave < join ? wave : join;
     return share < 1 ? 1 : (share < most ? share : most);
 }
 
@@ -589,12 +675,12 @@ static int beam_slices(int rows, int vocab, int type) {
 using namespace nexrt;
 
 // Slices of a row: a call's scratch is batch * beams * slices * (k + 2) words of 8 bytes.
-extern "C" int nexrt_beam_slices(int rows, int vocab, int type) { return beam_slices(rows, vocab, type); }
+extern "C" int nexrt_beam_slices(int rows, int beams, int vocab, int k, int type) { return beams < 1 || k < 1 ? 1 : beam_slices(rows, beams, vocab, k, type); }
 
 extern "C" int nexrt_beam_select(const NexrtBeamArgs* x, void* stream) {
     if (x->size != sizeof(*x) || x->batch < 0 || x->beams < 1 || x->beams > kBeamMaxWidth || x->vocab < 1 || x->vocab > kBeamMaxVocab || x->k < 1 || x->k > kBeamMaxK ||
         static_cast<int64_t>(x->beams) * x->vocab < x->k || (x->finished != nullptr && (x->eos < 0 || x->eos >= x->vocab)) ||
-        static_cast<int64_t>(x->batch) * x->beams > 65535 || x->type < 0 || x->type > 2 || x->slices != beam_slices(x->batch * x->beams, x->vocab, x->type))
+        static_cast<int64_t>(x->batch) * x->beams > 65535 || x->type < 0 || x->type > 2 || x->slices != beam_slices(x->batch * x->beams, x->beams, x->vocab, x->k, x->type))
         return cudaErrorInvalidValue;
     if (x->batch == 0) return 0;
     BeamArgs a = {};

@@ -55,7 +55,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, finished:
     best, rows, tokens = scores.new_empty(batch, k), scores.new_empty(batch, k, dtype=I32), scores.new_empty(batch, k, dtype=I32)
     if batch:
         L = lib()
-        slices = L.nexrt_beam_slices(batch * beams, vocab, TYPES[kind])
+        slices = L.nexrt_beam_slices(batch * beams, beams, vocab, k, TYPES[kind])
         scratch = scores.new_empty(batch * beams * slices * (k + 2), dtype=torch.int64)
         on_device(device, L.nexrt_beam_select, _BEAM.pack(
             _BEAM.size, logits.data_ptr(), scores.data_ptr(), address(finished), best.data_ptr(), rows.data_ptr(), tokens.data_ptr(), scratch.data_ptr(), address(status),

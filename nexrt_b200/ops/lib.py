@@ -118,7 +118,7 @@ _PROTOTYPES = {
     "nexrt_page_fork": [c_char_p, vp],
     "nexrt_page_compact": [c_char_p, vp],
     "nexrt_page_copy": [c_char_p, vp],
-    "nexrt_beam_slices": [ci, ci, ci],
+    "nexrt_beam_slices": [ci, ci, ci, ci, ci],
     "nexrt_beam_select": [c_char_p, vp],
     "nexrt_reorder_rows": [c_char_p, vp],
     "nexrt_ipc_alloc": [c_size_t, POINTER(c_void_p)],

@@ -98,6 +98,38 @@ def test_masked_vocabularies():
     check(x, s, 8)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V,k", [(50257, 8), (248320, 16), (33000, 64)])
+def test_values_in_masses(dtype, V, k):
+    """Almost everything masked, by -inf and by the lowest number, the little that is allowed at either end, in the middle, or less than k; a
+    block of equal values; logits in ascending order, where every step has more above the bound than there is room for."""
+    x, s = inputs(2, 4, V, dtype)
+    for mask in (-math.inf, torch.finfo(dtype).min):
+        for first, n in ((0, 40), (V - 700, 700), (V // 2, 3), (V // 3, 9000)):
+            y = torch.full_like(x, mask)
+            y[..., first : first + n] = x[..., first : first + n]
+            check(y, s, k)
+    y = x.clone()
+    y[..., 100 : V // 2] = 3.0
+    check(y, s, k)
+    check(torch.sort(x, -1).values, s, k)
+    check(torch.sort(x, -1, descending=True).values, s, k)
+
+
+def test_many_beams_of_one_score():
+    """Candidates of eight beams whose lists lie side by side in the join; and of 256, where the high ones all lie with half of its threads and
+    more of them reach its bound than there is room for - different ones, and equal ones, of which the order of beams and tokens decides."""
+    x, s = inputs(1, 8, 248320)
+    check(x, torch.zeros_like(s), 64)
+    x, s = inputs(1, 256, 300, std=0.01)
+    w = torch.arange(256, device=DEV)
+    high = (64 * (w % 8) - 199 * (w // 8)) % 512 <= 188
+    assert int(high.sum()) * 64 > 4096
+    s = torch.where(high, 0.0, -1000.0)[None]
+    check(x, s, 64)
+    check(torch.zeros_like(x), s, 64)
+
+
 def test_finished_and_broken_beams():
     x, s = inputs(4, 4, 3000)
     fin = torch.zeros(4, 4, dtype=torch.bool, device=DEV)
