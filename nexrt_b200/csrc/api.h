@@ -245,9 +245,9 @@ typedef struct NexrtPagesArgs {
     int64_t table_row, out_row;
     int planes, pages, heads, slots, slot_bytes, rows, width, rows_out, grow_all, reserved;
 } NexrtPagesArgs;
-int nexrt_page_fork(const NexrtPagesArgs* args, void* stream);      /* scratch: int[pages + 3 rows_out + 1] */
+int nexrt_page_fork(const NexrtPagesArgs* args, void* stream);      /* scratch: int[3 (pages + rows_out) + 1] */
 int nexrt_page_compact(const NexrtPagesArgs* args, void* stream);   /* scratch: int[5 pages + 1] */
-int nexrt_page_copy(const NexrtPagesArgs* args, void* stream);      /* table: sources, lens: targets, rows of them; scratch: int[3 rows] */
+int nexrt_page_copy(const NexrtPagesArgs* args, void* stream);      /* table: sources, lens: targets, rows of them; scratch: int[3 rows + 2 pages] */
 
 // ---- beam search (beam.cu) ------------------------------------------------------------------------------------------------
 int nexrt_beam_slices(int rows, int beams, int vocab, int k, int type);   /* a call's scratch is batch * beams * slices * (k + 2) words of 8 bytes */

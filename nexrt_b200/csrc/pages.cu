@@ -17,6 +17,9 @@ namespace nexrt {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanRows = 4096;         // rows whose plan one CTA holds in shared memory
 constexpr int kPagesPerThread = 8;
+// Rows up to which each searches the others for holders of its begun page (a microsecond less at 64 rows); more are counted page by page (4096
+// rows of eight a page: a fork 548 -> 51 us).
+constexpr int kSearchRows = 256;
 // Entries of a table that the planning CTA counts itself (8 rows of 130 entries: a fork 14.4 -> 9.6 us on the device; a CTA takes
 // about 1 us a thousand entries, a launch and a memset 5 us).
 constexpr int kSmallTable = 4096;
@@ -87,7 +90,14 @@ __global__ void __launch_bounds__(256) fork_rows_kernel(PageTable t, const int* 
 __device__ __forceinline__ void count_here(const PageTable& t, const int* lens, const int* parents, int* out, int64_t out_stride, int* refs, int n, int* status) {
     for (int p = threadIdx.x; p < t.pages; p += blockDim.x) refs[p] = 0;
     __syncthreads();
-    for (int r = threadIdx.x >> 5; r < n; r += blockDim.x >> 5) go_on(t, lens, parents, out, out_stride, refs, r, threadIdx.x & 31, 32, status);
+    const int warps = blockDim.x >> 5, cols = t.width > 0 ? t.width : 1;
+    // a row a warp, whose parent and length are then found once; of more rows an entry a thread (8 rows of 130 entries 9.6 us, by entries
+    // 11.3; 512 rows of 8 entries 29 and 17)
+    if (n <= warps) {
+        if (threadIdx.x >> 5 < n) go_on(t, lens, parents, out, out_stride, refs, threadIdx.x >> 5, threadIdx.x & 31, 32, status);
+    } else {
+        for (int e = threadIdx.x; e < n * cols; e += blockDim.x) go_on(t, lens, parents, out, out_stride, refs, e / cols, e % cols, cols, status);
+    }
     __syncthreads();
 }
 
@@ -100,6 +110,7 @@ struct ForkPlan {
     int* copies;                // [n][3]: source page, target page, positions to copy
     int* n_copies;
     int* free_list;             // [pages] scratch
+    int *writers, *first;       // [pages] scratch: rows that go on writing in a begun page, the lowest of them
     int* status;
     int n, grow_all, pages;
     int count;                  // the table has not been copied and counted yet
@@ -139,17 +150,37 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkPlan 
         a.lens_out[r] = len + g;
     }
     __syncthreads();
+    const bool many = a.n > kSearchRows;
+    if (many) {
+        for (int r = threadIdx.x; r < a.n; r += blockDim.x)
+            if (const int page = last[r]; page >= 0) {
+                a.writers[page] = 0;
+                a.first[page] = a.n;
+            }
+        __syncthreads();
+        for (int r = threadIdx.x; r < a.n; r += blockDim.x)
+            if (const int page = last[r]; page >= 0) {
+                atomicAdd(a.writers + page, 1);
+                atomicMin(a.first + page, r);
+            }
+        __syncthreads();
+    }
     for (int r = threadIdx.x; r < a.n; r += blockDim.x) {
         const int page = last[r];
         if (page < 0) continue;
         const int held = a.refs[page];
         if (held <= 1) continue;
         int same = 0, first = 1;
-        for (int i = 0; i < a.n; ++i)
-            if (last[i] == page) {
-                ++same;
-                if (i < r) first = 0;
-            }
+        if (many) {
+            same = a.writers[page];
+            first = a.first[page] == r;
+        } else {
+            for (int i = 0; i < a.n; ++i)
+                if (last[i] == page) {
+                    ++same;
+                    if (i < r) first = 0;
+                }
+        }
         if (!(same == held && first)) fresh[r] += 1 + kCopy;     // only this thread reads or writes this entry
     }
     __syncthreads();
@@ -308,31 +339,39 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Compac
 }
 
 // Checks a caller's list of copies: pages that do not exist, a target that is also a source, a target given twice (the last one counts).
-__global__ void __launch_bounds__(256) copy_list_kernel(const int* src, const int* dst, int n, int pages, int* copies, int* status) {
+// One CTA marks sources and targets page by page, so that a list costs its length (1000 copies of 128 bytes 56 us where each copy looked
+// through the others).
+__global__ void __launch_bounds__(kPlanThreads) copy_list_kernel(const int* src, const int* dst, int n, int pages, int* copies, int* source, int* writer, int* status) {
     pdl_launch_dependents();
     pdl_wait();
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= n) return;
-    const int s = src[i], d = dst[i];
-    int fill = -1;
-    if (s < 0 || d < 0 || s == d) {
-        fill = 0;                                                // left out
-    } else if (s >= pages || d >= pages) {
-        latch(status, kStatusBadPage);
-        fill = 0;
-    } else {
-        for (int j = 0; j < n; ++j) {
-            const int sj = src[j], dj = dst[j];
-            if (sj < 0 || dj < 0 || sj == dj || j == i) continue;
-            if (sj == d || (dj == d && j > i)) {
-                latch(status, kStatusPageConflict);
-                fill = 0;
-            }
-        }
+    auto counts = [&](int s, int d) { return s >= 0 && d >= 0 && s != d; };
+    for (int i = threadIdx.x; i < n; i += blockDim.x)
+        for (const int p : {src[i], dst[i]})
+            if (p >= 0 && p < pages) source[p] = writer[p] = -1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const int s = src[i], d = dst[i];
+        if (!counts(s, d)) continue;
+        if (s < pages) source[s] = i;
+        if (d < pages) atomicMax(writer + d, i);
     }
-    copies[3 * i] = s;
-    copies[3 * i + 1] = d;
-    copies[3 * i + 2] = fill;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const int s = src[i], d = dst[i];
+        int fill = -1;
+        if (!counts(s, d)) {
+            fill = 0;                                                // left out
+        } else if (s >= pages || d >= pages) {
+            latch(status, kStatusBadPage);
+            fill = 0;
+        } else if (source[d] >= 0 || writer[d] > i) {
+            latch(status, kStatusPageConflict);
+            fill = 0;
+        }
+        copies[3 * i] = s;
+        copies[3 * i + 1] = d;
+        copies[3 * i + 2] = fill;
+    }
 }
 
 struct PageMove {
@@ -444,6 +483,7 @@ extern "C" int nexrt_page_fork(const NexrtPagesArgs* x, void* stream) {
     p.t = t; p.lens = static_cast<const int*>(x->lens); p.parents = static_cast<const int*>(x->parents); p.grow = static_cast<const int*>(x->grow);
     p.table = static_cast<int*>(x->table_out); p.table_stride = x->out_row; p.lens_out = static_cast<int*>(x->lens_out); p.refs = static_cast<int*>(x->refs);
     p.free_list = static_cast<int*>(x->scratch); p.copies = p.free_list + x->pages; p.n_copies = p.copies + 3 * x->rows_out;
+    p.writers = p.n_copies + 1; p.first = p.writers + x->pages;
     p.status = static_cast<int*>(x->status); p.n = x->rows_out; p.grow_all = x->grow_all; p.pages = x->pages; p.count = counts_here(*x, x->rows_out);
     // up to a row a warp few threads plan sooner, barriers are what it waits for: 8 rows 9.8 us, by 1024 threads 10.6 (24 rows 10.0 and 9.1)
     const bool few = x->rows_out <= 8 && x->pages <= 8 * kSmallTable;
@@ -478,8 +518,9 @@ extern "C" int nexrt_page_copy(const NexrtPagesArgs* x, void* stream) {
     if (n == 0) return 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     int* copies = static_cast<int*>(x->scratch);
-    if (const int e = launch(copy_list_kernel, dim3((n + 255) / 256), dim3(256), 0, st, static_cast<const int*>(x->table), static_cast<const int*>(x->lens), n, x->pages, copies,
-                             static_cast<int*>(x->status)))
+    int* source = copies + static_cast<int64_t>(3) * n;
+    if (const int e = launch(copy_list_kernel, dim3(1), dim3(n < kPlanThreads ? (n + 31) / 32 * 32 : kPlanThreads), 0, st, static_cast<const int*>(x->table),
+                             static_cast<const int*>(x->lens), n, x->pages, copies, source, source + x->pages, static_cast<int*>(x->status)))
         return e;
     PageMove m = {};
     m.copies = copies; m.n = n;

@@ -112,14 +112,25 @@ def _pool(what: str, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor):
     return base, (2 * shape[0], shape[2], shape[3], shape[4], slot, t_shape[0], t_shape[1]), t_s[0]
 
 
-def _fresh(what: str, name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor, *old: torch.Tensor) -> torch.Tensor:
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    """First byte and the one behind the last of an int32 list or table with contiguous rows."""
+    first, shape = t.data_ptr(), t.shape
+    if not t.numel():
+        return 0, 0
+    return first, first + 4 * (shape[0] if len(shape) == 1 else (shape[0] - 1) * t.stride()[0] + shape[1])
+
+
+def _fresh(what: str, name: str, t: Optional[torch.Tensor], shape, like: torch.Tensor, *old: Optional[torch.Tensor]) -> torch.Tensor:
     if t is None:
         return like.new_empty(*shape)        # (ints cost half of what a tuple does)
     if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or (t.numel() and t.stride(-1) != 1) or (t.dim() == 1 and not t.is_contiguous()):
         raise ValueError(f"{what}: {name} is int32 {list(shape)} with contiguous rows")
+    begin, end = _span(t)
     for o in old:
-        if o is not None and t.numel() and o.numel() and t.untyped_storage().data_ptr() == o.untyped_storage().data_ptr():
-            raise ValueError(f"{what}: {name} shares memory with an input: the rows are read while it is written")
+        if o is not None and end:
+            first, last = _span(o)
+            if begin < last and first < end:
+                raise ValueError(f"{what}: {name} shares memory with another argument: the rows are read while it is written")
     return t
 
 
@@ -132,7 +143,7 @@ def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent
     Full pages are shared.  A begun page that a growing row shares with others is copied, its written positions in all layers;
     where all its holders grow, the lowest row keeps it.  New pages are the lowest free ones, in the order of the rows.  A row for
     which there is no page, or no column in the table, keeps its length and latches ``NO_PAGES``; a page or parent that does not
-    exist latches ``BAD_PAGE``.  The outputs must not share memory with ``table`` or ``lens``."""
+    exist latches ``BAD_PAGE``.  The outputs must not share memory with the inputs."""
     what = "fork_pages"
     base, sizes, row = _pool(what, kv, table, lens)
     n, width, pages = parents.numel(), sizes[6], sizes[1]
@@ -144,12 +155,12 @@ def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent
     if each is None and not 0 <= grow < 2**31:
         raise ValueError(f"{what}: grow is not negative")
     check_status(what, status)
-    table_out = _fresh(what, "table_out", table_out, (n, width), table, table)
-    lens_out = _fresh(what, "lens_out", lens_out, (n,), table, lens, parents, each)
-    refs = _fresh(what, "refs", refs, (pages,), table, lens, parents, each, table)
+    table_out = _fresh(what, "table_out", table_out, (n, width), table, table, lens, parents, each)
+    lens_out = _fresh(what, "lens_out", lens_out, (n,), table, table, lens, parents, each, table_out)
+    refs = _fresh(what, "refs", refs, (pages,), table, table, lens, parents, each, table_out, lens_out)
     device = same_cuda_device(what, {kv.get_device(), table.get_device(), lens.get_device(), parents.get_device(), table_out.get_device(), lens_out.get_device(),
                                      refs.get_device()}, each, status)
-    scratch = table.new_empty(pages + 3 * n + 1)
+    scratch = table.new_empty(3 * pages + 3 * n + 1)
     on_device(device, lib().nexrt_page_fork, _PAGES.pack(
         _PAGES.size, base, table.data_ptr(), lens.data_ptr(), parents.data_ptr(), address(each), table_out.data_ptr(), lens_out.data_ptr(), refs.data_ptr(), 0, 0,
         scratch.data_ptr(), address(status), row, table_out.stride()[0], *sizes, n, 0 if each is not None else grow, 0), what)
@@ -165,8 +176,8 @@ def compact_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, 
     base, sizes, row = _pool(what, kv, table, lens)
     pages = sizes[1]
     check_status(what, status)
-    table_out = _fresh(what, "table_out", table_out, tuple(table.shape), table, table)
-    refs = _fresh(what, "refs", refs, (pages,), table, lens, table)
+    table_out = _fresh(what, "table_out", table_out, tuple(table.shape), table, table, lens)
+    refs = _fresh(what, "refs", refs, (pages,), table, lens, table, table_out)
     remap, live = table.new_empty(pages), table.new_empty(1)
     device = same_cuda_device(what, {kv.get_device(), table.get_device(), lens.get_device(), table_out.get_device(), refs.get_device()}, status)
     scratch = table.new_empty(5 * pages + 1)
@@ -186,7 +197,7 @@ def copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *, status
     base, sizes, _ = _pool(what, kv, src.view(-1, 1), src)
     check_status(what, status)
     device = same_cuda_device(what, {kv.get_device(), src.get_device(), dst.get_device()}, status)
-    scratch = src.new_empty(3 * src.numel())
+    scratch = src.new_empty(3 * src.numel() + 2 * sizes[1])
     on_device(device, lib().nexrt_page_copy, _PAGES.pack(_PAGES.size, base, src.data_ptr(), dst.data_ptr(), 0, 0, 0, 0, 0, 0, 0, scratch.data_ptr(), address(status), 1, 0, *sizes, 0, 0, 0), what)
 
 
@@ -227,7 +238,7 @@ class PagedCache:
             raise ValueError("PagedCache.load_kv: k and v are [kv heads, positions, dim] for a row of the cache")
         k, v = k.transpose(0, 1), v.transpose(0, 1)
         at = torch.arange(k.shape[0], dtype=I32, device=k.device)
-        self.append(layer, k[:, :0], k, v, at, torch.full_like(at, row), torch.empty(0, device=k.device))
+        self.append(layer, k[:, :0], k, v, at, torch.full_like(at, row), torch.empty(0, dtype=F32, device=k.device))
 
     def attend(self, layer: int, q: torch.Tensor, **how) -> torch.Tensor:
         return paged_attention(q, self.kv[layer, 0], self.kv[layer, 1], self.table, self.lens, status=self.status, **how)

@@ -109,6 +109,45 @@ def test_fork_of_many_rows_and_a_wide_table():
     assert t.tolist() == want[1] and l.tolist() == want[2] and refs.tolist() == want[3] and torch.equal(kv, want[0])
 
 
+@pytest.mark.parametrize("rows,width", [(9, 7), (33, 3), (256, 3), (257, 3), (700, 5), (700, 9)])
+def test_begun_pages_that_many_rows_hold(rows, width):
+    """Groups of rows on one begun page, all of which write on, or some; tables that the planning kernel counts itself, by rows and by entries, and
+    one that it does not."""
+    r = random.Random(rows + width)
+    page, table, lens, at = 4, [], [], 0
+    while len(table) < rows:
+        n = r.choice([0, 3, page, page + 1, 2 * page + 3])
+        used, many = -(-n // page), min(r.choice([1, 2, 40]), rows - len(table))
+        table += [list(range(at, at + used)) + [-1] * (width - used)] * many
+        lens += [n] * many
+        at += used
+    pages = at + 2 * rows
+    kv = torch.randint(-100, 100, (1, 2, pages, 1, page, 16), device=DEV).to(torch.int8)
+    for grow in ([1] * rows, [r.choice([0, 1, 1, 2]) for _ in range(rows)]):
+        a = kv.clone()
+        want = fork_in_python(a, table, lens, list(range(rows)), grow, page)
+        status = ints([0])
+        t, l, refs = fork_pages(a, ints(table), ints(lens), ints(range(rows)), ints(grow), status=status)
+        assert t.tolist() == want[1] and l.tolist() == want[2] and refs.tolist() == want[3] and torch.equal(a, want[0])
+        assert int(status) == (Status.NO_PAGES if want[4] else 0)
+
+
+def test_outputs_beside_the_inputs_in_one_allocation():
+    """Disjoint parts of one buffer are outputs like any others."""
+    kv = torch.zeros(1, 2, 8, 1, 4, 64, dtype=torch.bfloat16, device=DEV)
+    work = torch.full((40,), -7, dtype=torch.int32, device=DEV)
+    table, lens, out, lens_out, refs = work[:4].view(2, 2), work[4:6], work[6:10].view(2, 2), work[10:12], work[12:20]
+    table.copy_(ints([[3, 5], [-1, -1]]))
+    lens.copy_(ints([6, 0]))
+    fork_pages(kv, table, lens, ints([0, 0]), 0, table_out=out, lens_out=lens_out, refs=refs)
+    assert work[:22].tolist() == [3, 5, -1, -1, 6, 0, 3, 5, 3, 5, 6, 6, 0, 0, 0, 2, 0, 2, 0, 0, -7, -7]
+    compact_pages(kv, out, lens_out, table_out=table, refs=refs)
+    assert table.tolist() == [[0, 1], [0, 1]]
+    for bad in (dict(table_out=work[2:6].view(2, 2)), dict(lens_out=work[5:7]), dict(refs=work[5:13]), dict(lens_out=work[20:22], refs=work[21:29])):
+        with pytest.raises(ValueError, match="shares memory"):
+            fork_pages(kv, table, lens, ints([0, 0]), 0, **bad)
+
+
 def test_fork_reports_and_survives_bad_input():
     kv = torch.zeros(1, 2, 6, 1, 4, 64, dtype=torch.bfloat16, device=DEV)
 
@@ -185,6 +224,30 @@ def test_copy_pages():
     want[:, :, 42], want[:, :, 41] = kv[:, :, 40], kv[:, :, 5]
     assert code == Status.PAGE_CONFLICT and torch.equal(a, want)
     assert torch.equal(run([], [])[0], kv)
+
+
+@pytest.mark.parametrize("n", [31, 1000, 1025, 6000])
+def test_long_lists_of_copies(n):
+    """Sources and targets at random, some of them both, given twice, left out or beyond the pool."""
+    r = random.Random(n)
+    pages = 3 * n
+    src = [r.choice([r.randrange(n), r.randrange(n), r.randrange(pages), -1, pages + r.randrange(3)]) if r.random() < 0.3 else r.randrange(n) for _ in range(n)]
+    dst = [r.choice([r.randrange(n), -2, pages]) if r.random() < 0.1 else n + r.randrange(2 * n) for _ in range(n)]
+    src[5] = dst[5] = 7
+    kv = torch.randint(-100, 100, (1, 2, pages, 1, 1, 16), device=DEV).to(torch.int8)
+    want, told = kv.clone(), set()
+    pairs = [(s, d) for s, d in zip(src, dst) if s >= 0 and d >= 0 and s != d]
+    sources, last = {s for s, _ in pairs}, {d: i for i, (_, d) in enumerate(pairs)}
+    for i, (s, d) in enumerate(pairs):
+        if s >= pages or d >= pages:
+            told.add(Status.BAD_PAGE)
+        elif d in sources or last[d] != i:
+            told.add(Status.PAGE_CONFLICT)
+        else:
+            want[:, :, d] = kv[:, :, s]
+    status = ints([0])
+    copy_pages(kv, ints(src), ints(dst), status=status)
+    assert torch.equal(kv, want) and int(status) in (told or {0})
 
 
 def test_offsets_beyond_32_bits():
@@ -295,3 +358,18 @@ def test_an_engine_prefill_becomes_rows_of_a_cache():
         assert torch.all((got.float() - want.float()).abs() <= 2.0**-7 * want.float().abs() + 2.0**-10)
     with pytest.raises(ValueError):
         cache.load_kv(0, 3, full[0]["k_cache"], full[0]["v_cache"])
+
+
+def test_load_kv_under_another_default_type():
+    cache = PagedCache(1, 4, 1, 4, 64, 1, 8)
+    k = torch.randn(1, 6, 64, device=DEV).to(torch.bfloat16)
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        cache.fork(grow=6)
+        cache.load_kv(0, 0, k, -k)
+    finally:
+        torch.set_default_dtype(before)
+    cache.check()
+    got = cache.kv[0][:, cache.table[0].long()].reshape(2, 8, 64)[:, :6]
+    assert torch.equal(got[0], k[0]) and torch.equal(got[1], -k[0])
