@@ -95,6 +95,16 @@ def test_append(src, dst, hq, hk, dim, rotary, page, interleaved):
     assert torch.equal(kv[keep], before[keep])                                     # all else is as it was
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dim", [16, 48, 80, 96, 112, 144, 192, 240])
+def test_all_dims_turned_of_heads_that_fill_no_power_of_two(dtype, dim):
+    test_rope_alone(dtype, 67, 5, dim, dim, False)
+    test_rope_alone(dtype, 3, 2, dim, dim, True)
+    if dtype != torch.float32:
+        test_append(dtype, dtype, 6, 2, dim, dim, 5, False)
+        test_append(torch.float32, dtype, 1, 3, dim, dim, 16, False)
+
+
 def test_append_leaves_out_what_has_no_page():
     table = torch.tensor([[2, -1, 9, 1]], dtype=torch.int32, device=DEV)           # no page, a page that the pool does not have
     kv = torch.zeros(2, 3, 1, 4, 64, dtype=torch.bfloat16, device=DEV)
