@@ -2,8 +2,10 @@
 //
 //   total(beam, token) = score(beam) + logit(beam, token) - log sum exp of the beam's logits
 //
-// in 64 bits, so that beams whose totals are near each other keep their order; equal totals go to the lower beam, then to the
-// larger logit, then to the lower token.  A finished beam has one candidate, its end token at its own score.
+// in 64 bits; equal totals go to the lower beam, then to the larger logit, then to the lower token.  A finished beam has one candidate, its
+// end token at its own score.  What is not 64 bits are the exponentials and the sums of 16 or 32 of them: a row's logarithm is off by up to
+// 2^-20, by 1e-7 as a rule, and beams whose totals are nearer than that may change places.  Beams that hold the same numbers tie to the
+// last bit: which values meet in a partial sum goes by their tokens, never by the address of the row.
 //
 // Within a beam the order of the totals is that of the logits, so one pass over a slice of a row gives everything that is
 // needed of it: its maximum, its sum of exp and its k largest logits.  A CTA walks its slice in steps of 16 KB, 64 bytes a thread in
@@ -111,9 +113,9 @@ template <typename T> struct Piece {
         else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
         else return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w[i / 2] >> 16 : w[i / 2])));
     }
-    __device__ __forceinline__ void operator=(const uint4& v) { w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
-    __device__ __forceinline__ void clear() {          // to -infinity
-        w[0] = w[1] = w[2] = w[3] = sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __nv_bfloat16>::value ? 0xff80ff80u : 0xfc00fc00u);
+    static __device__ __forceinline__ uint4 nothing() {          // -infinity throughout
+        constexpr uint32_t low = sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __nv_bfloat16>::value ? 0xff80ff80u : 0xfc00fc00u);
+        return make_uint4(low, low, low, low);
     }
     // value(i) of an i that is not known when this is compiled
     __device__ __forceinline__ float value_at(int i) const {
@@ -164,26 +166,33 @@ template <typename T> struct Piece {
     }
 };
 
-// The piece at value `at` of a row where it reaches over an end of it, -infinity outside.  Out of line: a row has two of them at most.
-template <typename T> __device__ __noinline__ uint4 edge_piece(const T* base, int at, int vocab) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) {
-            w[i] = at + i >= 0 && at + i < vocab ? reinterpret_cast<const uint32_t*>(base)[at + i] : 0xff800000u;
-        } else {
-            const uint32_t low = std::is_same<T, __nv_bfloat16>::value ? 0xff80u : 0xfc00u;
-            const unsigned short* p = reinterpret_cast<const unsigned short*>(base);
-            const int j = at + 2 * i;
-            w[i] = (j >= 0 && j < vocab ? p[j] : low) | (j + 1 >= 0 && j + 1 < vocab ? p[j + 1] : low) << 16;
-        }
+// The word at value `at` of a row where it may reach over an end of it, -infinity outside.
+template <typename T> __device__ __forceinline__ uint32_t edge_word(const T* base, int at, int vocab) {
+    if constexpr (sizeof(T) == 4) {
+        return at >= 0 && at < vocab ? reinterpret_cast<const uint32_t*>(base)[at] : 0xff800000u;
+    } else {
+        const uint32_t low = std::is_same<T, __nv_bfloat16>::value ? 0xff80u : 0xfc00u;
+        const unsigned short* p = reinterpret_cast<const unsigned short*>(base);
+        return (at >= 0 && at < vocab ? p[at] : low) | (at + 1 >= 0 && at + 1 < vocab ? p[at + 1] : low) << 16;
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Four of them.  Out of line: a row has two such pieces at most.
+template <typename T> __device__ __noinline__ uint4 edge_piece(const T* base, int at, int vocab) {
+    constexpr int PER = 4 / sizeof(T);
+    return make_uint4(edge_word(base, at, vocab), edge_word(base, at + PER, vocab), edge_word(base, at + 2 * PER, vocab), edge_word(base, at + 3 * PER, vocab));
+}
+__device__ __forceinline__ uint32_t ld_word(const void* p) {     // (a line serves several such loads: it may stay in L1)
+    uint32_t v;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
 }
 
-template <typename T>
+// ALIGNED: every row starts on a 16-byte boundary and is read 16 bytes at a time.  Else by words, so that a thread has the same values wherever its
+// row starts (128 rows of 248320 or 248321 values: bf16 31.3 and 35.3 us, fp32 39.4 and 41.7).
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const BeamArgs a) {
-    constexpr int VEC = Piece<T>::kValues, NV = kPieces, kWarps = kSliceThreads / 32;
+    constexpr int VEC = Piece<T>::kValues, NV = kPieces, kWarps = kSliceThreads / 32, PER = 4 / sizeof(T);
+    constexpr int WORDS = ALIGNED || PER == 1 ? 4 : 5;                 // of a piece: one of 16-bit values that starts in the middle of a word touches five
     __shared__ float group_top[kBeamGroups], warp_top[kWarps];
     __shared__ double warp_part[kWarps];
     __shared__ u64 keep[kBeamKeep];
@@ -196,12 +205,12 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
     const int row = blockIdx.y, slice = blockIdx.x, b = row / a.beams, w = row - b * a.beams;
     const bool closed = beam_is_closed(a, b, w);        // looked at when the first loads are on their way
     const T* base = static_cast<const T*>(a.logits) + b * a.l_b + w * a.l_w;
-    // the row in 16-byte pieces: piece c holds values [c VEC - off, (c + 1) VEC - off)
-    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(base) / sizeof(T) % VEC);
-    const int pieces = (a.vocab + off + VEC - 1) / VEC;
+    // the row in pieces of 16 bytes: piece c holds values [c VEC, (c + 1) VEC)
+    const int pieces = (a.vocab + VEC - 1) / VEC;
+    const int odd = WORDS == 5 ? static_cast<int>(reinterpret_cast<uintptr_t>(base) >> 1 & 1) : 0;     // the row starts in the middle of a word
     // a slice is whole steps: only a row's last one is ragged
     const int steps = (pieces + kSliceThreads * NV - 1) / (kSliceThreads * NV);
-    const unsigned int slices = a.slices;                              // (no more than there are steps, at most 4097: 32 bits will do)
+    const unsigned int slices = a.slices;                              // (no more than there are steps, at most 4096: 32 bits will do)
     const int lo = static_cast<int>(static_cast<unsigned int>(steps * slice) / slices) * kSliceThreads * NV;
     const int hi = min(pieces, static_cast<int>(static_cast<unsigned int>(steps * (slice + 1)) / slices) * kSliceThreads * NV);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -213,21 +222,33 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
     float top = -INFINITY, bound = 0.f;
     double sum = 0.0;
     bool over = false;                  // more candidates than there is room for
-    Piece<T> ahead[NV];                 // the next step's pieces are on their way while a step is worked on
-    const int full0 = off ? 1 : 0, full1 = (a.vocab + off) / VEC;      // pieces that lie in the row entirely
-    auto fetch = [&](int p0) {
-        if (p0 >= full0 && p0 + kSliceThreads * NV <= min(hi, full1)) {
-            const T* from = base + (static_cast<int64_t>(p0 + threadIdx.x) * VEC - off);
+    uint32_t ahead[NV][WORDS];          // the next step's pieces are on their way while a step is worked on
+    auto load = [&](uint32_t (&to)[WORDS], const T* from) {
+        if constexpr (ALIGNED) {
+            const uint4 v = ld_stream16(from);
+            to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+        } else {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) ahead[j] = ld_stream16(from + j * kSliceThreads * VEC);
+            for (int i = 0; i < WORDS; ++i) to[i] = ld_word(from + i * PER);
+        }
+    };
+    auto fetch = [&](int p0) {
+        if (p0 >= odd && (p0 + kSliceThreads * NV) * VEC + (WORDS - 4) * PER - odd <= a.vocab) {
+            const T* from = base + (static_cast<int64_t>(p0 + threadIdx.x) * VEC - odd);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) load(ahead[j], from + j * kSliceThreads * VEC);
             return;
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = p0 + j * kSliceThreads + threadIdx.x, at = c * VEC - off;
-            if (c < hi && at >= 0 && at + VEC <= a.vocab) ahead[j] = ld_stream16(base + at);
-            else if (c < hi) ahead[j] = edge_piece(base, at, a.vocab);
-            else ahead[j].clear();
+            const int at = (p0 + j * kSliceThreads + static_cast<int>(threadIdx.x)) * VEC - odd;
+            if (at >= 0 && at + WORDS * PER <= a.vocab) {
+                load(ahead[j], base + at);
+            } else {
+                const uint4 v = at + odd < a.vocab ? edge_piece(base, at, a.vocab) : Piece<T>::nothing();
+                ahead[j][0] = v.x; ahead[j][1] = v.y; ahead[j][2] = v.z; ahead[j][3] = v.w;
+                if constexpr (WORDS == 5) ahead[j][4] = edge_word(base, at + 4 * PER, a.vocab);
+            }
         }
     };
     fetch(lo);
@@ -236,7 +257,12 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
     for (int p0 = lo; p0 < hi; p0 += kSliceThreads * NV, ++step) {
         Piece<T> x[NV];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) x[j] = ahead[j];
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (WORDS == 5) x[j].w[i] = __funnelshift_r(ahead[j][i], ahead[j][i + 1], odd * 16);
+                else x[j].w[i] = ahead[j][i];
+            }
         if (p0 + kSliceThreads * NV < hi) fetch(p0 + kSliceThreads * NV);
         float piece_top[NV], new_top = top;
 #pragma unroll
@@ -291,11 +317,11 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (piece_top[j] >= bound) {
-                const int first = (p0 + j * kSliceThreads + static_cast<int>(threadIdx.x)) * VEC - off, end = min(a.vocab, hi * VEC - off);
+                const int first = (p0 + j * kSliceThreads + static_cast<int>(threadIdx.x)) * VEC;
 #pragma unroll 1
                 for (uint32_t there = x[j].at_least(bound); there; there &= there - 1) {
                     const int i = __ffs(there) - 1, token = first + i;
-                    if (token < 0 || token >= end) continue;
+                    if (token >= a.vocab) continue;
                     const float v = x[j].value_at(i);
                     const int to = atomicAdd(&count_s, 1);
                     if (to < kBeamKeep) keep[to] = (static_cast<u64>(ord32(v)) << 32) | static_cast<unsigned int>(~token);
@@ -359,11 +385,11 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
         a.sums[at_slice] = t;
         a.tops[at_slice] = m;
     }
-    const int first = max(lo * VEC - off, 0), last = min(hi * VEC - off, a.vocab);
+    const int first = lo * VEC, last = min(hi * VEC, a.vocab);
     if (tied_s) {
         // of the first step's values equal to its bound the k lowest tokens
         const float equal = equal_s;
-        const int end = min(last, (lo + kSliceThreads * NV) * VEC - off);
+        const int end = min(last, (lo + kSliceThreads * NV) * VEC);
         for (int t0 = first, taken = 0; t0 < end && taken < a.k; t0 += kSliceThreads) {
             const int token = t0 + threadIdx.x;
             const bool here = token < end && static_cast<float>(base[token]) == equal;
@@ -409,6 +435,11 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
     }
     __syncthreads();
     for (int i = count_s + threadIdx.x; i < a.k; i += kSliceThreads) out[i] = 0;
+}
+
+template <typename T> static int slice_launch(const BeamArgs& a, bool aligned, cudaStream_t st) {
+    const dim3 grid(a.slices, a.batch * a.beams), block(kSliceThreads);
+    return aligned ? launch(beam_slice_kernel<T, true>, grid, block, 0, st, a) : launch(beam_slice_kernel<T, false>, grid, block, 0, st, a);
 }
 
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamArgs a) {
@@ -664,7 +695,7 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
 // and many beams no more of them than it reads in a few microseconds (8 beams of 248320, k = 64: 61 slices 80 us, 16 slices 39).
 constexpr int kJoinMost = 8192;
 static int beam_slices(int rows, int beams, int vocab, int k, int type) {
-    const int64_t bytes = (static_cast<int64_t>(vocab) + 8) * (type == 2 ? 4 : 2);
+    const int64_t bytes = static_cast<int64_t>(vocab) * (type == 2 ? 4 : 2);
     const int most = static_cast<int>((bytes + kStepBytes - 1) / kStepBytes), wave = 8 * sm_count() / (rows > 0 ? rows : 1), join = kJoinMost / (beams * k);
     const int share = wave < join ? wave : join;
     return share < 1 ? 1 : (share < most ? share : most);
@@ -694,9 +725,9 @@ extern "C" int nexrt_beam_select(const NexrtBeamArgs* x, void* stream) {
     a.scores_out = static_cast<float*>(x->scores_out); a.rows_out = static_cast<int*>(x->rows_out); a.tokens_out = static_cast<int*>(x->tokens_out);
     a.status = static_cast<int*>(x->status);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const dim3 grid(a.slices, a.batch * a.beams), block(kSliceThreads);
-    const int e = x->type == 0 ? launch(beam_slice_kernel<__nv_bfloat16>, grid, block, 0, st, a)
-                               : (x->type == 1 ? launch(beam_slice_kernel<__half>, grid, block, 0, st, a) : launch(beam_slice_kernel<float>, grid, block, 0, st, a));
+    const int64_t size = x->type == 2 ? 4 : 2, strides = (x->batch > 1 ? x->logits_request : 0) | (x->beams > 1 ? x->logits_beam : 0);
+    const bool aligned = ((reinterpret_cast<uintptr_t>(x->logits) | static_cast<uintptr_t>(strides * size)) & 15) == 0;
+    const int e = x->type == 0 ? slice_launch<__nv_bfloat16>(a, aligned, st) : (x->type == 1 ? slice_launch<__half>(a, aligned, st) : slice_launch<float>(a, aligned, st));
     if (e) return e;
     return launch(beam_join_kernel, dim3(a.batch), dim3(kJoinThreads), 0, st, a);
 }

@@ -316,3 +316,35 @@ def test_a_captured_beam_step_goes_on_like_an_eager_one():
     a.cache.check()
     b.cache.check()
     assert a.cache.lens.tolist() == [21] * W + [0] and torch.equal(a.cache.kv, b.cache.kv)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [501, 1001, 4098, 50257, 131075])
+def test_equal_beams_of_any_alignment_tie(dtype, V):
+    """Rows of an odd vocabulary start anywhere between two 16-byte boundaries.  Beams that hold the same numbers have the same totals to the last bit
+    all the same, so the lower beam goes first; and a row's totals do not go by its address."""
+    one = inputs(1, 1, V, dtype, seed=1)[0]
+    x, s = one.expand(2, 9, V).contiguous(), torch.full((2, 9), -1.5, device=DEV)
+    scores, rows, tokens = beam_select(x, s, 20)
+    logits, at = torch.sort(one[0, 0].float(), descending=True, stable=True)
+    want = sorted((-v, w, t) for v, t in zip(logits[:40].tolist(), at[:40].tolist()) for w in range(9))[:20]
+    for b in range(2):
+        assert list(zip(rows[b].tolist(), tokens[b].tolist())) == [(w + 9 * b, t) for _, w, t in want]
+        assert len(set(scores[b].tolist())) == len({v for v, _, _ in want})
+    totals = []
+    for off in range(8):
+        wide = torch.zeros(V + 8, device=DEV, dtype=dtype)
+        wide[off : off + V] = one[0, 0]
+        totals.append(beam_select(wide[off : off + V].view(1, 1, V), s[:1, :1], 20)[0])
+    assert all(torch.equal(t, totals[0]) for t in totals)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("off", range(1, 8))
+@pytest.mark.parametrize("V", [1, 6, 8, 13, 4093, 4096, 8192, 16384 + 5, 33000])
+def test_rows_at_every_start(dtype, off, V):
+    """Vocabularies that end in, at and behind a step, between neighbours that must not be read as logits."""
+    x, s = inputs(1, 1, V, dtype, seed=off)
+    wide = torch.full((V + 16,), 1000.0, device=DEV, dtype=dtype)
+    wide[off : off + V] = x[0, 0]
+    check(wide[off : off + V].view(1, 1, V), s, min(V, 12))
