@@ -206,7 +206,7 @@ int nexrt_tc_oproj_allreduce(const void* planes, const void* descale, const void
 int nexrt_attn_front_tail(const void* pre, const void* ctl, void* q_raw, void* gate, void* k_raw, void* v_cache, int hd, int nq, int ngate, int kvh, int M,
                           int cache_len, int ksplit, void* stream);   /* pre: [ksplit][M][R] partial planes of a chunk's GEMM */
 
-// ---- a key-value cache in pages, shared by several sequences (rope.cu, paged_attn.cu, pages.cu) -------------------------
+// ---- a key-value cache in pages, shared by several sequences (rope.cu, paged_attn.cuh, pages.cu) ------------------------
 // These entry points take their arguments as one block (ops/rope.py, ops/paged.py and ops/beam.py pack it; `size` is that of the block
 // and checked).  Pools: [pages][kv heads][slots][dim], one for K and one for V of every layer; table: int32 [rows][width], -1 where
 // there is no page.  Types: 0 bf16, 1 fp16, 2 fp32.  Strides count elements.  A bad page or row is left out and latches kStatusBadPage

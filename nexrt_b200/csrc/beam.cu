@@ -278,9 +278,9 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
 #pragma unroll
             for (int i = 0; i < VEC; i += 2) {
                 const float2 e = mul2(add2(make_float2(x[j].value(i), x[j].value(i + 1)), minus), log2e);
-                part = add2(part, make_float2(exp2_down(e.x), exp2_down(e.y)));
+                part = add2(part, make_float2(exp2_ftz(e.x), exp2_ftz(e.y)));
             }
-        sum = fma(sum, static_cast<double>(exp2_down((top - shift) * 1.4426950408889634f)), static_cast<double>(part.x + part.y));
+        sum = fma(sum, static_cast<double>(exp2_ftz((top - shift) * 1.4426950408889634f)), static_cast<double>(part.x + part.y));
         top = new_top;
         if (p0 == lo) {
             // the k-th largest maximum of 64 groups of lanes (of 128 for many beams) bounds the k-th largest value of the slice from below
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
     float all = top;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-    if (top != all && top > -INFINITY) sum *= exp2_down((top - all) * 1.4426950408889634f);
+    if (top != all && top > -INFINITY) sum *= exp2_ftz((top - all) * 1.4426950408889634f);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) {
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kSliceThreads, 4) beam_slice_kernel(const Beam
         for (int i = 1; i < kWarps; ++i) m = fmaxf(m, warp_top[i]);
         double t = 0.0;
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) t += warp_top[i] == m || warp_top[i] == -INFINITY ? warp_part[i] : warp_part[i] * exp2_down((warp_top[i] - m) * 1.4426950408889634f);
+        for (int i = 0; i < kWarps; ++i) t += warp_top[i] == m || warp_top[i] == -INFINITY ? warp_part[i] : warp_part[i] * exp2_ftz((warp_top[i] - m) * 1.4426950408889634f);
         a.sums[at_slice] = t;
         a.tops[at_slice] = m;
     }
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamArgs 
                     ms = a.tops[at + s];
                     part = a.sums[at + s];
                 }
-                sum += ms == m ? part : part * static_cast<double>(exp2_down((ms - m) * 1.4426950408889634f));
+                sum += ms == m ? part : part * static_cast<double>(exp2_ftz((ms - m) * 1.4426950408889634f));
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);

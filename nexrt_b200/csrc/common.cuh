@@ -193,8 +193,8 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return r;
 }
 
-// 2^x for x <= 0, to 2^-22 of the value; below 2^-126 zero
-__device__ __forceinline__ float exp2_down(float x) {
+// 2^x, to 2^-22 of the value; below 2^-126 zero
+__device__ __forceinline__ float exp2_ftz(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;

@@ -1,4 +1,4 @@
-"""A key-value cache in pages that several sequences share (``csrc/paged_attn.cu``, ``csrc/pages.cu``).
+"""A key-value cache in pages that several sequences share (``csrc/paged_attn.cuh``, ``csrc/pages.cu``).
 
 The engine's own cache (``attn.py: FullAttn``) is one contiguous block for one sequence.  Here the keys and values of a batch lie
 in a pool of pages: ``kv [layers, 2, pages, kv heads, slots, dim]`` (K and V of every layer), and ``table`` int32 ``[rows, width]``

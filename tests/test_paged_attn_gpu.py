@@ -235,3 +235,55 @@ def test_two_streams_at_once():
                 got[i].append(paged_attention(q, kv[0], kv[1], table, lens))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gap", [5.0, 10.0, 17.0, 25.0, 30.0])
+@pytest.mark.parametrize("hq,dim,page", [(4, 64, 16), (12, 128, 40), (1, 256, 64), (16, 192, 16)])
+def test_a_key_that_outweighs_all_others(dtype, gap, hq, dim, page):
+    """One key of a row, the first, one in the middle, the last, with a value of zero (an attention sink): the result is what the others weigh, however
+    little that is.  Values are large, so that the result is a number that fp16 holds."""
+    lens = [3000, 2999, 70, 800]
+    q, kv, table, n = build(lens, hq, 1, dim, page, dtype, seed=5)
+    q.zero_()
+    q[..., 0] = 4 * dim**0.5                                                   # scores are 4 K[0]: about N(0, 1)
+    kv[0, ..., 0] *= 0.25
+    kv[1] = (kv[1].abs().clamp(max=2.0) + 0.5) * 2.0**13
+    for b, j in ((0, 0), (1, 1500), (2, 69), (3, 17)):
+        kv[0, table[b, j // page].long(), 0, j % page, 0] = gap / 4
+        kv[1, table[b, j // page].long(), 0, j % page] = 0.0
+    out, lse = paged_attention(q, kv[0], kv[1], table, n, return_lse=True)
+    check(out, lse, formula(q, kv, table, n))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rise", [1, -1])
+def test_scores_that_rise_and_fall_through_their_range(dtype, rise):
+    """Scores from 0 to 200 from key to key, upwards and downwards, and back and forth between 0 and 40 from tile to tile: what a weight is formed against moves all the time."""
+    q, kv, table, n = build([2000, 1111], 3, 1, 128, 16, dtype, seed=9)
+    q.zero_()
+    q[..., 0] = 4 * 128**0.5
+    ramp = torch.arange(2000, device=DEV) / 40.0
+    for b, x in ((0, ramp if rise > 0 else ramp.flip(0)), (1, 10.0 * (torch.arange(2000, device=DEV) // 16 % 2))):
+        for j in range(int(n[b])):
+            kv[0, table[b, j // 16].long(), 0, j % 16, 0] = x[j]
+    out, lse = paged_attention(q, kv[0], kv[1], table, n, return_lse=True)
+    check(out, lse, formula(q, kv, table, n))
+
+
+@pytest.mark.parametrize("keys", [40, 3000])
+def test_infinities_and_nan_in_fp16(keys):
+    q, kv, table, lens = build([keys] * 5, 4, 1, 64, 16, torch.float16, seed=1)
+    q = q.abs() + 0.1
+    kv[0][table[0, : -(-keys // 16)].long()] = -math.inf                       # every score -inf: nothing is seen
+    kv[0][table[1, 0].long(), 0, 3] = -math.inf                                # one of them: the key drops out
+    q[2] = math.nan
+    kv[0][table[3, 1].long(), 0, 5, 7] = math.nan
+    kv[0][table[4, 1].long(), 0, 5] = math.inf                                 # inf - inf
+    out, lse = paged_attention(q, kv[0], kv[1], table, lens, return_lse=True)
+    assert not out[0].any() and torch.all(lse[0] == -math.inf)
+    clean = kv.clone()
+    clean[0][table[1, 0].long(), 0, 3] = -30000.0
+    want = formula(q[1:2], clean, table[1:2], lens[1:2])
+    check(out[1:2], lse[1:2], want[:2] + formula(q[1:2], kv.nan_to_num(neginf=0.0, posinf=0.0), table[1:2], lens[1:2])[2:])
+    assert torch.isnan(out[2:]).all() and torch.isnan(lse[2:]).all()
