@@ -241,7 +241,7 @@ typedef struct NexrtPagesArgs {
     uint64_t size;
     void* pool;
     const void *table, *lens, *parents, *grow;        /* parents, grow: of a fork; grow NULL: grow_all for all rows */
-    void *table_out, *lens_out, *refs, *remap, *live, *scratch, *status;
+    void *table_out, *lens_out, *refs, *remap, *live, *scratch, *status, *grown;   /* grown: of a fork, may be NULL */
     int64_t table_row, out_row;
     int planes, pages, heads, slots, slot_bytes, rows, width, rows_out, grow_all, reserved;
 } NexrtPagesArgs;

@@ -112,6 +112,7 @@ struct ForkPlan {
     int* free_list;             // [pages] scratch
     int *writers, *first;       // [pages] scratch: rows that go on writing in a begun page, the lowest of them
     int* status;
+    int* grown;                 // may be null: the row where it got its positions, else -1
     int n, grow_all, pages;
     int count;                  // the table has not been copied and counted yet
 };
@@ -148,6 +149,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkPlan 
         last[r] = open;
         fresh[r] = want;
         a.lens_out[r] = len + g;
+        if (a.grown) a.grown[r] = g > 0 ? r : -1;
     }
     __syncthreads();
     const bool many = a.n > kSearchRows;
@@ -221,6 +223,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkPlan 
         if (k > 0 && at + k > found) {
             latch(a.status, kStatusNoPages);                     // the pool is full: the row keeps what it has and does not grow
             a.lens_out[r] = len;
+            if (a.grown) a.grown[r] = -1;
         } else if (k > 0) {
             int* row = a.table + r * a.table_stride;
             int used = pages_of(len, a.t.page), i = 0;
@@ -484,7 +487,7 @@ extern "C" int nexrt_page_fork(const NexrtPagesArgs* x, void* stream) {
     p.table = static_cast<int*>(x->table_out); p.table_stride = x->out_row; p.lens_out = static_cast<int*>(x->lens_out); p.refs = static_cast<int*>(x->refs);
     p.free_list = static_cast<int*>(x->scratch); p.copies = p.free_list + x->pages; p.n_copies = p.copies + 3 * x->rows_out;
     p.writers = p.n_copies + 1; p.first = p.writers + x->pages;
-    p.status = static_cast<int*>(x->status); p.n = x->rows_out; p.grow_all = x->grow_all; p.pages = x->pages; p.count = counts_here(*x, x->rows_out);
+    p.status = static_cast<int*>(x->status); p.grown = static_cast<int*>(x->grown); p.n = x->rows_out; p.grow_all = x->grow_all; p.pages = x->pages; p.count = counts_here(*x, x->rows_out);
     // up to a row a warp few threads plan sooner, barriers are what it waits for: 8 rows 9.8 us, by 1024 threads 10.6 (24 rows 10.0 and 9.1)
     const bool few = x->rows_out <= 8 && x->pages <= 8 * kSmallTable;
     if (const int e = launch(fork_plan_kernel, dim3(1), dim3(few ? 256 : kPlanThreads), sizeof(int) * 2 * x->rows_out, st, p)) return e;

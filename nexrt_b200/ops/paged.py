@@ -27,7 +27,7 @@ MAX_ROWS = 4096
 _CHUNK = 64                                     # keys of a unit of the attention's work, and what an item counts beside them
 _ITEM_COST = 3
 _ATTN = struct.Struct("Q10P9q10i2f")            # NexrtPagedAttnArgs
-_PAGES = struct.Struct("Q12P2q10i")             # NexrtPagesArgs
+_PAGES = struct.Struct("Q13P2q10i")             # NexrtPagesArgs
 _POOL_TYPES = (torch.bfloat16, torch.float16)
 
 
@@ -135,7 +135,8 @@ def _fresh(what: str, name: str, t: Optional[torch.Tensor], shape, like: torch.T
 
 
 def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, grow: Union[int, torch.Tensor] = 0, *, table_out: Optional[torch.Tensor] = None,
-               lens_out: Optional[torch.Tensor] = None, refs: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+               lens_out: Optional[torch.Tensor] = None, refs: Optional[torch.Tensor] = None, grown: Optional[torch.Tensor] = None,
+               status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Row ``r`` of the new table goes on with row ``parents[r]`` of the old one (int32, at most 4096; -1: the row is empty) and gets
     room for ``grow`` more positions (an int for all rows, or int32 ``[rows]``): ``(table, lens + grow, refs)``, where ``refs`` int32
     ``[pages]`` says how many rows name a page.  Rows that nobody continues are freed with what they alone held.
@@ -143,7 +144,10 @@ def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent
     Full pages are shared.  A begun page that a growing row shares with others is copied, its written positions in all layers;
     where all its holders grow, the lowest row keeps it.  New pages are the lowest free ones, in the order of the rows.  A row for
     which there is no page, or no column in the table, keeps its length and latches ``NO_PAGES``; a page or parent that does not
-    exist latches ``BAD_PAGE``.  The outputs must not share memory with the inputs."""
+    exist latches ``BAD_PAGE``.  The outputs must not share memory with the inputs.
+
+    The last position of a row that did not grow may lie on a page that other rows read: nothing is to be stored there.  ``grown`` int32
+    ``[rows]`` gets the row's number where the row grew and -1 elsewhere, which is what ``rope_append`` takes as ``rows``."""
     what = "fork_pages"
     base, sizes, row = _pool(what, kv, table, lens)
     n, width, pages = parents.numel(), sizes[6], sizes[1]
@@ -158,12 +162,14 @@ def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent
     table_out = _fresh(what, "table_out", table_out, (n, width), table, table, lens, parents, each)
     lens_out = _fresh(what, "lens_out", lens_out, (n,), table, table, lens, parents, each, table_out)
     refs = _fresh(what, "refs", refs, (pages,), table, table, lens, parents, each, table_out, lens_out)
+    if grown is not None:
+        _fresh(what, "grown", grown, (n,), table, table, lens, parents, each, table_out, lens_out, refs)
     device = same_cuda_device(what, {kv.get_device(), table.get_device(), lens.get_device(), parents.get_device(), table_out.get_device(), lens_out.get_device(),
-                                     refs.get_device()}, each, status)
+                                     refs.get_device()}, each, grown, status)
     scratch = table.new_empty(3 * pages + 3 * n + 1)
     on_device(device, lib().nexrt_page_fork, _PAGES.pack(
         _PAGES.size, base, table.data_ptr(), lens.data_ptr(), parents.data_ptr(), address(each), table_out.data_ptr(), lens_out.data_ptr(), refs.data_ptr(), 0, 0,
-        scratch.data_ptr(), address(status), row, table_out.stride()[0], *sizes, n, 0 if each is not None else grow, 0), what)
+        scratch.data_ptr(), address(status), address(grown), row, table_out.stride()[0], *sizes, n, 0 if each is not None else grow, 0), what)
     return table_out, lens_out, refs
 
 
@@ -183,7 +189,7 @@ def compact_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, 
     scratch = table.new_empty(5 * pages + 1)
     on_device(device, lib().nexrt_page_compact, _PAGES.pack(
         _PAGES.size, base, table.data_ptr(), lens.data_ptr(), 0, 0, table_out.data_ptr(), 0, refs.data_ptr(), remap.data_ptr(), live.data_ptr(), scratch.data_ptr(),
-        address(status), row, table_out.stride()[0], *sizes, 0, 0, 0), what)
+        address(status), 0, row, table_out.stride()[0], *sizes, 0, 0, 0), what)
     return table_out, refs, remap, live
 
 
@@ -198,14 +204,16 @@ def copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *, status
     check_status(what, status)
     device = same_cuda_device(what, {kv.get_device(), src.get_device(), dst.get_device()}, status)
     scratch = src.new_empty(3 * src.numel() + 2 * sizes[1])
-    on_device(device, lib().nexrt_page_copy, _PAGES.pack(_PAGES.size, base, src.data_ptr(), dst.data_ptr(), 0, 0, 0, 0, 0, 0, 0, scratch.data_ptr(), address(status), 1, 0, *sizes, 0, 0, 0), what)
+    on_device(device, lib().nexrt_page_copy, _PAGES.pack(_PAGES.size, base, src.data_ptr(), dst.data_ptr(), 0, 0, 0, 0, 0, 0, 0, scratch.data_ptr(), address(status), 0, 1, 0, *sizes, 0, 0, 0), what)
 
 
 class PagedCache:
     """Pool, table, lengths and status word of a batch, at fixed addresses (a captured step stays valid).
 
-    One decode step: ``fork(parents, 1)`` - or ``fork(grow=1)`` to go on with every row -, then for every layer ``append`` (the new
-    tokens' positions are ``lens - 1``) and ``attend``.  ``check()`` waits for the device and raises what the kernels latched."""
+    One decode step: ``fork(parents, 1)`` - or ``fork(grow=1)`` to go on with every row -, then for every layer ``append`` with the
+    positions ``lens - 1`` and the rows ``grown``, and ``attend``.  ``grown`` int32 ``[rows]`` is what the last fork left: the row's
+    number where the row grew, -1 where it was freed, did not ask for room or found none, so that nothing is stored for it.  ``check()``
+    waits for the device and raises what the kernels latched."""
 
     def __init__(self, layers: int, pages: int, kv_heads: int, slots: int, dim: int, rows: int, max_len: int, dtype: torch.dtype = torch.bfloat16,
                  device: Union[str, torch.device] = "cuda"):
@@ -218,13 +226,14 @@ class PagedCache:
         self.refs = torch.zeros(pages, **i32)
         self.status = torch.zeros(1, **i32)
         self.same = torch.arange(rows, **i32)
+        self.grown = torch.full((rows,), -1, **i32)
 
     def fork(self, parents: Optional[torch.Tensor] = None, grow: Union[int, torch.Tensor] = 0) -> None:
         """``fork_pages`` on the cache's own table: every row of it goes on with one of its rows, or is freed (-1)."""
         parents = self.same if parents is None else parents
         if parents.shape != self.lens.shape:
             raise ValueError("PagedCache.fork: one parent for every row of the cache")
-        table, lens, _ = fork_pages(self.kv, self.table, self.lens, parents, grow, refs=self.refs, status=self.status)
+        table, lens, _ = fork_pages(self.kv, self.table, self.lens, parents, grow, refs=self.refs, grown=self.grown, status=self.status)
         self.table.copy_(table)
         self.lens.copy_(lens)
 

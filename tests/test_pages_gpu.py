@@ -373,3 +373,48 @@ def test_load_kv_under_another_default_type():
     cache.check()
     got = cache.kv[0][:, cache.table[0].long()].reshape(2, 8, 64)[:, :6]
     assert torch.equal(got[0], k[0]) and torch.equal(got[1], -k[0])
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_rows_that_grew(seed):
+    """``grown`` names the rows that got their positions: not those that are freed, bad, did not ask, or found no page or column."""
+    r = random.Random(50 + seed)
+    page, rows, width = r.choice([1, 4, 7]), r.choice([5, 31, 200]), r.randint(1, 6)
+    pages = max(4, rows * width // 3)
+    table, lens = random_rows(r, rows, width, pages, page)
+    parents = [r.choice([-1, rows + 3, r.randrange(rows), r.randrange(rows), r.randrange(rows)]) for _ in range(rows)]
+    grow = [r.choice([-2, 0, 1, 1, page + 1]) for _ in range(rows)]
+    kv = torch.zeros(1, 2, pages, 1, page, 64, dtype=torch.bfloat16, device=DEV)
+    grown = torch.full((rows + 2,), 77, dtype=torch.int32, device=DEV)
+    t, l, _ = fork_pages(kv, ints(table), ints(lens), ints(parents), ints(grow), grown=grown[1 : rows + 1])
+    before = [lens[p] if 0 <= p < rows else 0 for p in parents]
+    assert grown.tolist() == [77] + [i if n > b else -1 for i, (n, b) in enumerate(zip(l.tolist(), before))] + [77]
+    fork_pages(kv, ints(table), ints(lens), ints([]), 0, grown=ints([]))
+    with pytest.raises(ValueError, match="shares memory"):
+        fork_pages(kv, ints(table), l, ints(parents), 0, grown=l)
+
+
+@pytest.mark.parametrize("n", [6, 4])
+def test_a_row_without_a_page_leaves_the_others_alone(n):
+    """Two rows go on with one prompt that ends inside a page (6 positions of 4 a page), or fills its page; there is a page for one of them.  What the
+    step stores for the other would lie on a position of the prompt that both read.  A third row is freed, which is no fault."""
+    cache = PagedCache(2, 2, 1, 4, 64, 3, 40)
+    inv = torch.zeros(0, device=DEV)
+    line = lambda v: torch.tensor([float(x) for x in v], device=DEV)[:, None, None].expand(-1, 1, 64).to(torch.bfloat16)  # noqa: E731
+    cache.fork(grow=ints([n, 0, 0]))
+    for layer in range(2):
+        cache.append(layer, line(range(n)), line(range(n)), line(range(n)), ints(range(n)), ints([0] * n), inv)
+    cache.fork(ints([0, 0, -1]), 0)
+    assert cache.grown.tolist() == [-1, -1, -1]
+    cache.check()
+    cache.fork(ints([0, 1, -1]), 1)
+    assert cache.lens.tolist() == [n + 1, n, 0] and cache.grown.tolist() == [0, -1, -1]
+    assert int(cache.status) == Status.NO_PAGES
+    cache.status.zero_()
+    for layer in range(2):
+        cache.append(layer, line([50, 60, 70]), line([50, 60, 70]), line([50, 60, 70]), cache.lens - 1, cache.grown, inv)
+    cache.check()                                                              # the freed row and the one that waits latch nothing
+    for layer in range(2):
+        for row, want in ((0, [*range(n), 50]), (1, [*range(n)])):
+            got = cache.kv[layer][:, cache.table[row, : -(-len(want) // 4)].long(), 0, :, 0].reshape(2, -1)[:, : len(want)]
+            assert got.tolist() == [want, want]
