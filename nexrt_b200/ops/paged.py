@@ -213,7 +213,7 @@ class PagedCache:
     One decode step: ``fork(parents, 1)`` - or ``fork(grow=1)`` to go on with every row -, then for every layer ``append`` with the
     positions ``lens - 1`` and the rows ``grown``, and ``attend``.  ``grown`` int32 ``[rows]`` is what the last fork left: the row's
     number where the row grew, -1 where it was freed, did not ask for room or found none, so that nothing is stored for it.  ``check()``
-    waits for the device and raises what the kernels latched."""
+    waits for the device and raises what the kernels latched, once: the cache goes on with a clean status."""
 
     def __init__(self, layers: int, pages: int, kv_heads: int, slots: int, dim: int, rows: int, max_len: int, dtype: torch.dtype = torch.bfloat16,
                  device: Union[str, torch.device] = "cuda"):
@@ -261,5 +261,6 @@ class PagedCache:
     def check(self) -> None:
         code = int(self.status.item())
         if code:
+            self.status.zero_()
             names = {v: k for k, v in vars(Status).items() if isinstance(v, int)}
             raise KernelError(f"paged cache: {names.get(code, code)}")

@@ -418,3 +418,19 @@ def test_a_row_without_a_page_leaves_the_others_alone(n):
         for row, want in ((0, [*range(n), 50]), (1, [*range(n)])):
             got = cache.kv[layer][:, cache.table[row, : -(-len(want) // 4)].long(), 0, :, 0].reshape(2, -1)[:, : len(want)]
             assert got.tolist() == [want, want]
+
+
+def test_a_cache_goes_on_after_a_raised_status():
+    """The status keeps the first code: one that stayed would hide what comes later."""
+    cache = PagedCache(1, 2, 1, 4, 64, 2, 40)
+    cache.fork(grow=4)
+    cache.fork(grow=1)
+    with pytest.raises(KernelError, match="NO_PAGES"):
+        cache.check()
+    cache.check()
+    cache.fork(ints([0, -1]), 1)
+    cache.check()
+    assert cache.lens.tolist() == [5, 0]
+    cache.fork(ints([7, 0]))
+    with pytest.raises(KernelError, match="BAD_PAGE"):
+        cache.check()
