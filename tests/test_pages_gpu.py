@@ -434,3 +434,29 @@ def test_a_cache_goes_on_after_a_raised_status():
     cache.fork(ints([7, 0]))
     with pytest.raises(KernelError, match="BAD_PAGE"):
         cache.check()
+
+
+def test_the_documented_step():
+    """The README's order: room for a prompt, its keys and values, a fork, then append and attend in every layer; a freed row among them."""
+    from nexrt_b200.ops.rope import rope_frequencies
+
+    L, layers, W = 11, 3, 8
+    cache = PagedCache(layers=layers, pages=64, kv_heads=2, slots=4, dim=64, rows=W, max_len=64)
+    inv, scale = rope_frequencies(32, 1e7)
+    cache.fork(grow=ints([L] + [0] * (W - 1)))
+    state = torch.randn(layers, 2, 2, L, 64, device=DEV).to(torch.bfloat16)
+    for layer in range(layers):
+        cache.load_kv(layer, 0, state[layer, 0], state[layer, 1])
+    for parents in ([0] * 7 + [-1], [3, 3, 2, 0, 5, 5, -1, 0]):
+        cache.fork(ints(parents), grow=1)
+        for layer in range(layers):
+            q, k, v = (torch.randn(W, n, 64, device=DEV) for n in (4, 2, 2))
+            q = cache.append(layer, q, k, v, cache.lens - 1, cache.grown, inv.cuda(), scale=scale)
+            y = cache.attend(layer, q, softcap=0.0, window=0, slopes=None)
+            assert y.shape == (W, 4, 64) and torch.isfinite(y).all()
+    cache.check()
+    assert cache.lens.tolist() == [L + 2] * 6 + [0, L + 2]
+    for layer in range(layers):
+        for row in (0, 5, 7):
+            got = cache.kv[layer][:, cache.table[row, :4].long()].transpose(1, 2).reshape(2, 2, 16, 64)[:, :, :L]
+            assert torch.equal(got, state[layer])
