@@ -265,7 +265,7 @@ typedef struct NexrtReorderArgs {
     const void* rows;
     void* status;
     int64_t rows_0, rows_1;
-    int cols, n, n_in, tensors;
+    int cols, n, n_in, tensors, clear, reserved;      /* clear: a row that does not exist becomes zeros, else it is left as it was */
     const void* in[16];                               /* out[t][i] = in[t][rows[i]] */
     void* out[16];
     int64_t in_row[16], out_row[16], bytes[16];       /* bytes between rows, and of a row */

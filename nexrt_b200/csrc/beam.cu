@@ -643,10 +643,14 @@ struct ReorderArgs {
     int width[kReorderTensors];              // 16, 4 or 1 bytes a access
     const int* rows;
     int64_t r_0, r_1;
-    int cols, n, n_in, tensors;
+    int cols, n, n_in, tensors, clear;
     int* status;
 };
 
+template <typename V> __device__ __forceinline__ void clear_piece(char* dst, int64_t begin, int64_t bytes) {
+    const int64_t end = begin + kReorderPiece < bytes ? begin + kReorderPiece : bytes;
+    for (int64_t o = begin + threadIdx.x * sizeof(V); o < end; o += kReorderThreads * sizeof(V)) *reinterpret_cast<V*>(dst + o) = V{};
+}
 template <typename V> __device__ __forceinline__ void copy_piece(const char* src, char* dst, int64_t begin, int64_t bytes) {
     constexpr int kSteps = 4;
     const int64_t end = begin + kReorderPiece < bytes ? begin + kReorderPiece : bytes;
@@ -677,13 +681,18 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
         int t = 0;
         while (p >= a.first[t + 1]) ++t;
         const int row = a.rows[i / a.cols * a.r_0 + i % a.cols * a.r_1];
+        char* dst = a.out[t] + i * a.out_stride[t];
+        const int64_t begin = (p - a.first[t]) * kReorderPiece;
         if (row < 0 || row >= a.n_in) {
             if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, static_cast<int>(kStatusBadPage));
+            if (a.clear) {
+                if (a.width[t] == 16) clear_piece<uint4>(dst, begin, a.bytes[t]);
+                else if (a.width[t] == 4) clear_piece<uint32_t>(dst, begin, a.bytes[t]);
+                else clear_piece<uint8_t>(dst, begin, a.bytes[t]);
+            }
             continue;
         }
         const char* src = a.in[t] + row * a.in_stride[t];
-        char* dst = a.out[t] + i * a.out_stride[t];
-        const int64_t begin = (p - a.first[t]) * kReorderPiece;
         if (a.width[t] == 16) copy_piece<uint4>(src, dst, begin, a.bytes[t]);
         else if (a.width[t] == 4) copy_piece<uint32_t>(src, dst, begin, a.bytes[t]);
         else copy_piece<uint8_t>(src, dst, begin, a.bytes[t]);
@@ -745,7 +754,7 @@ extern "C" int nexrt_reorder_rows(const NexrtReorderArgs* x, void* stream) {
         a.width[t] = all % 16 == 0 ? 16 : (all % 4 == 0 ? 4 : 1);
         a.first[t + 1] = a.first[t] + (a.bytes[t] + kReorderPiece - 1) / kReorderPiece;
     }
-    a.rows = static_cast<const int*>(x->rows); a.r_0 = x->rows_0; a.r_1 = x->rows_1; a.cols = x->cols; a.n = x->n; a.n_in = x->n_in; a.tensors = x->tensors;
+    a.rows = static_cast<const int*>(x->rows); a.r_0 = x->rows_0; a.r_1 = x->rows_1; a.cols = x->cols; a.n = x->n; a.n_in = x->n_in; a.tensors = x->tensors; a.clear = x->clear;
     a.status = static_cast<int*>(x->status);
     const int64_t units = a.first[x->tensors] * x->n, most = 8ll * sm_count();
     if (units == 0) return 0;

@@ -20,7 +20,7 @@ MAX_BEAMS = 256
 MAX_VOCAB = 1 << 24
 _TENSORS = 16                                   # of one launch of the reorder kernel
 _BEAM = struct.Struct("Q8P6q8i")                # NexrtBeamArgs
-_REORDER = struct.Struct("Q2P2q4i32P48q")       # NexrtReorderArgs
+_REORDER = struct.Struct("Q2P2q6i32P48q")       # NexrtReorderArgs
 _BOOL = torch.bool
 
 
@@ -75,7 +75,8 @@ def _row_stride(what: str, t: torch.Tensor) -> int:
 def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Optional[Sequence[torch.Tensor]] = None, status: Optional[torch.Tensor] = None) -> List[torch.Tensor]:
     """``out[t][i] = tensors[t][rows[i]]`` for all tensors (any type, rows dense) in one launch per sixteen of them; ``rows`` is int32,
     one- or two-dimensional (the columns of ``beam_select``'s that go on), and may name a row several times.  ``out`` must not share
-    memory with ``tensors``: keep two sets and change places.  A row that does not exist is left as it was and latches ``BAD_PAGE``."""
+    memory with ``tensors``: keep two sets and change places.  A row that does not exist is left as it was, zeros where ``out`` is not given,
+    and latches ``BAD_PAGE``."""
     what = "reorder_rows"
     r_shape, r_s = rows.shape, rows.stride()
     if rows.dtype is not I32 or len(r_shape) not in (1, 2):
@@ -84,7 +85,8 @@ def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Op
     if not tensors:
         return []
     n_in = tensors[0].shape[0] if tensors[0].dim() else 0
-    if out is None:
+    clear = out is None
+    if clear:
         out = [t.new_empty((n, *t.shape[1:])) for t in tensors]
     if len(out) != len(tensors):
         raise ValueError(f"{what}: one out for every tensor")
@@ -120,5 +122,5 @@ def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Op
         columns = []
         for column in zip(*part):
             columns += [*column, *none]
-        on_device(device, lib().nexrt_reorder_rows, _REORDER.pack(_REORDER.size, rows.data_ptr(), address(status), r0, r1, cols, n, n_in, len(part), *columns), what)
+        on_device(device, lib().nexrt_reorder_rows, _REORDER.pack(_REORDER.size, rows.data_ptr(), address(status), r0, r1, cols, n, n_in, len(part), clear, 0, *columns), what)
     return list(out)

@@ -348,3 +348,14 @@ def test_rows_at_every_start(dtype, off, V):
     wide = torch.full((V + 16,), 1000.0, device=DEV, dtype=dtype)
     wide[off : off + V] = x[0, 0]
     check(wide[off : off + V].view(1, 1, V), s, min(V, 12))
+
+
+@pytest.mark.parametrize("n_in", [3, 0])
+def test_rows_that_do_not_exist_are_zeros_of_a_new_tensor(n_in):
+    torch.full((1 << 20,), 7.0, device=DEV)                                     # what the allocator gives out next is not zeros
+    xs = [torch.ones(n_in, *s, device=DEV).to(t) for s, t in (((100,), torch.float32), ((7,), torch.int8), ((3, 5), torch.float16), ((40000,), torch.bfloat16), ((), torch.int64))]
+    status = ints([0])
+    got = reorder_rows(xs, ints([0, 3, -1, 2]), status=status)
+    want = [float(0 <= r < n_in) for r in (0, 3, -1, 2)]
+    assert all(torch.equal(g.double().flatten(1) if g.dim() > 1 else g.double()[:, None], torch.tensor(want, device=DEV, dtype=torch.float64)[:, None].expand(4, max(1, g[0].numel()))) for g in got)
+    assert int(status) == Status.BAD_PAGE
