@@ -215,7 +215,7 @@ typedef struct NexrtRopeArgs {
     uint64_t size;
     const void *q, *k, *v, *positions, *rows;
     void *q_out, *k_pages, *v_pages;
-    const void *table, *inv_freq, *q_norm, *k_norm;   /* table NULL: q alone, kv_heads 0 */
+    const void *table, *inv_freq, *q_norm, *k_norm;   /* rows NULL: q alone, kv_heads 0 */
     void* status;
     int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head, page, head, slot, table_row;
     int tokens, q_heads, kv_heads, dim, rotary, interleaved, table_rows, width, slots, pages, in_type, out_type;

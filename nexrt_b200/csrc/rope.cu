@@ -372,7 +372,7 @@ using namespace nexrt;
 
 extern "C" int nexrt_rope_append(const NexrtRopeArgs* x, void* stream) {
     if (x->size != sizeof(*x)) return cudaErrorInvalidValue;
-    const bool paged = x->table != nullptr;
+    const bool paged = x->rows != nullptr;      // (a table without entries has no address)
     if (x->tokens < 0 || x->q_heads < 0 || x->kv_heads < 0 || x->dim < 8 || x->dim > 256 || x->dim % 8 || x->rotary < 0 || x->rotary > x->dim || x->rotary % 2) return cudaErrorInvalidValue;
     if (paged ? (x->slots < 1 || x->width < 0 || x->pages < 0 || x->table_rows < 0) : x->kv_heads != 0) return cudaErrorInvalidValue;
     if (x->tokens == 0 || x->q_heads + x->kv_heads == 0) return 0;

@@ -135,3 +135,21 @@ def test_pool_strides_and_offsets_beyond_32_bits():
     rope_append(x, x, x, pos, row, kp, vp, table, inv)
     near(kp[69, :, page - 1], formula(x, pos, inv)[0])
     assert torch.equal(vp[69, :, page - 1], x[0]) and float(wide[69, :, : page - 1].float().abs().sum()) == 0.0
+
+
+@pytest.mark.parametrize("shape", [(0, 4), (3, 0), (0, 0)])
+def test_append_with_a_table_without_entries(shape):
+    """Padding is rotated as ever; a token that names a row has no page."""
+    kv = torch.zeros(2, 3, 1, 4, 64, dtype=torch.bfloat16, device=DEV)
+    x = torch.randn(2, 1, 64, device=DEV).to(torch.bfloat16)
+    pos, inv = torch.tensor([0, 3], dtype=torch.int32, device=DEV), rope_frequencies(16, 1e4)[0].to(DEV)
+    table = torch.zeros(*shape, dtype=torch.int32, device=DEV)
+    for rows, code in (([-1, -1], 0), ([0, -1], Status.BAD_PAGE)):
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        out = rope_append(x, x, x, pos, torch.tensor(rows, dtype=torch.int32, device=DEV), kv[0], kv[1], table, inv, status=status)
+        near(out, formula(x, pos, inv))
+        assert int(status) == code and not kv.any()
+    none = torch.zeros(2, 0, 1, 4, 64, dtype=torch.bfloat16, device=DEV)          # and so has one of a pool without pages
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    near(rope_append(x, x, x, pos, pos * 0, none[0], none[1], torch.zeros(1, 2, dtype=torch.int32, device=DEV), inv, status=status), formula(x, pos, inv))
+    assert int(status) == Status.BAD_PAGE
