@@ -37,7 +37,7 @@ __host__ __device__ __forceinline__ int pages_of(int len, int page) { return len
 constexpr int kChunk = 64;
 constexpr int kItemCost = 3;
 
-// Keys [lo, hi) that the query behind the last of `len` keys sees; `room` keys have a place in the table.
+// Keys [lo, hi) that the query behind the last of `len` keys sees; `room` keys have a place in the table, and a longer row ends with them.
 __host__ __device__ __forceinline__ void key_span(int len, int64_t room, int window, int& lo, int& hi) {
     hi = len < 0 ? 0 : (len > room ? static_cast<int>(room) : len);
     lo = window > 0 && hi > window ? hi - window : 0;

@@ -46,7 +46,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Scores are ``q.k * scale`` (default ``dim ** -0.5``), then ``softcap * tanh(s / softcap)`` if it is not zero, then
     ``s - slopes[head] * distance`` if ``slopes`` (fp32 ``[heads]``) is given.  A row without keys gives zeros and an lse of -inf, and so
     does one whose scores are all -inf.  Returns ``out [rows, heads, dim]``, with ``return_lse`` also fp32 ``[rows, heads]``: the natural
-    logarithm of the sum of exp of the scores.  Keys on a page that the table does not name count as masked and latch ``BAD_PAGE``."""
+    logarithm of the sum of exp of the scores.  Keys on a page that the table does not name count as masked and latch ``BAD_PAGE``.  A
+    length beyond the table's columns is cut to them, here as in the calls below, and latches ``BAD_PAGE``: window and distances count
+    from the last position that has a place."""
     what = "paged_attention"
     kind, shape, q_s = q.dtype, q.shape, q.stride()
     if len(shape) != 3 or kind not in _POOL_TYPES or q_s[2] != 1:
@@ -144,7 +146,8 @@ def fork_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, parent
     Full pages are shared.  A begun page that a growing row shares with others is copied, its written positions in all layers;
     where all its holders grow, the lowest row keeps it.  New pages are the lowest free ones, in the order of the rows.  A row for
     which there is no page, or no column in the table, keeps its length and latches ``NO_PAGES``; a page or parent that does not
-    exist latches ``BAD_PAGE``.  The outputs must not share memory with the inputs.
+    exist latches ``BAD_PAGE``, and so does a length beyond the table's columns, which is cut to them.  Where a row finds no page, the rows
+    behind it that want one find none either.  The outputs must not share memory with the inputs.
 
     The last position of a row that did not grow may lie on a page that other rows read: nothing is to be stored there.  ``grown`` int32
     ``[rows]`` gets the row's number where the row grew and -1 elsewhere, which is what ``rope_append`` takes as ``rows``."""
@@ -194,8 +197,10 @@ def compact_pages(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, 
 
 
 def copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *, status: Optional[torch.Tensor] = None) -> None:
-    """Page ``src[i]`` to page ``dst[i]`` in all layers (int32, one list each).  A negative entry is left out; one beyond the pool latches
-    ``BAD_PAGE``.  A target that is also a source is left out, of a target given twice only the last counts; both latch ``PAGE_CONFLICT``."""
+    """Page ``src[i]`` to page ``dst[i]`` in all layers (int32, one list each).  A copy with a negative entry, or of a page to itself, is left out;
+    one with an entry beyond the pool is too and latches ``BAD_PAGE``.  A copy to a page that is also a source is left out, of those to one
+    page only the last counts (if it is left out, none); both latch ``PAGE_CONFLICT``.  Copies that are left out for an entry beyond the pool
+    still count as naming their other page."""
     what = "copy_pages"
     for t in (src, dst):
         if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() != src.numel():

@@ -287,3 +287,18 @@ def test_infinities_and_nan_in_fp16(keys):
     want = formula(q[1:2], clean, table[1:2], lens[1:2])
     check(out[1:2], lse[1:2], want[:2] + formula(q[1:2], kv.nan_to_num(neginf=0.0, posinf=0.0), table[1:2], lens[1:2])[2:])
     assert torch.isnan(out[2:]).all() and torch.isnan(lse[2:]).all()
+
+
+def test_a_length_that_is_cut_moves_the_window_and_the_distances():
+    """A row longer than its table is the row that ends with the table's last column."""
+    q, kv, table, lens = build([640, 40], 4, 2, 128, 16, torch.bfloat16, seed=2)
+    table = table[:, :40].contiguous()
+    slopes = torch.tensor([0.5, 0.1, 0.0, 1.0], device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for n in (641, 700, 2**31 - 1):
+        status.zero_()
+        long = torch.tensor([n, 40], dtype=torch.int32, device=DEV)
+        got = paged_attention(q, kv[0], kv[1], table, long, window=100, slopes=slopes, return_lse=True, status=status)
+        want = paged_attention(q, kv[0], kv[1], table, lens, window=100, slopes=slopes, return_lse=True)
+        assert int(status) == Status.BAD_PAGE and all(torch.equal(a, b) for a, b in zip(got, want))
+    check(*want, formula(q, kv, table, lens, window=100, slopes=slopes))
