@@ -2,7 +2,8 @@
 
 The engine's head samples one sequence (``head.py``); these entry points rank the continuations of several beams of several
 requests.  The rows that ``beam_select`` returns go to ``ops.paged.fork_pages`` (pages of the cache) and to ``reorder_rows``
-(recurrent states, conv histories, whatever has one row per beam).
+(recurrent states, conv histories, whatever has one row per beam).  For inference: tensors that require a gradient are refused, unless
+gradients are off.
 """
 
 from __future__ import annotations
@@ -12,7 +13,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
-from .lib import address, check_status, load as lib, on_device, same_cuda_device
+from .lib import address, check_status, inference_only, load as lib, on_device, same_cuda_device
 from .rope import F32, I32, TYPES
 
 MAX_K = 64
@@ -53,6 +54,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, finished:
             raise ValueError(f"{what}: finished is bool [requests, beams], with an end token of the vocabulary")
         f_s = finished.stride()
     check_status(what, status)
+    inference_only(what, logits, scores)
     device = same_cuda_device(what, {logits.get_device(), scores.get_device()}, finished, status)
     best, rows, tokens = scores.new_empty(batch, k), scores.new_empty(batch, k, dtype=I32), scores.new_empty(batch, k, dtype=I32)
     if batch:
@@ -91,6 +93,7 @@ def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Op
     if len(out) != len(tensors):
         raise ValueError(f"{what}: one out for every tensor")
     check_status(what, status)
+    inference_only(what, *tensors, *out)
     moves, spans = [], []
     for t, o in zip(tensors, out):
         t_shape, o_shape = t.shape, o.shape

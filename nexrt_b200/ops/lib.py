@@ -241,6 +241,14 @@ def same_cuda_device(what: str, devices: set, *optional: Optional[torch.Tensor])
     return device
 
 
+def inference_only(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """A ``ValueError`` where a gradient would be lost without a word: the operators for batches have no backward pass."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
 def check_status(what: str, status: Optional[torch.Tensor]) -> None:
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
         raise ValueError(f"{what}: status is one int32")

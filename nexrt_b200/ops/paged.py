@@ -7,7 +7,8 @@ names, row by row, the page of positions ``[slots * j, slots * (j + 1))``; behin
 names it within its length.
 
 Everything is planned on the device: no call waits for the host, all of them can be captured into a CUDA graph.  What a kernel
-finds wrong (a page that does not exist, a full pool) is left out and latched in ``status`` (``runtime/control.py: Status``).
+finds wrong (a page that does not exist, a full pool) is left out and latched in ``status`` (``runtime/control.py: Status``).  The calls
+are for inference: they refuse tensors that require a gradient, unless gradients are off.
 """
 
 from __future__ import annotations
@@ -19,7 +20,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ..runtime.control import Status
-from .lib import KernelError, address, check_status, load as lib, on_device, same_cuda_device, sm_count
+from .lib import KernelError, address, check_status, inference_only, load as lib, on_device, same_cuda_device, sm_count
 from .rope import F32, I32, TYPES, rope_append
 
 HEAD_DIMS = (64, 128, 192, 256)
@@ -77,6 +78,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if slopes is not None and (slopes.dtype is not F32 or slopes.shape != (heads,) or not slopes.is_contiguous()):
         raise ValueError(f"{what}: slopes is fp32 [heads]")
     check_status(what, status)
+    inference_only(what, q, k_pages, v_pages, slopes, out)
     if out is None:
         out, o_s = q.new_empty(rows, heads, dim), (heads * dim, dim)
     else:
@@ -100,6 +102,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 def _pool(what: str, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor):
     """Base of the pool; planes, pages, heads, slots, bytes of a slot, rows and width of the table; its row stride."""
+    inference_only(what, kv)
     shape = kv.shape
     if len(shape) != 6 or shape[1] != 2 or not kv.is_contiguous():
         raise ValueError(f"{what}: kv is a contiguous [layers, 2, pages, kv heads, slots, dim]")

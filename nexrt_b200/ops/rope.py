@@ -3,7 +3,7 @@ sequences, in one launch.  The decode kernels of the engine rotate in their own 
 these entry points are for batches over a paged cache (``ops/paged.py``) and for models with another layout or scaling.
 
 Pair ``i`` of a head at position ``p`` turns by ``p * inv_freq[i]``; ``scale`` multiplies cos and sin.  The angle is formed in
-64 bits, so far positions lose nothing.
+64 bits, so far positions lose nothing.  For inference: tensors that require a gradient are refused, unless gradients are off.
 """
 
 from __future__ import annotations
@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from .lib import address, check_status, load as lib, on_device, same_cuda_device
+from .lib import address, check_status, inference_only, load as lib, on_device, same_cuda_device
 
 I32, F32 = torch.int32, torch.float32
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -87,6 +87,7 @@ def rope(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, in
          eps: float = 1e-6, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``q [tokens, heads, dim]`` at ``positions`` int32 ``[tokens]``, rotated (after an RMSNorm with the multiplier ``norm``, if given); ``out`` may be ``q``."""
     tokens, heads, dim, rotary, q_s = _common("rope", q, positions, inv_freq, (norm,))
+    inference_only("rope", q, inv_freq, norm, out)
     out, o_s = _out("rope", out, q, tokens, heads, dim, q.dtype)
     device = same_cuda_device("rope", {q.get_device(), positions.get_device(), inv_freq.get_device(), out.get_device()}, norm)
     if tokens and heads:
@@ -127,6 +128,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     if table.dtype is not I32 or len(t_shape) != 2 or t_s[1] != 1:
         raise ValueError(f"{what}: table is int32 [rows, pages of a row] with contiguous rows")
     check_status(what, status)
+    inference_only(what, q, k, v, k_pages, v_pages, inv_freq, q_norm, k_norm, out)
     out, o_s = _out(what, out, q, tokens, hq, dim, pool_kind)
     device = same_cuda_device(what, {q.get_device(), k.get_device(), v.get_device(), positions.get_device(), rows.get_device(), k_pages.get_device(), v_pages.get_device(),
                                      table.get_device(), inv_freq.get_device(), out.get_device()}, q_norm, k_norm, status)

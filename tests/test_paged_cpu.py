@@ -231,3 +231,30 @@ def test_frequencies():
                 lambda: rope_frequencies(64, 1e4, "linear", 0.5), lambda: rope_frequencies(0, 1e4)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_gradients_are_not_lost_without_a_word():
+    """Nothing here has a backward pass: a tensor that requires a gradient is refused, and taken as any other where gradients are off (here: until
+    its device is looked at)."""
+    kv, table, lens, one = torch.zeros(1, 2, 4, 2, 16, 64), _i32(3, 4), _i32(3), torch.zeros(3, 2, 64)
+    bf = kv.to(torch.bfloat16)
+    need = lambda t: t.clone().requires_grad_()  # noqa: E731
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    append = dict(q=one, k=one, v=one, positions=lens, rows=lens, k_pages=bf[0, 0], v_pages=bf[0, 1], table=table, inv_freq=torch.zeros(8), q_norm=torch.ones(64), k_norm=torch.ones(64))
+    attend = dict(q=q, k_pages=bf[0, 0], v_pages=bf[0, 1], table=table, lens=lens, slopes=torch.ones(4))
+    turn = dict(q=one, positions=lens, inv_freq=torch.zeros(8), norm=torch.ones(64))
+    pick = dict(logits=torch.zeros(2, 3, 10), scores=torch.zeros(2, 3), k=3)
+    calls = [(rope_append, append, n) for n in ("q", "k", "v", "k_pages", "v_pages", "inv_freq", "q_norm", "k_norm")]
+    calls += [(paged_attention, attend, n) for n in ("q", "k_pages", "v_pages", "slopes")] + [(rope, turn, n) for n in ("q", "inv_freq", "norm")]
+    calls += [(beam_select, pick, n) for n in ("logits", "scores")]
+    calls += [(fork_pages, dict(kv=bf, table=table, lens=lens, parents=lens), "kv"), (compact_pages, dict(kv=bf, table=table, lens=lens), "kv"), (copy_pages, dict(kv=bf, src=lens, dst=lens), "kv")]
+    for call, args, name in calls:
+        args = dict(args, **{name: need(args[name])})
+        with pytest.raises(ValueError, match="backward"):
+            call(**args)
+        with torch.no_grad(), pytest.raises(ValueError, match="CPU"):
+            call(**args)
+    with pytest.raises(ValueError, match="backward"):
+        reorder_rows([need(one)], _i32(2))
+    with pytest.raises(ValueError, match="backward"):
+        reorder_rows([one], _i32(2), out=[need(torch.zeros(2, 2, 64))])
