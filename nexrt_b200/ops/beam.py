@@ -105,6 +105,8 @@ def reorder_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, *, out: Op
             src, dst, src_row, dst_row = t.data_ptr(), o.data_ptr(), size, size
             if not o.is_contiguous():
                 dst_row = _row_stride(what, o)
+                if n > 1 and dst_row < size:
+                    raise ValueError(f"{what}: rows of out lie over one another")
             if n_in and not t.is_contiguous():
                 src_row = _row_stride(what, t)
             moves.append((src, dst, src_row, dst_row, size))

@@ -83,8 +83,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out, o_s = q.new_empty(rows, heads, dim), (heads * dim, dim)
     else:
         o_s = out.stride()
-        if out.shape != shape or out.dtype is not kind or o_s[2] != 1:
-            raise ValueError(f"{what}: out is like q")
+        if out.shape != shape or out.dtype is not kind or o_s[2] != 1 or (o_s[0] == 0 and rows > 1) or (o_s[1] == 0 and heads > 1):
+            raise ValueError(f"{what}: out is like q, each head in a place of its own")
     lse = q.new_empty(rows, heads, dtype=F32) if return_lse else None
     device = same_cuda_device(what, {q.get_device(), k_pages.get_device(), v_pages.get_device(), table.get_device(), lens.get_device(), out.get_device()}, slopes, status)
     if rows:
@@ -130,6 +130,8 @@ def _fresh(what: str, name: str, t: Optional[torch.Tensor], shape, like: torch.T
         return like.new_empty(*shape)        # (ints cost half of what a tuple does)
     if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or (t.numel() and t.stride(-1) != 1) or (t.dim() == 1 and not t.is_contiguous()):
         raise ValueError(f"{what}: {name} is int32 {list(shape)} with contiguous rows")
+    if t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{what}: rows of {name} lie over one another")
     begin, end = _span(t)
     for o in old:
         if o is not None and end:

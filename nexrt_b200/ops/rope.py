@@ -78,8 +78,8 @@ def _out(what, out, q, tokens, heads, dim, kind):
     if out is None:
         return q.new_empty(tokens, heads, dim) if q.dtype is kind else q.new_empty(tokens, heads, dim, dtype=kind), (heads * dim, dim)
     strides = out.stride()
-    if out.shape != (tokens, heads, dim) or out.dtype is not kind or strides[2] != 1:
-        raise ValueError(f"{what}: out is [tokens, heads, dim] of {kind} with a contiguous last dimension")
+    if out.shape != (tokens, heads, dim) or out.dtype is not kind or strides[2] != 1 or (strides[0] == 0 and tokens > 1) or (strides[1] == 0 and heads > 1):
+        raise ValueError(f"{what}: out is [tokens, heads, dim] of {kind} with a contiguous last dimension, each head in a place of its own")
     return out, strides
 
 

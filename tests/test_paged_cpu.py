@@ -258,3 +258,23 @@ def test_gradients_are_not_lost_without_a_word():
         reorder_rows([need(one)], _i32(2))
     with pytest.raises(ValueError, match="backward"):
         reorder_rows([one], _i32(2), out=[need(torch.zeros(2, 2, 64))])
+
+
+def test_outputs_whose_rows_lie_over_one_another_are_refused():
+    kv, table, lens = torch.zeros(1, 2, 4, 1, 16, 64, dtype=torch.bfloat16), _i32(3, 4), _i32(3)
+    q, kp = torch.zeros(3, 4, 64, dtype=torch.bfloat16), torch.zeros(5, 2, 16, 64, dtype=torch.bfloat16)
+    one = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    flat = _i32(20)
+    append = lambda out: rope_append(q, one, one, lens, lens, kp, kp, table, torch.zeros(8), out=out)  # noqa: E731
+    for call in (lambda: fork_pages(kv, table, lens, lens, table_out=flat[:4].expand(3, 4)),
+                 lambda: fork_pages(kv, table, lens, lens, table_out=flat.as_strided((3, 4), (3, 1))),
+                 lambda: compact_pages(kv, table, lens, table_out=flat[:4].expand(3, 4)),
+                 lambda: paged_attention(q, kp, kp, table, lens, out=q[:1].clone().expand(3, 4, 64)),
+                 lambda: paged_attention(q, kp, kp, table, lens, out=q[:, :1].clone().expand(3, 4, 64)),
+                 lambda: rope(q, lens, torch.zeros(8), out=q[:1].clone().expand(3, 4, 64)),
+                 lambda: append(q[:, :1].clone().expand(3, 4, 64)),
+                 lambda: reorder_rows([torch.zeros(4, 6)], lens, out=[torch.zeros(1, 6).expand(3, 6)])):
+        with pytest.raises(ValueError, match="over one another|place of its own"):
+            call()
+    with pytest.raises(ValueError, match="CPU"):                                  # one row may have any stride
+        fork_pages(kv, table, lens, lens[:1], table_out=flat.as_strided((1, 4), (0, 1)))
