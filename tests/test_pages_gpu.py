@@ -460,3 +460,46 @@ def test_the_documented_step():
         for row in (0, 5, 7):
             got = cache.kv[layer][:, cache.table[row, :4].long()].transpose(1, 2).reshape(2, 2, 16, 64)[:, :, :L]
             assert torch.equal(got, state[layer])
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_every_row_after_every_step(seed):
+    """The walk of a cache by its documented step (positions ``lens - 1``, rows ``grown``) in a pool that runs full: after each step all rows read back
+    their own tokens in all layers, and each status is the one that the step earns."""
+    r = random.Random(200 + seed)
+    page, rows, width, layers = r.choice([1, 3, 8]), 7, 6, 2
+    cache = PagedCache(layers, r.choice([20, 30]), 2, page, 64, rows, width * page)
+    inv, tokens, counter, full = torch.zeros(0, device=DEV), [[] for _ in range(rows)], 0, 0
+    for step in range(80):
+        parents = [r.choice([i, i, i, r.randrange(rows), -1]) for i in range(rows)]
+        grow = [r.choice([0, 1, 1, 1]) for _ in range(rows)]
+        cache.fork(ints(parents), ints(grow))
+        lens, grown = cache.lens.tolist(), cache.grown.tolist()
+        old, tokens = tokens, []
+        for i, p in enumerate(parents):
+            before = list(old[p]) if p >= 0 else []
+            assert grown[i] == (i if lens[i] > len(before) else -1) and lens[i] - len(before) in (0, grow[i])
+            tokens.append(before + ([counter + i] if grown[i] >= 0 else []))
+        short = any(p >= 0 and g > 0 and n < 0 for p, g, n in zip(parents, grow, grown))
+        assert int(cache.status) == (Status.NO_PAGES if short else 0), step
+        cache.status.zero_()
+        full += short
+        number = torch.arange(counter, counter + rows, device=DEV) % 199
+        for layer in range(layers):
+            x = (number + layer).float()[:, None, None].expand(-1, 2, 64).to(torch.bfloat16).contiguous()
+            x[:, 1] += 1
+            cache.append(layer, x, x, -x, cache.lens - 1, cache.grown, inv)
+        counter += rows
+        if r.random() < 0.2:
+            live = int(cache.compact())
+            assert live == int((cache.refs > 0).sum()) and not cache.refs[live:].any()
+        assert int(cache.status) == 0, step
+        table, refs = cache.table.tolist(), cache.refs.tolist()
+        assert refs == [held(table, lens, page).get(p, 0) for p in range(len(refs))]
+        pool = cache.kv[..., 0].float().cpu()                                  # [layers, 2, pages, heads, slots]
+        for i in range(rows):
+            for j, t in enumerate(tokens[i]):
+                for layer in range(layers):
+                    want = [float(t % 199 + layer + h) for h in range(2)]
+                    assert pool[layer, :, table[i][j // page], :, j % page].tolist() == [want, [-w for w in want]], (step, i, j)
+    assert full > 5 or page > 1                                                # (of one position a page the pool runs out all the time)
