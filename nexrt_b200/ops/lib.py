@@ -243,10 +243,8 @@ def same_cuda_device(what: str, devices: set, *optional: Optional[torch.Tensor])
 
 def inference_only(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """A ``ValueError`` where a gradient would be lost without a word: the operators for batches have no backward pass."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled() and torch._C._any_requires_grad(*tensors):      # 0.5 us for nine tensors, a loop over them 0.9
+        raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 def check_status(what: str, status: Optional[torch.Tensor]) -> None:
