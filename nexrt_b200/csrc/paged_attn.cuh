@@ -20,8 +20,9 @@
 // numerator, and where that key's value is near zero they are the result.  So there exp(s_j - m) is formed against a reference of the
 // row that goes down as well as up, the same in numerator and sum, and the largest weight of a tile lies between 2^6 and 2^15; weights of the
 // same tile below 2^-13, which the pair does not hold to 2^-12, go through the value product once more against a lower reference.  32-bit sums
-// hold the maximum 60 binary orders above the reference.  It costs nothing with 128 dims (ragged batch 93 us), 4 % with 64 (64 sequences of 2000 keys
-// 36.9 -> 38.4), 12 % where a steep bias moves the reference in every tile (the ragged batch with cap and bias 79 -> 88).
+// hold the maximum 60 binary orders above the reference.  It costs 2 % under sustained load with 128 dims (ragged batch
+// 98.8 -> 101.1 us), 3 % with 64 (64 sequences of 2000 keys 37.3 -> 38.3), 12 % where a steep bias moves the reference in every tile (the
+// ragged batch with cap and bias 80 -> 90).
 //
 // An item that lies in one CTA's range is written at once; of one that is cut, each CTA leaves its part (at most two parts a
 // CTA) and a second kernel joins them in the order of the keys: results do not depend on timing (they do, in the last bits, on where the
@@ -112,8 +113,8 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 // reference lies more than kRefSpan below the highest so far.
 constexpr float kRefLeast = 6.f, kRefMost = 15.f;
 constexpr int kRefPlace = 11, kRefSpan = 45;
-// Whether fp16 holds a weight too coarsely (below 2^-13), and it is large enough to be held better (above 2^-70).
-__device__ __forceinline__ bool is_low(float p) { return __float_as_uint(p) - 0x1c800000u < 0x39000000u - 0x1c800000u; }
+// A weight that fp16 holds too coarsely, and one that is too small to matter, in binary orders above the reference.
+constexpr float kLow = -13.f, kNothing = -70.f;
 // The logarithm of l 2^ref.  (fp16: l may be 2^70, and its logarithm's last bits would be as large as those of a far larger result.)
 template <typename T> __device__ __forceinline__ float log_of(float ref, float l) {
     if (l == 0.f) return -INFINITY;
@@ -438,39 +439,60 @@ __global__ void __launch_bounds__(kPaThreads, resident_ctas(D)) paged_attn_kerne
                     }
                     if (!(have >> key & 1)) v[u] = -INFINITY;
                 }
-                float m = max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3]));
-                bool stays = false;                                    // the references of all rows g + 8 r
-                if constexpr (kHalf) {
-                    const uint32_t above = __ballot_sync(0xffffffffu, !(m <= mx[r] + kRefMost)), there = __ballot_sync(0xffffffffu, m >= mx[r] + kRefLeast);
-                    const uint32_t pairs = there | there >> 1;
-                    stays = above == 0 && ((pairs | pairs >> 2) & 0x11111111u) == 0x11111111u;
-                }
-                corr[r] = 1.f;
-                if (!stays) {
+                auto row_max = [&](float m) {
                     m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                    if constexpr (kHalf) {
-                        // (a whole number, so that differences of references are exact; a row without a key in this tile keeps its own)
-                        const bool fits = m <= mx[r] + kRefMost && (m >= mx[r] + kRefLeast || m == -INFINITY);
-                        m = fits ? mx[r] : rintf(max_nan(m - kRefPlace, highest[r] - kRefSpan));
-                        highest[r] = max_nan(highest[r], m);
-                    } else {
-                        m = max_nan(m, mx[r]);
-                    }
-                    if (mx[r] != m) corr[r] = exp2_ftz(mx[r] - (m == -INFINITY ? 0.f : m));
-                    mx[r] = m;
-                }
-                const float shift = mx[r] == -INFINITY ? 0.f : mx[r];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = exp2_ftz(v[u] - shift);
-                sum[r] = fmaf(sum[r], corr[r], (v[0] + v[1]) + (v[2] + v[3]));
-                if (kHalf && __any_sync(0xffffffffu, is_low(v[0]) || is_low(v[1]) || is_low(v[2]) || is_low(v[3]))) {
-                    again |= 1 << r;
+                    return max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                };
+                corr[r] = 1.f;
+                if constexpr (kHalf) {
+                    // as a rule the references of all rows g + 8 r stay and no weight has to wait: that is looked up beside the exponentials
+                    float p[4];
+                    bool low = false;
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        low_s[kHalf ? warp : 0][kHalf ? r * 4 + u : 0][lane] = is_low(v[u]) ? v[u] : 0.f;
-                        if (is_low(v[u])) v[u] = 0.f;
+                        p[u] = v[u] - mx[r];
+                        low |= p[u] < kLow && p[u] > kNothing;
                     }
+                    const float m = max_nan(max_nan(p[0], p[1]), max_nan(p[2], p[3]));
+                    const uint32_t above = __ballot_sync(0xffffffffu, !(m <= kRefMost) || low), there = __ballot_sync(0xffffffffu, m >= kRefLeast), pairs = there | there >> 1;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) p[u] = exp2_ftz(p[u]);
+                    if (above != 0 || ((pairs | pairs >> 2) & 0x11111111u) != 0x11111111u) {
+                        // (a whole number, so that differences of references are exact; a row without a key in this tile keeps its own)
+                        const float top = row_max(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])));
+                        const bool fits = top <= mx[r] + kRefMost && (top >= mx[r] + kRefLeast || top == -INFINITY);
+                        const float ref = fits ? mx[r] : rintf(max_nan(top - kRefPlace, highest[r] - kRefSpan)), shift = ref == -INFINITY ? 0.f : ref;
+                        highest[r] = max_nan(highest[r], ref);
+                        if (mx[r] != ref) corr[r] = exp2_ftz(mx[r] - shift);
+                        mx[r] = ref;
+                        low = false;
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            p[u] = v[u] - shift;
+                            low |= p[u] < kLow && p[u] > kNothing;
+                        }
+                        const bool waits = __any_sync(0xffffffffu, low);
+                        if (waits) again |= 1 << r;
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const bool late = p[u] < kLow && p[u] > kNothing;
+                            p[u] = exp2_ftz(p[u]);
+                            v[u] = late ? 0.f : p[u];
+                            if (waits) low_s[warp][r * 4 + u][lane] = late ? p[u] : 0.f;
+                        }
+                        sum[r] = fmaf(sum[r], corr[r], (p[0] + p[1]) + (p[2] + p[3]));
+                    } else {
+                        sum[r] += (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) v[u] = p[u];
+                    }
+                } else {
+                    const float m = max_nan(row_max(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3]))), mx[r]), shift = m == -INFINITY ? 0.f : m;
+                    if (mx[r] != m) corr[r] = exp2_ftz(mx[r] - shift);
+                    mx[r] = m;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) v[u] = exp2_ftz(v[u] - shift);
+                    sum[r] = fmaf(sum[r], corr[r], (v[0] + v[1]) + (v[2] + v[3]));
                 }
                 split2(v[0], v[1], ph[r][0], pl[r][0], T());
                 split2(v[2], v[3], ph[r][1], pl[r][1], T());
