@@ -29,7 +29,7 @@
 // batch's lengths cut an item).
 //
 // Measured: 200K keys, 2 key heads of 256, 32 query heads: 75 us, 5.4 TB/s of keys and values, 0.84 of copy rate (the rings alone fill in
-// 64); 48 sequences of 0 to 16384 keys, 8 heads of 128: 93 us, 0.86; 16 sequences of up to
+// 64); 48 sequences of 0 to 16384 keys, 8 heads of 128, fp16: 93 us, 0.86; 16 sequences of up to
 // 4097 keys, 8 heads of 64, capped and biased: 16 us; one sequence of 1100 keys: 9.2 us, two launches and their chains.
 #pragma once
 
@@ -734,7 +734,9 @@ template <typename T, int D> static int paged_launch(const PagedAttnArgs& a, boo
     if (e || !join) return e;
     const int rows = a.group < kPaRows ? a.group : kPaRows, items = a.seqs * a.kv_heads * a.head_groups;
     // items cut into dozens of parts are few and want many threads (200K keys in 148 parts: 75.5 us, with 256 threads 80.3), items cut once
-    // or twice are many and want many CTAs (a ragged batch 91.9, with 1024 threads where it may 95.0; 1100 keys 9.2 and 10.0)
+    // or twice are many and want many CTAs (a ragged batch 91.9, with 1024 threads where it may 95.0; 1100 keys 9.2 and 10.0).  Between them the
+    // line is a matter of a microsecond, and it depends on the dims (4 heads on one, 256 and 1024 threads: 9 sequences of 4000 keys, 33 parts each,
+    // of 128 dims 10.6 and 11.6 us, of 256 dims 15.7 and 15.5; 2 of 4000, 66 parts, 9.3 and 8.9, 11.7 and 10.9)
     if (a.by_item && a.grid >= 32 * items) return launch(paged_join_kernel<T, D, 1024>, dim3(items, rows), dim3(1024), 0, st, a);
     return launch(paged_join_kernel<T, D, 256>, dim3(a.by_item ? items : a.grid, rows), dim3(256), 0, st, a);
 }

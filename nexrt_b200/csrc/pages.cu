@@ -7,7 +7,7 @@
 // the table names; the lowest go first, to the rows in their order.
 //
 // Bound by the bytes of the copied pages; for a table without copies by the launches and the plan's few round trips.  Measured: 360
-// pages of 15 layers (708 MB both ways) compacted in 124 us, 0.88 of copy rate; eight beams of 8191 keys forked in 9.8 us, 128 of up to
+// pages of 15 layers (708 MB both ways) compacted in 124 us, 0.88 of copy rate; eight beams of 8191 keys forked in 9.6 us, 128 of up to
 // 20000 in 15, 4096 of 300 in 51.
 #include "api.h"
 #include "paged.cuh"
@@ -17,8 +17,9 @@ namespace nexrt {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanRows = 4096;         // rows whose plan one CTA holds in shared memory
 constexpr int kPagesPerThread = 8;
-// Rows up to which each searches the others for holders of its begun page; of more they are counted page by page (forks on the device, searched
-// and counted: 8 rows 9.7 and 10.0 us, 128 rows of 8 a page 12.5 and 10.6, 4096 rows 548 and 51).
+// Rows up to which each searches the others for holders of its begun page; of more they are counted page by page (forks of 300 positions, eight
+// rows a prompt, searched and counted: 8 rows 7.4 and 7.5 us, 32 rows 9.2 and 9.3, 64 rows 9.0 and 8.9, 96 rows 9.5 and 9.3, 256 rows 13.4 and
+// 11.5, 4096 rows 548 and 51: the line may lie anywhere up to 64).
 constexpr int kSearchRows = 32;
 // Entries of a table that the planning CTA counts itself (8 rows of 130 entries: a fork 14.4 -> 9.6 us on the device; a CTA takes
 // about 1 us a thousand entries, a launch and a memset 5 us).

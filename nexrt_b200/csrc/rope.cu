@@ -13,7 +13,7 @@
 // squares is two to four shuffles for several heads at once; sums and products go two values an instruction.
 //
 // Measured: 4099 tokens of 36 heads of 256 (151 MB) 34 us, 0.69 of copy rate: 130 instructions a head keep the schedulers half busy, with
-// four warps each to hide their latencies (six CTAs an SM have to spill: 37 us).  Eight tokens of six heads: 3.9 us, the chain from
+// four warps each to hide their latencies (six CTAs an SM have to spill: 37 us).  Eight tokens of six heads: 4.1 us, the chain from
 // the position to the stores.
 #include "api.h"
 #include "paged.cuh"
