@@ -4,7 +4,8 @@
 //
 // in 64 bits; equal totals go to the lower beam, then to the larger logit, then to the lower token.  A finished beam has one candidate, its
 // end token at its own score.  What is not 64 bits are the exponentials and the sums of 16 or 32 of them: a row's logarithm is off by
-// 1e-7 as a rule, by 1e-6 at worst, and beams whose totals are nearer than that may change places.  Beams that hold the same numbers tie to the
+// 1e-7 as a rule, at worst by a few 1e-6 (where values 16 below the maximum make up the sum: each is off by up to 2.5 units of 2^-24 of its
+// distance), and beams whose totals are nearer than that may change places.  Beams that hold the same numbers tie to the
 // last bit: which values meet in a partial sum goes by their tokens, never by the address of the row.
 //
 // Within a beam the order of the totals is that of the logits, so one pass over a slice of a row gives everything that is

@@ -33,7 +33,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, finished:
 
     The total of a candidate is the beam's score plus the logit's log-softmax, added in 64 bits; equal totals go to the lower beam, then
     to the larger logit, then to the lower token.  A row's log of the sum of exp comes from 32-bit exponentials and is off by 1e-7 as a
-    rule, by 1e-6 at worst: candidates of different beams that are nearer than that may change places; beams with the same logits and the
+    rule, at worst by a few 1e-6: candidates of different beams that are nearer than that may change places; beams with the same logits and the
     same score always tie.  A beam marked in ``finished`` (bool ``[requests, beams]``) has one candidate, token
     ``eos`` at its own score.  Where fewer than ``k`` candidates are above -inf the rest are at -inf.  A beam with a NaN or +inf among its
     logits, or as its score, has no candidate and latches ``NON_FINITE`` in ``status``."""

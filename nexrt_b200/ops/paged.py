@@ -47,9 +47,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Scores are ``q.k * scale`` (default ``dim ** -0.5``), then ``softcap * tanh(s / softcap)`` if it is not zero, then
     ``s - slopes[head] * distance`` if ``slopes`` (fp32 ``[heads]``) is given.  A row without keys gives zeros and an lse of -inf, and so
     does one whose scores are all -inf.  Returns ``out [rows, heads, dim]``, with ``return_lse`` also fp32 ``[rows, heads]``: the natural
-    logarithm of the sum of exp of the scores.  Keys on a page that the table does not name count as masked and latch ``BAD_PAGE``.  A
+    logarithm of the sum of exp of the scores.  An infinite value that a row sees makes that dim of its result NaN or infinite.  Keys on a page that the table does not name count as masked and latch ``BAD_PAGE``.  A
     length beyond the table's columns is cut to them, here as in the calls below, and latches ``BAD_PAGE``: window and distances count
-    from the last position that has a place."""
+    from the last position that has a place.  ``out`` may be ``q``."""
     what = "paged_attention"
     kind, shape, q_s = q.dtype, q.shape, q.stride()
     if len(shape) != 3 or kind not in _POOL_TYPES or q_s[2] != 1:
@@ -252,7 +252,7 @@ class PagedCache:
 
     def load_kv(self, layer: int, row: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Install ``k, v [kv heads][positions][dim]`` (already normalised and rotated, as ``DecodeEngine.export_state`` gives them) as the first
-        positions of ``row``, which has room for them (``fork`` with ``grow``)."""
+        positions of ``row``, which has room for them (``fork`` with ``grow``).  Rows that share its pages read them too."""
         if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or not 0 <= row < self.lens.numel():
             raise ValueError("PagedCache.load_kv: k and v are [kv heads, positions, dim] for a row of the cache")
         k, v = k.transpose(0, 1), v.transpose(0, 1)

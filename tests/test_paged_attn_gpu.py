@@ -302,3 +302,27 @@ def test_a_length_that_is_cut_moves_the_window_and_the_distances():
         want = paged_attention(q, kv[0], kv[1], table, lens, window=100, slopes=slopes, return_lse=True)
         assert int(status) == Status.BAD_PAGE and all(torch.equal(a, b) for a, b in zip(got, want))
     check(*want, formula(q, kv, table, lens, window=100, slopes=slopes))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_infinite_values_stay_in_their_dim(dtype, dim):
+    q, kv, table, lens = build([40, 700, 700], 8, 2, dim, 16, dtype, seed=8)
+    want = formula(q, kv, table, lens)
+    bad = kv.clone()
+    bad[1][table[0, 1].long(), 0, 3, 5] = math.inf
+    bad[1][table[1, 30].long(), 1, 0, 6] = -math.inf
+    bad[1][table[1, 31].long(), 1, 9, 7] = math.nan
+    out, lse = paged_attention(q, bad[0], bad[1], table, lens, return_lse=True)
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[0, :4, 5] = hit[1, 4:, 6] = hit[1, 4:, 7] = True
+    assert not torch.isfinite(out[hit]).any() and torch.isfinite(out[~hit]).all()
+    check(torch.where(hit, want[0].to(dtype), out), lse, want)
+
+
+def test_the_result_may_take_the_place_of_q():
+    """Items cut over many CTAs, whole ones and rows without keys."""
+    for keys in ([50000], [3000, 0, 3, 70, 1000], [40] * 300):
+        q, kv, table, lens = build(keys, 20, 2, 128, 16, torch.bfloat16, seed=5)
+        want = paged_attention(q, kv[0], kv[1], table, lens)
+        assert paged_attention(q, kv[0], kv[1], table, lens, out=q) is q and torch.equal(q, want)
